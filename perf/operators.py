@@ -328,7 +328,7 @@ def _own(state):
     else:
         prefix, suffix = (state["prefix_k"], state["prefix_v"]), (state["suffix_k"], state["suffix_v"])
     return K.prefix_attention(state["q"], prefix, suffix, members=state["bounds"], prefix_lengths=state["prefix_lengths"],
-                              suffix_lengths=state["suffix_lengths"], causal=case["causal"])
+                              own_lengths=state["suffix_lengths"], causal=case["causal"])
 
 
 def run(state):
