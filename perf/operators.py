@@ -19,8 +19,8 @@ import torch
 
 own = False
 
-#: rows whose largest magnitude is below this are stored as zero
-TINY = 2.0 ** -90
+#: the magnitudes that a quantised cache holds: rows whose largest is below TINY are stored as zero, from HUGE on as NaN
+TINY, HUGE = 2.0 ** -50, 2.0 ** 40
 E4M3_MAX = 448.0
 
 
@@ -236,7 +236,7 @@ def _rotated(x, sine, cosine):
 def _encoded(x):
     """fp32 rows -> (e4m3 codes, fp32 scales) as a cache holds them"""
     largest = x.abs().amax(-1)
-    scale = torch.where(largest < TINY, 0.0, torch.where(largest.isfinite(), largest / E4M3_MAX, math.nan))
+    scale = torch.where(largest < TINY, 0.0, torch.where(largest < HUGE, largest / E4M3_MAX, math.nan))
     codes = (x / scale.unsqueeze(-1)).clamp(-E4M3_MAX, E4M3_MAX)
     return torch.where(scale.unsqueeze(-1) == 0, 0.0, codes).to(torch.float8_e4m3fn), scale
 
