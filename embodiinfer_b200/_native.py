@@ -25,10 +25,12 @@ LINEAR_SINGLE_CTA = 64
 LINEAR_PAIRS = 128
 LINEAR_CLUSTER = 256
 NORM_RESIDUAL_EVICT_LAST = 1
+ROPE_OWN_SPECTRUM = 1
+ATTENTION_CAUSAL = 1
 SCALE_SCRATCH_BYTES = 8
 STATIC_SCRATCH_BYTES = 16640
 STATIC_SCALE_MAX_COUNT = 67108864
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 _ERRORS = {
     E_INVALID: "invalid argument (null, non-positive size or misaligned pointer)",
@@ -89,7 +91,27 @@ class NormDesc(ctypes.Structure):
         "blocked", "gate", "inverse")] + [(name, ctypes.c_int32) for name in ("rows", "columns", "tokens", "bits", "flags")]
 
 
-_P, _I, _I64, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
+class KVCacheDesc(ctypes.Structure):
+    """``b2_kv_cache_desc``."""
+
+    _fields_ = [(name, ctypes.c_void_p) for name in (
+        "q", "q_out", "k", "v", "sine", "cosine", "k_codes", "k_scales", "v_codes", "v_scales", "offsets", "lengths")] + \
+        [(name, ctypes.c_int64 * 3) for name in ("q_stride", "k_stride", "v_stride")] + [("factor_batch_stride", ctypes.c_int64)] + \
+        [(name, ctypes.c_int32) for name in ("batch", "tokens", "heads", "kv_heads", "head_dim", "capacity")]
+
+
+class PrefixAttentionDesc(ctypes.Structure):
+    """``b2_prefix_attention_desc``."""
+
+    _fields_ = [(name, ctypes.c_void_p) for name in (
+        "q", "out", "prefix_k", "prefix_v", "prefix_k_scales", "prefix_v_scales", "own_k", "own_v", "own_k_scales", "own_v_scales",
+        "members", "prefix_lengths", "own_lengths", "status", "workspace")] + \
+        [("workspace_bytes", ctypes.c_int64), ("q_stride", ctypes.c_int64 * 3), ("scale", ctypes.c_float)] + \
+        [(name, ctypes.c_int32) for name in ("flags", "batch", "groups", "heads", "kv_heads", "queries", "head_dim", "prefix_capacity",
+                                             "own_capacity", "cache_bits")]
+
+
+_P, _I, _I64, _F, _D = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_double
 
 # name -> argtypes; every entry returns int.
 SIGNATURES: dict[str, list] = {
@@ -112,8 +134,13 @@ SIGNATURES: dict[str, list] = {
     "b2_attention": [_P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P],
     "b2_attention_fp8": [_P, _P, _P, _P, _F, _I, _I, _I, _I, _I, _P, _P],
     "b2_attention_nvfp4": [_P, _P, _P, _P, _P, _P, _F, _I, _I, _I, _I, _I, _P, _P],
+    "b2_rope_axes": [_P, _I, ctypes.POINTER(ctypes.c_int32), _I, _I64, _I, _D, _I, _P, _P, _P],
+    "b2_kv_cache_write": [ctypes.POINTER(KVCacheDesc), _P],
+    "b2_kv_cache_read": [ctypes.POINTER(KVCacheDesc), _P],
+    "b2_prefix_attention": [ctypes.POINTER(PrefixAttentionDesc), _P],
+    "b2_prefix_attention_workspace_bytes": [ctypes.POINTER(PrefixAttentionDesc)],
 }
-RESULT_TYPES = {"b2_linear_workspace_bytes": ctypes.c_int64}
+RESULT_TYPES = {"b2_linear_workspace_bytes": ctypes.c_int64, "b2_prefix_attention_workspace_bytes": ctypes.c_int64}
 
 _lock = threading.Lock()
 _library: ctypes.CDLL | None = None

@@ -15,6 +15,12 @@ int launch_rope_split(const void* qkv, const void* sine, const void* cosine, voi
 int launch_geglu(const void* gate, const void* up, void* output, void* scales, void* blocked, const void* scale,
                  int rows, int columns, int64_t row_stride, int bits, const void* table, int flags,
                  cudaStream_t stream);
+int launch_rope_axes(const void* positions, int position_bytes, const int32_t* sections, int axes, int64_t tokens, int head_dim,
+                     double theta, int own_spectrum, void* sine, void* cosine, cudaStream_t stream);
+int launch_kv_cache_write(const b2_kv_cache_desc* desc, cudaStream_t stream);
+int launch_kv_cache_read(const b2_kv_cache_desc* desc, cudaStream_t stream);
+int launch_prefix_attention(const b2_prefix_attention_desc* desc, cudaStream_t stream);
+int64_t prefix_attention_workspace(const b2_prefix_attention_desc* desc);
 int launch_norm_quant(const b2_norm_desc* desc, cudaStream_t stream);
 int launch_resize_frames(const void* frames, void* images, const void* row_bounds, const void* row_weights, int row_taps,
                          const void* column_bounds, const void* column_weights, int column_taps, int cameras, int height,
@@ -181,6 +187,106 @@ int b2_rope_split(const void* qkv, const void* sine, const void* cosine, void* q
     if (alignment & 15u) return B2_E_INVALID;
     return b2::launch_rope_split(qkv, sine, cosine, q_out, k_out, v_out, batch, tokens, heads, kv_heads, head_dim,
                                  factor_batch_stride, kv_capacity, kv_offset, static_cast<cudaStream_t>(stream));
+}
+
+int b2_rope_axes(const void* positions, int32_t position_bytes, const int32_t* sections, int32_t axes, int64_t tokens,
+                 int32_t head_dim, double theta, int32_t flags, void* sine, void* cosine, void* stream) {
+    if (positions == nullptr || sections == nullptr || sine == nullptr || cosine == nullptr) return B2_E_INVALID;
+    if (tokens <= 0 || head_dim <= 0 || (flags & ~B2_ROPE_OWN_SPECTRUM) || !(theta > 0.0) || theta > 1.0e300) return B2_E_INVALID;
+    if (position_bytes != 4 && position_bytes != 8) return B2_E_INVALID;
+    if (axes < 1 || axes > 4 || head_dim % 2 != 0 || head_dim > 1024) return B2_E_UNSUPPORTED;
+    int64_t sum = 0;
+    for (int a = 0; a < axes; ++a) {
+        if (sections[a] <= 0) return B2_E_INVALID;
+        sum += sections[a];
+    }
+    if (sum != head_dim / 2) return B2_E_INVALID;
+    if (!is_aligned(positions, position_bytes) || !is_aligned(sine, 4) || !is_aligned(cosine, 4)) return B2_E_INVALID;
+    if (tokens > (int64_t(1) << 40)) return B2_E_TOO_LARGE;
+    return b2::launch_rope_axes(positions, position_bytes, sections, axes, tokens, head_dim, theta, flags & B2_ROPE_OWN_SPECTRUM, sine,
+                                cosine, static_cast<cudaStream_t>(stream));
+}
+
+static bool strides_valid(const int64_t (&stride)[3]) {
+    for (const int64_t s : stride)
+        if (s < 0 || (s & 7) != 0 || s > (int64_t(1) << 40)) return false;
+    return true;
+}
+
+// What the write and the read of the quantised cache ask of a descriptor alike.
+static int check_kv_cache(const b2_kv_cache_desc* desc) {
+    if (desc == nullptr || desc->k == nullptr || desc->v == nullptr || desc->k_codes == nullptr || desc->k_scales == nullptr ||
+        desc->v_codes == nullptr || desc->v_scales == nullptr)
+        return B2_E_INVALID;
+    if (desc->batch <= 0 || desc->tokens <= 0 || desc->kv_heads <= 0 || desc->capacity <= 0 || desc->heads < 0) return B2_E_INVALID;
+    if (desc->head_dim != 128 && desc->head_dim != 256) return B2_E_UNSUPPORTED;
+    const void* vectors[] = {desc->q, desc->q_out, desc->k, desc->v, desc->sine, desc->cosine, desc->k_codes, desc->v_codes};
+    for (const void* pointer : vectors)
+        if (!is_aligned(pointer, 16)) return B2_E_INVALID;
+    const void* words[] = {desc->k_scales, desc->v_scales, desc->offsets, desc->lengths};
+    for (const void* pointer : words)
+        if (!is_aligned(pointer, 4)) return B2_E_INVALID;
+    if (!strides_valid(desc->k_stride) || !strides_valid(desc->v_stride)) return B2_E_INVALID;
+    const int64_t heads = desc->q == nullptr ? 0 : desc->heads, limit = (int64_t(1) << 31) - 1;
+    if (heads > limit / 4 || desc->kv_heads > limit / 4) return B2_E_TOO_LARGE;
+    if (int64_t(desc->batch) * desc->tokens > limit / (heads + 2 * int64_t(desc->kv_heads))) return B2_E_TOO_LARGE;
+    return B2_OK;
+}
+
+int b2_kv_cache_write(const b2_kv_cache_desc* desc, void* stream) {
+    const int status = check_kv_cache(desc);
+    if (status != B2_OK) return status;
+    if ((desc->q == nullptr) != (desc->q_out == nullptr) || (desc->sine == nullptr) != (desc->cosine == nullptr)) return B2_E_INVALID;
+    if (desc->q != nullptr && (desc->heads <= 0 || !strides_valid(desc->q_stride))) return B2_E_INVALID;
+    if (desc->factor_batch_stride < 0 || (desc->factor_batch_stride & 3) != 0) return B2_E_INVALID;
+    return b2::launch_kv_cache_write(desc, static_cast<cudaStream_t>(stream));
+}
+
+int b2_kv_cache_read(const b2_kv_cache_desc* desc, void* stream) {
+    const int status = check_kv_cache(desc);
+    if (status != B2_OK) return status;
+    if (desc->q != nullptr || desc->q_out != nullptr || desc->sine != nullptr || desc->cosine != nullptr) return B2_E_INVALID;
+    return b2::launch_kv_cache_read(desc, static_cast<cudaStream_t>(stream));
+}
+
+static int check_prefix_attention(const b2_prefix_attention_desc* desc) {
+    if (desc == nullptr || (desc->flags & ~B2_ATTENTION_CAUSAL)) return B2_E_INVALID;
+    if (desc->batch <= 0 || desc->groups <= 0 || desc->heads <= 0 || desc->kv_heads <= 0 || desc->queries <= 0) return B2_E_INVALID;
+    if (desc->prefix_capacity < 0 || desc->own_capacity < 0 || (desc->prefix_capacity == 0 && desc->own_capacity == 0)) return B2_E_INVALID;
+    if (desc->heads % desc->kv_heads != 0 || (desc->members == nullptr && desc->batch % desc->groups != 0)) return B2_E_INVALID;
+    if (desc->head_dim != 128 && desc->head_dim != 256) return B2_E_UNSUPPORTED;
+    if (desc->cache_bits != 8 && desc->cache_bits != 16) return B2_E_UNSUPPORTED;
+    // row numbers, key rows of a tensor map and CTAs are 32-bit in the kernel
+    const int64_t limit = int64_t(1) << 30;
+    if (int64_t(desc->batch) * desc->heads > limit / desc->queries) return B2_E_TOO_LARGE;
+    if (int64_t(desc->groups) * desc->kv_heads > limit / (int64_t(desc->prefix_capacity) + 64)) return B2_E_TOO_LARGE;
+    if (int64_t(desc->batch) * desc->kv_heads > limit / (int64_t(desc->own_capacity) + 64)) return B2_E_TOO_LARGE;
+    return B2_OK;
+}
+
+int64_t b2_prefix_attention_workspace_bytes(const b2_prefix_attention_desc* desc) {
+    return check_prefix_attention(desc) == B2_OK ? b2::prefix_attention_workspace(desc) : 0;
+}
+
+int b2_prefix_attention(const b2_prefix_attention_desc* desc, void* stream) {
+    const int status = check_prefix_attention(desc);
+    if (status != B2_OK) return status;
+    if (desc->q == nullptr || desc->out == nullptr || !(desc->scale > 0.0f) || desc->scale > 1.0e30f) return B2_E_INVALID;
+    if (desc->prefix_capacity > 0 && (desc->prefix_k == nullptr || desc->prefix_v == nullptr)) return B2_E_INVALID;
+    if (desc->own_capacity > 0 && (desc->own_k == nullptr || desc->own_v == nullptr)) return B2_E_INVALID;
+    if (desc->cache_bits == 8) {
+        if (desc->prefix_capacity > 0 && (desc->prefix_k_scales == nullptr || desc->prefix_v_scales == nullptr)) return B2_E_INVALID;
+        if (desc->own_capacity > 0 && (desc->own_k_scales == nullptr || desc->own_v_scales == nullptr)) return B2_E_INVALID;
+    }
+    const void* vectors[] = {desc->q, desc->out, desc->prefix_k, desc->prefix_v, desc->own_k, desc->own_v};
+    for (const void* pointer : vectors)
+        if (!is_aligned(pointer, 16)) return B2_E_INVALID;
+    const void* words[] = {desc->prefix_k_scales, desc->prefix_v_scales, desc->own_k_scales, desc->own_v_scales, desc->members,
+                           desc->prefix_lengths, desc->own_lengths, desc->status};
+    for (const void* pointer : words)
+        if (!is_aligned(pointer, 4)) return B2_E_INVALID;
+    if (!strides_valid(desc->q_stride) || !is_aligned(desc->workspace, 32)) return B2_E_INVALID;
+    return b2::launch_prefix_attention(desc, static_cast<cudaStream_t>(stream));
 }
 
 int b2_norm_quant(const b2_norm_desc* desc, void* stream) {

@@ -9,10 +9,12 @@ These are the calls the plan objects (``embodiinfer_b200.backend``) and the regi
 from __future__ import annotations
 
 import ctypes
+from contextlib import nullcontext
 
 import torch
 
 from . import _native as N
+from .kv_cache import QuantizedKVCache
 
 
 def _stream(device: torch.device) -> int:
@@ -37,6 +39,11 @@ def _require_cuda(*tensors: torch.Tensor | None) -> torch.device:
     if device is None:
         raise ValueError("no tensor operands")
     return device
+
+
+def _on(device: torch.device):
+    """The device's context, or none when it is already current (entering one costs more than the launch)."""
+    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def gelu_table_range(table: torch.Tensor) -> tuple[int, int]:
@@ -256,6 +263,184 @@ def rope_split(qkv: torch.Tensor, sine: torch.Tensor, cosine: torch.Tensor, q_ou
                                         v_out.data_ptr(), batch, tokens, heads, kv_heads, head_dim, stride, k_out.shape[2],
                                         kv_offset, _stream(device))
     N.check(status, "b2_rope_split")
+
+
+def rope_axes(positions: torch.Tensor, sections: tuple[int, ...], sine: torch.Tensor | None = None, cosine: torch.Tensor | None = None, *,
+              theta: float = 10000.0, own_spectrum: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    """Sine / cosine tables of rotary positions with several axes, see ``b2_rope_axes``: ``positions`` int32 or int64
+    [axes, ..., T] (contiguous), ``sections`` the number of frequencies of each axis (their sum is head_dim / 2).  Returns
+    fp32 (sine, cosine) [..., T, head_dim / 2], the factors of :func:`rope_split` and :func:`kv_cache_write`."""
+    device = _require_cuda(positions, sine, cosine)
+    if positions.dtype not in (torch.int32, torch.int64) or positions.ndim < 2 or not positions.is_contiguous():
+        raise ValueError("rope_axes requires contiguous int32 or int64 positions [axes, ..., tokens]")
+    axes, half = positions.shape[0], sum(sections)
+    if len(sections) != axes or any(type(section) is not int or section <= 0 for section in sections):
+        raise ValueError("rope_axes requires one positive section for each axis")
+    shape = (*positions.shape[1:], half)
+    if sine is None and cosine is None:
+        sine, cosine = (torch.empty(shape, device=device, dtype=torch.float32) for _ in range(2))
+    for table in (sine, cosine):
+        if table is None or table.dtype != torch.float32 or table.shape != shape or not table.is_contiguous():
+            raise ValueError("rope_axes requires contiguous fp32 tables [..., tokens, head_dim/2], both or neither")
+    tokens = positions.numel() // axes if axes else 0
+    if tokens == 0:
+        return sine, cosine
+    with _on(device):
+        status = N.load().b2_rope_axes(positions.data_ptr(), positions.element_size(), (ctypes.c_int32 * axes)(*sections), axes, tokens,
+                                       2 * half, float(theta), N.ROPE_OWN_SPECTRUM if own_spectrum else 0, sine.data_ptr(),
+                                       cosine.data_ptr(), _stream(device))
+    N.check(status, "b2_rope_axes")
+    return sine, cosine
+
+
+def _check_cache(cache: QuantizedKVCache, what: str) -> tuple[int, int, int, int]:
+    """The (batch, kv_heads, capacity, head_dim) of a quantised cache."""
+    shape = cache.k_codes.shape
+    if len(shape) != 4 or cache.v_codes.shape != shape or cache.k_scales.shape != shape[:3] or cache.v_scales.shape != shape[:3]:
+        raise ValueError(f"{what} requires codes [batch, kv_heads, capacity, head_dim] and scales [batch, kv_heads, capacity]")
+    for codes, scales in ((cache.k_codes, cache.k_scales), (cache.v_codes, cache.v_scales)):
+        if codes.element_size() != 1 or scales.dtype != torch.float32 or not codes.is_contiguous() or not scales.is_contiguous():
+            raise ValueError(f"{what} requires contiguous one-byte codes and contiguous fp32 scales")
+    return tuple(shape)
+
+
+def _check_whole(values: torch.Tensor | None, count: int, what: str) -> None:
+    if values is not None and (values.dtype != torch.int32 or values.shape != (count,) or not values.is_contiguous()):
+        raise ValueError(f"{what} must be a contiguous int32 tensor of {count} values")
+
+
+def _kv_cache_desc(rows: tuple[torch.Tensor, torch.Tensor], cache: QuantizedKVCache, offsets, lengths, what: str) -> "N.KVCacheDesc":
+    """The descriptor of a write or a read, without queries and tables; checks everything the two have in common."""
+    batch, kv_heads, capacity, head_dim = _check_cache(cache, what)
+    k, v = rows
+    if k.shape != v.shape or k.ndim != 4 or k.shape[0] != batch or k.shape[1] != kv_heads or k.shape[3] != head_dim:
+        raise ValueError(f"{what} requires keys and values [batch, kv_heads, tokens, head_dim] that fit the cache")
+    for row in rows:
+        if row.dtype != torch.bfloat16 or row.stride(3) != 1:
+            raise ValueError(f"{what} requires bf16 keys and values whose last dimension is contiguous")
+    _check_whole(offsets, batch, "offsets")
+    _check_whole(lengths, batch, "lengths")
+    return N.KVCacheDesc(
+        k=k.data_ptr(), v=v.data_ptr(), k_codes=cache.k_codes.data_ptr(), k_scales=cache.k_scales.data_ptr(),
+        v_codes=cache.v_codes.data_ptr(), v_scales=cache.v_scales.data_ptr(), offsets=_ptr(offsets), lengths=_ptr(lengths),
+        k_stride=k.stride()[:3], v_stride=v.stride()[:3], batch=batch, tokens=k.shape[2], kv_heads=kv_heads, head_dim=head_dim,
+        capacity=capacity)
+
+
+def kv_cache_write(k: torch.Tensor, v: torch.Tensor, cache: QuantizedKVCache, *, q: torch.Tensor | None = None,
+                   q_out: torch.Tensor | None = None, sine: torch.Tensor | None = None, cosine: torch.Tensor | None = None,
+                   offsets: torch.Tensor | None = None, lengths: torch.Tensor | None = None) -> None:
+    """Quantise keys and values [B, kv_heads, T, D] into ``cache`` at positions ``offsets[b] + t`` for ``t < lengths[b]``
+    (int32 [B]; default 0 and T); with ``sine`` / ``cosine`` (fp32 [T, D/2] or [B, T, D/2]) keys are rotated first, and the
+    rotated ``q`` [B, H, T, D] goes to ``q_out`` (contiguous).  k, v and q may be views of one packed projection.  See
+    ``b2_kv_cache_write``; padded tokens and positions outside the cache are passed over."""
+    device = _require_cuda(k, v, *cache, q, q_out, sine, cosine, offsets, lengths)
+    desc = _kv_cache_desc((k, v), cache, offsets, lengths, "kv_cache_write")
+    tokens, head_dim = k.shape[2], k.shape[3]
+    if (q is None) != (q_out is None) or (sine is None) != (cosine is None):
+        raise ValueError("kv_cache_write takes q with q_out, and sine with cosine")
+    if q is not None:
+        if q.dtype != torch.bfloat16 or q.ndim != 4 or q.shape[0] != k.shape[0] or q.shape[2:] != k.shape[2:] or q.stride(3) != 1:
+            raise ValueError("q must be bf16 [batch, heads, tokens, head_dim] with a contiguous last dimension")
+        if q_out.dtype != torch.bfloat16 or q_out.shape != q.shape or not q_out.is_contiguous():
+            raise ValueError("q_out must be a contiguous bf16 tensor of q's shape")
+        desc.q, desc.q_out, desc.heads, desc.q_stride = q.data_ptr(), q_out.data_ptr(), q.shape[1], q.stride()[:3]
+    if sine is not None:
+        for factor in (sine, cosine):
+            if factor.dtype != torch.float32 or not factor.is_contiguous() or factor.shape != sine.shape or \
+                    tuple(factor.shape) not in ((tokens, head_dim // 2), (k.shape[0], tokens, head_dim // 2)):
+                raise ValueError("kv_cache_write requires contiguous fp32 factors [tokens, head_dim/2] or [batch, tokens, head_dim/2]")
+        desc.sine, desc.cosine = sine.data_ptr(), cosine.data_ptr()
+        desc.factor_batch_stride = tokens * (head_dim // 2) if sine.ndim == 3 else 0
+    if k.numel() == 0 or desc.capacity == 0:
+        return
+    with _on(device):
+        status = N.load().b2_kv_cache_write(ctypes.byref(desc), _stream(device))
+    N.check(status, "b2_kv_cache_write")
+
+
+def kv_cache_read(cache: QuantizedKVCache, k_out: torch.Tensor, v_out: torch.Tensor, *, offsets: torch.Tensor | None = None,
+                  lengths: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Positions ``offsets[b] + t`` of ``cache`` as bf16 into row ``t`` of ``k_out`` / ``v_out`` [B, kv_heads, T, D], for
+    ``t < lengths[b]`` (defaults 0 and T); the other rows are left as they are.  See ``b2_kv_cache_read``."""
+    device = _require_cuda(*cache, k_out, v_out, offsets, lengths)
+    desc = _kv_cache_desc((k_out, v_out), cache, offsets, lengths, "kv_cache_read")
+    if k_out.numel() != 0 and desc.capacity != 0:
+        with _on(device):
+            status = N.load().b2_kv_cache_read(ctypes.byref(desc), _stream(device))
+        N.check(status, "b2_kv_cache_read")
+    return k_out, v_out
+
+
+def _cache_part(part, count: int, q: torch.Tensor, what: str) -> tuple[int, int, int, tuple]:
+    """(bits, kv_heads, capacity, the four pointers) of a prefix or own cache; bits 0 when there is none."""
+    if part is None:
+        return 0, 0, 0, (None, None, None, None)
+    if isinstance(part, QuantizedKVCache):
+        batch, kv_heads, capacity, head_dim = _check_cache(part, "prefix_attention")
+        bits, pointers = 8, (part.k_codes.data_ptr(), part.v_codes.data_ptr(), part.k_scales.data_ptr(), part.v_scales.data_ptr())
+    else:
+        k, v = part
+        if k.ndim != 4 or k.shape != v.shape or k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16 or not k.is_contiguous() or \
+                not v.is_contiguous():
+            raise ValueError("prefix_attention requires contiguous bf16 keys and values [n, kv_heads, capacity, head_dim], or quantised caches")
+        batch, kv_heads, capacity, head_dim = k.shape
+        bits, pointers = 16, (k.data_ptr(), v.data_ptr(), None, None)
+    if batch != count and count >= 0 or head_dim != q.shape[3]:
+        raise ValueError(f"prefix_attention: the {what} cache does not fit the queries")
+    return bits, kv_heads, capacity, pointers if capacity else (None, None, None, None)
+
+
+def prefix_attention(q: torch.Tensor, prefix, own=None, *, members: torch.Tensor | None = None, prefix_lengths: torch.Tensor | None = None,
+                     own_lengths: torch.Tensor | None = None, causal: bool = False, scale: float | None = None,
+                     out: torch.Tensor | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of a batch whose members share prefixes: ``q`` bf16 [B, H, T, D]; ``prefix`` holds one key/value cache for each
+    of G groups and ``own`` (or None) one for each batch element -- a pair (k, v) of bf16 tensors [G or B, kv_heads, capacity, D]
+    or a :class:`QuantizedKVCache`, both of one kind.  ``members`` int32 [G + 1]: group g is the batch elements
+    [members[g], members[g + 1]); default B / G each.  ``prefix_lengths`` int32 [G], ``own_lengths`` int32 [B]: default the
+    capacities.  ``causal``: query t sees all but the last T - 1 - t own keys.  ``scale`` defaults to 1 / sqrt(D).  Returns bf16
+    [B, H, T, D]; rows that see no key are zero.  See ``b2_prefix_attention``."""
+    parts = tuple(t for part in (prefix, own) if part is not None for t in part)
+    device = _require_cuda(q, *parts, members, prefix_lengths, own_lengths, out, status)
+    if q.ndim != 4 or q.dtype != torch.bfloat16 or q.stride(3) != 1:
+        raise ValueError("prefix_attention requires bf16 queries [batch, heads, tokens, head_dim] with a contiguous last dimension")
+    batch, heads, queries, head_dim = q.shape
+    if prefix is None:
+        raise ValueError("prefix_attention requires a prefix cache (its capacity may be 0)")
+    bits, kv_heads, prefix_capacity, prefix_pointers = _cache_part(prefix, -1, q, "prefix")
+    own_bits, own_kv_heads, own_capacity, own_pointers = _cache_part(own, batch, q, "own")
+    if own is not None and (own_bits != bits or own_kv_heads != kv_heads):
+        raise ValueError("prefix_attention requires prefix and own caches of one kind with equal kv_heads")
+    groups = prefix[0].shape[0]
+    _check_whole(members, groups + 1, "members")
+    _check_whole(prefix_lengths, groups, "prefix_lengths")
+    _check_whole(own_lengths, batch, "own_lengths")
+    if kv_heads == 0 or heads % kv_heads or groups == 0 or (members is None and batch % groups):
+        raise ValueError("prefix_attention requires heads divisible by kv_heads, and a batch divisible by the groups unless members is given")
+    if out is None:
+        out = torch.empty((batch, heads, queries, head_dim), device=device, dtype=torch.bfloat16)
+    elif out.shape != q.shape or out.dtype != torch.bfloat16 or not out.is_contiguous():
+        raise ValueError("attention output must be a contiguous bf16 tensor of the queries' shape")
+    if out.numel() == 0:
+        return out
+    if prefix_capacity == 0 and own_capacity == 0:
+        return out.zero_()
+    if status is None:
+        status = status_word(device)
+    desc = N.PrefixAttentionDesc(
+        q.data_ptr(), out.data_ptr(), *prefix_pointers[:2], *prefix_pointers[2:], *own_pointers[:2], *own_pointers[2:], _ptr(members),
+        _ptr(prefix_lengths), _ptr(own_lengths), status.data_ptr(), None, 0, q.stride()[:3], head_dim ** -0.5 if scale is None else scale,
+        N.ATTENTION_CAUSAL if causal else 0, batch, groups, heads, kv_heads, queries, head_dim, prefix_capacity, own_capacity, bits)
+    library = N.load()
+    with _on(device):
+        # scratch of this call alone (also inside a captured graph: it is the graph's own)
+        size = library.b2_prefix_attention_workspace_bytes(ctypes.byref(desc))
+        workspace = torch.empty(size, device=device, dtype=torch.uint8) if size else None
+        if size:
+            desc.workspace, desc.workspace_bytes = workspace.data_ptr(), size
+        code = library.b2_prefix_attention(ctypes.byref(desc), _stream(device))
+    N.check(code, "b2_prefix_attention")
+    return out
 
 
 def norm_quant(inputs: torch.Tensor, output: torch.Tensor, *, bits: int, tokens: int, scale: torch.Tensor | None = None,

@@ -21,7 +21,9 @@
 extern "C" {
 #endif
 
-/* 7: b2_attention_nvfp4.
+/* 8: the quantised key/value cache and attention over shared prefixes (b2_kv_cache_write, b2_kv_cache_read,
+ * b2_prefix_attention, b2_rope_axes).
+ * 7: b2_attention_nvfp4.
  * 6: launches of at most 128 tokens may run on the cluster schedule (weights as the MMA's "A" operand, K split across a
  * thread-block cluster; B2_LINEAR_CLUSTER asks for it whenever it applies, B2_LINEAR_SINGLE_CTA opts out);
  * b2_gelu_table_range returns ranges on multiples of eight codes; FP8 launches accept 32 features per tile;
@@ -31,7 +33,7 @@ extern "C" {
  * b2_linear_desc are rejected; the opt-in cluster split of K of version 3 (flag value 32) is gone.
  * 3: added the producers in front of the GEMMs (b2_norm_quant, b2_layer_norm_quant, b2_bhsd_quant, b2_normalize_frames,
  * b2_frames_to_patches, b2_resize_frames). */
-#define B2_ABI_VERSION 7
+#define B2_ABI_VERSION 8
 
 /* ---- status codes ---------------------------------------------------------- */
 #define B2_OK 0
@@ -241,6 +243,104 @@ int b2_attention_fp8(const void* q, const void* k, const void* v, void* codes, f
  * global scale (calibrated maximum / (448 * 6)), finite and positive. */
 int b2_attention_nvfp4(const void* q, const void* k, const void* v, void* codes, void* scales, void* blocked, float global_scale,
                        int32_t batch, int32_t heads, int32_t queries, int32_t keys, int32_t head_dim, void* status, void* stream);
+
+/* Sine / cosine tables of rotary positions with several axes (time, height, width of image patches and video frames; one axis
+ * gives the ordinary table): the factors that b2_rope_split, b2_linear_desc.rope and b2_kv_cache_write take.
+ *   positions  int32 (position_bytes 4) or int64 (8) [axes, tokens]; tokens counts all rows (batch * tokens per sequence)
+ *   sections   HOST int32[axes]: how many of the head_dim / 2 frequencies belong to each axis, in order; their sum is head_dim / 2
+ *   sine, cosine  fp32 [tokens, head_dim / 2]:  sin / cos(positions[a(i), t] * f_i)
+ * f_i = theta^(-i / (head_dim / 2)), one spectrum dealt to the axes; with B2_ROPE_OWN_SPECTRUM every axis has its own,
+ * f = theta^(-j / sections[a]) with j counted inside the section.  The angle is formed in 64 bits, so far positions keep their
+ * fraction of a turn.  1 to 4 axes, head_dim even and at most 1024, theta finite and > 0.  No reference counterpart on this path
+ * (its towers build one-axis tables with torch). */
+#define B2_ROPE_OWN_SPECTRUM 1
+int b2_rope_axes(const void* positions, int32_t position_bytes, const int32_t* sections, int32_t axes, int64_t tokens,
+                 int32_t head_dim, double theta, int32_t flags, void* sine, void* cosine, void* stream);
+
+/* The quantised key/value cache: e4m3 codes [batch, kv_heads, capacity, head_dim] and one fp32 scale per row,
+ * [batch, kv_heads, capacity], for keys and for values; head_dim 128 or 256.  Token t of sequence b stands at position
+ * offsets[b] + t; tokens at or beyond lengths[b], and positions outside [0, capacity), are passed over, and nothing of theirs is
+ * written.
+ * b2_kv_cache_write: `k`, `v` bf16 [batch, kv_heads, tokens, head_dim] in any strides (head_dim contiguous), so that slices of a
+ * packed QKV projection can be given as they lie.  With `sine` / `cosine` (fp32 [tokens, head_dim / 2], or per sequence at
+ * factor_batch_stride) keys are rotated with b2_rope_split's arithmetic before they are quantised, and with `q` (same strides rule;
+ * [batch, heads, tokens, head_dim]) rotated queries are written to `q_out` (bf16, contiguous) for every t < lengths[b].  Per row:
+ *   scale = max|x| / 448,  code = e4m3(x / scale), both in fp32 from the fp32 rotation
+ * scale and codes are 0 when max|x| < 2^-50, and the scale is NaN (the whole row reads back as NaN) when max|x| >= 2^40 or a value
+ * is not finite.
+ * Two tokens of one call that fall on one position (only possible by overlapping sequences' memory) are not ordered.
+ * b2_kv_cache_read: writes bf16(code * scale) of position offsets[b] + t to row t of `k`, `v` (any strides).  q, q_out, sine and
+ * cosine must be NULL.
+ * All pointers 16-byte aligned (scales, offsets and lengths: 4), strides multiples of 8 elements and not negative, and
+ * batch * tokens * (heads + 2 kv_heads) < 2^31.  The reference has no quantised cache. */
+typedef struct b2_kv_cache_desc {
+    const void* q;          /* bf16 or NULL */
+    void* q_out;            /* bf16 [batch, heads, tokens, head_dim], given exactly when q is */
+    void* k;                /* bf16: read by the write, written by the read */
+    void* v;
+    const void* sine;       /* fp32 or NULL: no rotation */
+    const void* cosine;
+    void* k_codes;
+    void* k_scales;
+    void* v_codes;
+    void* v_scales;
+    const void* offsets;    /* int32[batch] or NULL: 0 */
+    const void* lengths;    /* int32[batch] or NULL: tokens */
+    int64_t q_stride[3];    /* elements between batch entries, heads, tokens */
+    int64_t k_stride[3];
+    int64_t v_stride[3];
+    int64_t factor_batch_stride;
+    int32_t batch, tokens, heads, kv_heads, head_dim, capacity;
+} b2_kv_cache_desc;
+int b2_kv_cache_write(const b2_kv_cache_desc* desc, void* stream);
+int b2_kv_cache_read(const b2_kv_cache_desc* desc, void* stream);
+
+/* Attention of a batch whose members share prefixes, each prefix read and multiplied once for all its members:
+ *   keys of member b of group g = prefix[g, :prefix_lengths[g]] followed by the first n of own[b],
+ *     n = own_lengths[b], or with B2_ATTENTION_CAUSAL clamp(own_lengths[b] - queries + t + 1, 0, own_lengths[b]) for query t
+ *   out[b, h, t, :] = softmax(scale * q[b, h, t, :] K^T) V, zero where a row sees no key
+ * Query heads h * kv_heads / heads share a key/value head.  Caches are bf16 (cache_bits 16; scales NULL) or quantised as
+ * b2_kv_cache_write leaves them (cache_bits 8): prefix [groups, kv_heads, prefix_capacity, head_dim], own
+ * [batch, kv_heads, own_capacity, head_dim], contiguous; one of the capacities may be 0 (its pointers NULL).  Group g has the
+ * members [members[g], members[g + 1]) of the batch (device int32[groups + 1], not decreasing, from 0 to batch; members that no
+ * group holds get no output), or batch / groups each when `members` is NULL.  Lengths are clamped to their capacity.  What lies
+ * behind a length is never used.  A key row that holds a NaN or an infinity gives NaN to the rows that see it, and to no other; so
+ * do such own values (a whole output row) and quantised values; bf16 prefix values that are not finite follow IEEE arithmetic.
+ * Scores, softmax statistics and outputs are held in fp32; probabilities enter the second product as bf16 (bf16 cache) or f16
+ * (quantised cache; there q enters the first as two e4m3 halves that hold its 8 bits).  head_dim 128 or 256.
+ * `workspace`: NULL, or 32-byte aligned device scratch; with b2_prefix_attention_workspace_bytes(desc) bytes a launch of few row
+ * tiles cuts their keys across the SMs and joins the parts in a fixed order.  It needs no zeroing and holds nothing between
+ * calls, but two calls that may run at the same time need one each.  `status` as in b2_linear_desc.
+ * Widens b2_attention (one copy of the keys per batch element, head_dim 256, one key/value head, no lengths); the reference
+ * attends per sample (embodiinfer/backend/torch/attention.py:97-106). */
+#define B2_ATTENTION_CAUSAL 1
+typedef struct b2_prefix_attention_desc {
+    const void* q;               /* bf16 [batch, heads, queries, head_dim], head_dim contiguous */
+    void* out;                   /* bf16 [batch, heads, queries, head_dim], contiguous */
+    const void* prefix_k;
+    const void* prefix_v;
+    const void* prefix_k_scales;
+    const void* prefix_v_scales;
+    const void* own_k;
+    const void* own_v;
+    const void* own_k_scales;
+    const void* own_v_scales;
+    const void* members;         /* int32[groups + 1] or NULL */
+    const void* prefix_lengths;  /* int32[groups] or NULL: prefix_capacity */
+    const void* own_lengths;     /* int32[batch] or NULL: own_capacity */
+    void* status;
+    void* workspace;
+    int64_t workspace_bytes;
+    int64_t q_stride[3];         /* elements between batch entries, heads, queries: multiples of 8, not negative */
+    float scale;                 /* finite, > 0 */
+    int32_t flags;               /* B2_ATTENTION_CAUSAL; any other bit: B2_E_INVALID */
+    int32_t batch, groups, heads, kv_heads, queries, head_dim, prefix_capacity, own_capacity, cache_bits;
+} b2_prefix_attention_desc;
+int b2_prefix_attention(const b2_prefix_attention_desc* desc, void* stream);
+
+/* Device scratch that b2_prefix_attention could use for `desc`, in bytes (0: it would not split).  Pointer fields are only
+ * compared with NULL. */
+int64_t b2_prefix_attention_workspace_bytes(const b2_prefix_attention_desc* desc);
 
 /* RMSNorm (+ residual update, + adaptive modulation) fused with the activation encoder: the step in front of
  * every quantised projection.  Replaces cc_norm_quant and cc_norm_quant_reduce
