@@ -8,11 +8,17 @@
 // a CTA takes 128 of them and walks the prefix in tiles of 64 keys -- every key tile is loaded once for all 128 rows -- and then
 // the own keys of the members its rows belong to, where the rows of the other members are masked.  The own part so spends tensor
 // instructions on masked rows; it stays below the time of loading those keys, which nobody else needs.
-//   warp 0       TMA producer: key and value tiles through rings
-//   warp 1       tensor-memory owner and MMA issuer: S = Q K^T (128 x 64) and O += P V (128 x D), fp32 accumulators in tensor memory
-//   warps 2-5    one thread per row: scores, running reference and sum, probabilities into shared memory, output
-//   warps 6..    what the value tile still needs before the tensor core may read it (see below)
-// S is double-buffered.  Every wait is bounded and reports through the status word.
+//   warp 0        TMA producer: key and value tiles through rings
+//   warp 1        tensor-memory owner and MMA issuer: S = Q K^T (128 x 64) and O += P V (128 x D), fp32 accumulators in tensor memory
+//   warps 2-9     two softmax groups of 128 threads, one thread per row, for the even and the odd key tiles: scores, reference and
+//                 sum, probabilities, output
+//   warps 10..    what the value tile still needs before the tensor core may read it (see below)
+// What bounds such a loop is shared memory: 128 bytes per cycle have to take the tiles from TMA and give them to the tensor core,
+// and with Q and P there as well (128 rows of 32 bytes again for every 64 keys) they cost more than K and V themselves.  So Q lives
+// in tensor memory as the first product's "A" operand, and P as the second one's:
+// S of the even and odd tiles 2 x 64 columns, O D columns, Q and P the rest (D = 256: a quarter of Q stays in shared memory).
+// The two softmax groups work a tile apart and pass one float per row: the running reference, which a group needs from the
+// other only after it has the maximum of its own tile.  Every wait is bounded and reports through the status word.
 //
 // bf16 cache.  K and V are read as they lie in memory.  What the tensor core must not see is taken out of the value tile in
 // shared memory, because a probability of zero times an infinity or a NaN is not zero: rows behind the end of a segment are set to
@@ -28,8 +34,10 @@
 //   2^-8).  vs cannot be divided out afterwards, so it joins the probability:
 //       w = 2^(s + log2 vs - M),   O = sum w v,   L = sum w / vs,   out = O / L
 //   with M the running reference of s + log2 vs: the weights that meet the values are at most 2^8, whatever the spread of the
-//   scales, and f16 with its 11 bits is enough (bf16 probabilities would double the error of the result).
-//   A row whose scale is 0 holds zeros; it takes part in L alone, with vs = 1.
+//   scales, and f16 with its 11 bits is enough (bf16 probabilities would double the error of the result; two e4m3 halves, which
+//   would spare the conversion of V, have no room for a long tail of weights 2^-15 below the largest).
+//   A row whose scale is 0 holds zeros; it takes part in L alone, with a vs below every scale that the cache's write leaves
+//   (2^-59 to 2^32), so that it never sets M.
 //
 // Few CTAs: the key tiles of a row tile are cut across `splits` CTAs, which leave O, M and L in fp32 in the workspace; a second
 // launch joins them in split order (no atomics: the result does not depend on timing).
@@ -44,7 +52,7 @@ namespace {
 
 constexpr int PA_ROWS = 128;                     // query rows per CTA
 constexpr int PA_KEYS = 64;                      // keys per tile
-constexpr uint32_t PA_P_BYTES = PA_ROWS * PA_KEYS * 2;
+constexpr int PA_SOFTMAX_WARP = 2, PA_VALUE_WARP = 10;      // first softmax warp (of 8), first value warp
 constexpr int PA_SCALE_STAGES = 4;
 constexpr int PA_SCALE_FLOATS = 3 * PA_KEYS;     // ks, log2 vs, 1 / vs of a key tile
 constexpr float PA_ZERO_ROW_SCALE = 8.6736173798840355e-19f;      // 2^-60
@@ -57,25 +65,26 @@ struct PaShape {
     static constexpr int KV_ATOMS = ROW_BYTES / 128;                        // 128-byte column groups of a cached tile
     static constexpr uint32_t KV_ATOM_BYTES = PA_KEYS * 128;
     static constexpr uint32_t KV_BYTES = KV_ATOMS * KV_ATOM_BYTES;
-    static constexpr uint32_t Q_ATOM_BYTES = PA_ROWS * 128;
-    static constexpr uint32_t Q_BYTES = D * 2 / 128 * Q_ATOM_BYTES;         // bf16, or two e4m3 halves
-    static constexpr int STAGES = D == 256 ? 2 : 4;                         // of the K and the V ring each
+    static constexpr int STAGES = D == 256 ? (FP8 ? 4 : 3) : (FP8 ? 8 : 6); // of the K and the V ring each
     static constexpr int VALUE_STAGES = FP8 ? 2 : 0;                        // converted value tiles
     static constexpr uint32_t VALUE_BYTES = PA_KEYS * D * 2;
-    static constexpr int VALUE_WARPS = 4;
-    static constexpr int WARPS = 6 + VALUE_WARPS + (FP8 ? 1 : 0);           // + the scale warp
+    static constexpr int VALUE_WARPS = FP8 ? 4 : 2;
+    static constexpr int WARPS = PA_VALUE_WARP + VALUE_WARPS + (FP8 ? 1 : 0);   // + the scale warp
     static constexpr int THREADS = WARPS * 32;
-    static constexpr uint32_t TMEM_COLUMNS_USED = D == 256 ? 512 : 256;
-    static constexpr uint32_t TMEM_O = 2 * PA_KEYS;
-    static constexpr uint32_t OFF_K = Q_BYTES;
+    // Q: atoms of 32 columns (64 bf16 or 128 e4m3 values of a row).  With D = 256 there is room for three of the four, and for one P;
+    // the last atom of Q lies in shared memory.
+    static constexpr int Q_ATOMS = D / 64, Q_TMEM_ATOMS = Q_ATOMS < 3 ? Q_ATOMS : 3, P_BUFFERS = D == 256 ? 1 : 2;
+    static constexpr uint32_t TMEM_S = 0, TMEM_O = 2 * PA_KEYS, TMEM_Q = TMEM_O + D, TMEM_P = TMEM_Q + Q_TMEM_ATOMS * 32;
+    static_assert(TMEM_P + P_BUFFERS * 32 <= TMEM_COLUMNS, "tensor memory");
+    static constexpr uint32_t OFF_K = 0;
     static constexpr uint32_t OFF_V = OFF_K + STAGES * KV_BYTES;
     static constexpr uint32_t OFF_VALUES = OFF_V + STAGES * KV_BYTES;
-    static constexpr uint32_t OFF_P = OFF_VALUES + VALUE_STAGES * VALUE_BYTES;
-    static constexpr uint32_t OFF_SCALES = OFF_P + PA_P_BYTES;
-    static constexpr uint32_t OFF_ROW_FACTOR = OFF_SCALES + (FP8 ? PA_SCALE_STAGES * PA_SCALE_FLOATS * 4 : 0);
-    static constexpr uint32_t OFF_SEGMENTS = OFF_ROW_FACTOR + PA_ROWS * 4;
+    static constexpr uint32_t OFF_Q = OFF_VALUES + VALUE_STAGES * VALUE_BYTES;
+    static constexpr uint32_t OFF_SCALES = OFF_Q + (Q_ATOMS - Q_TMEM_ATOMS) * PA_ROWS * 128;
+    static constexpr uint32_t OFF_ROWS = OFF_SCALES + (FP8 ? PA_SCALE_STAGES * PA_SCALE_FLOATS * 4 : 0);      // float [2][128], twice
+    static constexpr uint32_t OFF_SEGMENTS = OFF_ROWS + 4 * PA_ROWS * 4;
     static constexpr uint32_t OFF_BARS = OFF_SEGMENTS + (PA_MAX_SEGMENTS + 3) * 8;
-    static constexpr int SHARED_BYTES = 1024 + int(OFF_BARS) + 512;
+    static constexpr int SHARED_BYTES = 1024 + int(OFF_BARS) + 768;
 };
 
 struct PaArgs {
@@ -111,7 +120,36 @@ __device__ __forceinline__ uint64_t pa_desc_mn(uint32_t mn_group_bytes) {
            (static_cast<uint64_t>(2) << 61);
 }
 
-__device__ __forceinline__ void pa_mma_16bit(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+// D[tmem] (+)= A[tmem] B[smem]: A's row is the tensor-memory lane, 32-bit columns hold 2 (16-bit) or 4 (8-bit) consecutive K values.
+template <bool EIGHT_BIT>
+__device__ __forceinline__ void pa_mma(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    if (EIGHT_BIT)
+        asm volatile(
+            "{\n\t"
+            ".reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], %2, %3, p;\n\t"
+            "}\n"
+            ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t"
+            ".reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+            "}\n"
+            ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+            : "memory");
+}
+
+// The same with A in shared memory.
+template <bool EIGHT_BIT>
+__device__ __forceinline__ void pa_mma_shared(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    if (EIGHT_BIT) {
+        mma_f8f6f4(d_tmem, a_desc, b_desc, idesc, accumulate);
+        return;
+    }
     asm volatile(
         "{\n\t"
         ".reg .pred p;\n\t"
@@ -133,6 +171,16 @@ __device__ __forceinline__ void pa_tmem_store(uint32_t address, const uint32_t (
           "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
         : "memory");
 }
+
+__device__ __forceinline__ void pa_tmem_store16(uint32_t address, const uint32_t* v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+        ::"r"(address), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+          "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+
+__device__ __forceinline__ void pa_tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ float pa_exp2(float x) {
     float y;
@@ -178,9 +226,8 @@ __device__ __forceinline__ bool has_not_finite(uint32_t word) {
 // Walks the key tiles of a CTA: the prefix (segment 0), then the own keys of its members.
 struct PaCursor {
     const int* first_tile;      // [segments + 1], shared memory
-    const int* length;          // [segments]
     int segment, offset;        // offset: key tile inside the segment
-    __device__ __forceinline__ PaCursor(const int* first, const int* lengths, int segments, int tile) : first_tile(first), length(lengths), segment(0), offset(0) {
+    __device__ __forceinline__ PaCursor(const int* first, int segments, int tile) : first_tile(first), segment(0), offset(0) {
         int low = 0, high = segments;      // the last segment that starts at or before `tile`; empty ones are passed over
         while (high - low > 1) {
             const int middle = (low + high) >> 1;
@@ -190,12 +237,9 @@ struct PaCursor {
         segment = low;
         offset = tile - first[low];
     }
-    __device__ __forceinline__ void next(int tile) {          // to `tile`, the one behind the current
-        ++offset;
-        while (first_tile[segment + 1] <= tile) {
-            ++segment;
-            offset = tile - first_tile[segment];
-        }
+    __device__ __forceinline__ void seek(int tile) {          // forward to `tile`, which exists
+        while (first_tile[segment + 1] <= tile) ++segment;
+        offset = tile - first_tile[segment];
     }
 };
 
@@ -209,20 +253,23 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
     extern __shared__ uint8_t shared_raw[];
     const uint32_t base = (smem_u32(shared_raw) + 1023u) & ~1023u;
     uint8_t* const generic = shared_raw + (base - smem_u32(shared_raw));
-    const uint32_t q_smem = base, k_smem = base + Shape::OFF_K, v_smem = base + Shape::OFF_V, values_smem = base + Shape::OFF_VALUES;
-    const uint32_t p_smem = base + Shape::OFF_P, scales_smem = base + Shape::OFF_SCALES;
-    float* const row_factor = reinterpret_cast<float*>(generic + Shape::OFF_ROW_FACTOR);
+    const uint32_t k_smem = base + Shape::OFF_K, v_smem = base + Shape::OFF_V, values_smem = base + Shape::OFF_VALUES;
+    const uint32_t q_smem = base + Shape::OFF_Q, scales_smem = base + Shape::OFF_SCALES;
+    float* const row_reference = reinterpret_cast<float*>(generic + Shape::OFF_ROWS);           // [2][128]: of the latest even and odd tile
+    float* const row_exchange = row_reference + 2 * PA_ROWS;                                    // [2][128]: row maxima of Q, then the sums
     int* const segment_first = reinterpret_cast<int*>(generic + Shape::OFF_SEGMENTS);
     int* const segment_length = segment_first + PA_MAX_SEGMENTS + 3;
     const uint32_t bars = base + Shape::OFF_BARS;
     constexpr int STAGES = Shape::STAGES;
-    const uint32_t k_full = bars, k_empty = bars + 32, v_full = bars + 64, v_empty = bars + 96;          // [STAGES] each
-    const uint32_t value_full = bars + 128, value_empty = bars + 160;      // converted tiles [2]; bf16: value_full [STAGES] = the tile's tail is zeroed
-    const uint32_t s_full = bars + 192, s_free = bars + 208;               // [2]
-    const uint32_t scale_full = bars + 224, scale_empty = bars + 256;      // [PA_SCALE_STAGES]
-    const uint32_t p_ready = bars + 288, o_done = bars + 296, q_ready = bars + 304, tmem_slot = bars + 312;
-    PaWork* const work = reinterpret_cast<PaWork*>(generic + Shape::OFF_BARS + 320);
-    unsigned long long* const bad_keys = reinterpret_cast<unsigned long long*>(generic + Shape::OFF_BARS + 352);      // bf16: [STAGES]
+    static_assert(STAGES <= 8, "barrier arrays");
+    const uint32_t k_full = bars, k_empty = bars + 64, v_full = bars + 128, v_empty = bars + 192;        // [STAGES] each
+    const uint32_t value_full = bars + 256, value_empty = bars + 320;      // converted tiles [2]; bf16: value_full [STAGES] = the tile may be read
+    const uint32_t s_full = bars + 384, s_free = bars + 400, p_ready = bars + 416, o_done = bars + 432;      // [2]: even and odd tiles
+    const uint32_t scale_full = bars + 448, scale_empty = bars + 480;      // [PA_SCALE_STAGES]
+    const uint32_t reference_ready = bars + 512;                           // [4 quarters][2]
+    const uint32_t all_done = bars + 576, q_ready = bars + 584, tmem_slot = bars + 592;
+    PaWork* const work = reinterpret_cast<PaWork*>(generic + Shape::OFF_BARS + 608);
+    unsigned long long* const bad_keys = reinterpret_cast<unsigned long long*>(generic + Shape::OFF_BARS + 640);      // bf16: [STAGES]
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // row tile fastest: CTAs that run together share the key tiles of their group in the L2
@@ -244,14 +291,16 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
         for (int i = 0; i < 2; ++i) {
             mbar_init(s_full + 8 * i, 1);
             mbar_init(s_free + 8 * i, 4);
+            mbar_init(p_ready + 8 * i, 4);
+            mbar_init(o_done + 8 * i, 1);
         }
         for (int i = 0; i < PA_SCALE_STAGES; ++i) {
             mbar_init(scale_full + 8 * i, 1);
             mbar_init(scale_empty + 8 * i, 4);
         }
-        mbar_init(p_ready, 4);
-        mbar_init(o_done, 1);
-        mbar_init(q_ready, Shape::WARPS - 1);
+        for (int i = 0; i < 8; ++i) mbar_init(reference_ready + 8 * i, 1);
+        mbar_init(all_done, 1);
+        mbar_init(q_ready, 8);
         fence_barrier_init();
         tma_prefetch_descriptor(&prefix_k_map);
         tma_prefetch_descriptor(&prefix_v_map);
@@ -259,7 +308,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
         tma_prefetch_descriptor(&own_v_map);
     }
     if (warp == 1) {
-        tmem_alloc(tmem_slot, Shape::TMEM_COLUMNS_USED);
+        tmem_alloc(tmem_slot, TMEM_COLUMNS);
         tmem_relinquish();
     }
     pdl_wait();
@@ -345,85 +394,12 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
     const int num_tiles = int(int64_t(w.key_tiles) * (split + 1) / args.splits) - start_tile;
 
     bool failed = false;
-    // ---- queries into shared memory, every warp but the producer: one row per warp and step
-    if (warp != 0) {
-        constexpr int LOADERS = Shape::WARPS - 1, PER_WARP = (PA_ROWS + LOADERS - 1) / LOADERS;
-        constexpr int LANE_ELEMENTS = D / 32;      // 8 or 4 bf16 values of a row per lane
-        uint4 packed[PER_WARP];
-#pragma unroll
-        for (int i = 0; i < PER_WARP; ++i) {
-            const int row = (warp - 1) + i * LOADERS;
-            packed[i] = make_uint4(0, 0, 0, 0);
-            if (row >= w.rows || num_tiles == 0) continue;
-            const int member = (w.row0 + row) / args.rows_per_member, inside = w.row0 + row - member * args.rows_per_member;
-            const int head = inside / args.queries, query = inside - head * args.queries;
-            const __nv_bfloat16* source = args.q + int64_t(w.first_member + member) * args.q_stride[0] +
-                                          (int64_t(kv_head) * (args.heads / args.kv_heads) + head) * args.q_stride[1] + query * args.q_stride[2] + lane * LANE_ELEMENTS;
-            if (D == 256) {
-                packed[i] = *reinterpret_cast<const uint4*>(source);
-            } else {
-                const uint2 half = *reinterpret_cast<const uint2*>(source);
-                packed[i].x = half.x;
-                packed[i].y = half.y;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < PER_WARP; ++i) {
-            const int row = (warp - 1) + i * LOADERS;
-            if (row >= PA_ROWS) continue;
-            const uint32_t line = uint32_t(row >> 3) * 1024u + uint32_t(row & 7) * 128u, swizzle = uint32_t(row & 7);
-            if (!FP8) {
-                const uint32_t byte = uint32_t(lane) * LANE_ELEMENTS * 2, atom = byte >> 7, chunk = (byte & 127u) >> 4;
-                const uint32_t address = q_smem + atom * Shape::Q_ATOM_BYTES + line + ((chunk ^ swizzle) << 4) + (byte & 15u);
-                if (D == 256) sts_u4(address, packed[i].x, packed[i].y, packed[i].z, packed[i].w);
-                else asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(address), "r"(packed[i].x), "r"(packed[i].y) : "memory");
-                if (lane == 0) row_factor[row] = args.scale_log2;
-            } else {
-                const uint32_t words[4] = {packed[i].x, packed[i].y, packed[i].z, packed[i].w};
-                uint32_t largest = 0;      // bf16 magnitude bits: NaN and infinities order above numbers
-#pragma unroll
-                for (int j = 0; j < LANE_ELEMENTS / 2; ++j) largest = max(largest, max(words[j] & 0x7fffu, (words[j] >> 16) & 0x7fffu));
-                largest = __reduce_max_sync(0xffffffffu, largest);
-                // 2^e that brings the largest magnitude into [128, 256), kept a normal number
-                int exponent = int(largest >> 7) - 127;
-                exponent = exponent < -110 ? -110 : (exponent > 120 ? 120 : exponent);
-                const float up = largest == 0u ? 1.0f : __uint_as_float(uint32_t(127 + 7 - exponent) << 23);
-                const float down = largest == 0u ? 1.0f : __uint_as_float(uint32_t(127 - 7 + exponent) << 23);
-                uint32_t high[2] = {0u, 0u}, low[2] = {0u, 0u};
-#pragma unroll
-                for (int j = 0; j < LANE_ELEMENTS / 2; ++j) {
-                    const float2 value = bf16x2_to_float2(words[j]);
-                    const float2 scaled = make_float2(value.x * up, value.y * up);
-                    const uint32_t h = __nv_cvt_float2_to_fp8x2(scaled, __NV_SATFINITE, __NV_E4M3);
-                    const float2 back = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(h), __NV_E4M3)));
-                    const uint32_t l = __nv_cvt_float2_to_fp8x2(make_float2(scaled.x - back.x, scaled.y - back.y), __NV_SATFINITE, __NV_E4M3);
-                    high[j >> 1] |= h << (16 * (j & 1));
-                    low[j >> 1] |= l << (16 * (j & 1));
-                }
-                const uint32_t byte = uint32_t(lane) * LANE_ELEMENTS, atom = byte >> 7, chunk = (byte & 127u) >> 4;
-                const uint32_t address = q_smem + atom * Shape::Q_ATOM_BYTES + line + ((chunk ^ swizzle) << 4) + (byte & 15u);
-                constexpr uint32_t LOW_HALF = uint32_t(D / 128) * Shape::Q_ATOM_BYTES;
-                if (D == 256) {
-                    asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(address), "r"(high[0]), "r"(high[1]) : "memory");
-                    asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(address + LOW_HALF), "r"(low[0]), "r"(low[1]) : "memory");
-                } else {
-                    asm volatile("st.shared.u32 [%0], %1;" ::"r"(address), "r"(high[0]) : "memory");
-                    asm volatile("st.shared.u32 [%0], %1;" ::"r"(address + LOW_HALF), "r"(low[0]) : "memory");
-                }
-                // a row with an infinity or a NaN: every score is NaN
-                if (lane == 0) row_factor[row] = largest >= 0x7f80u ? __uint_as_float(0x7fc00000u) : args.scale_log2 * down;
-            }
-        }
-        fence_async_shared();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(q_ready);
-    }
-
     if (warp == 0) {
         // ------------------------------------------------------------- TMA producer
         if (num_tiles > 0) {
-            PaCursor cursor(segment_first, segment_length, w.segments, start_tile);
+            PaCursor cursor(segment_first, w.segments, start_tile);
             for (int j = 0; j < num_tiles; ++j) {
+                cursor.seek(start_tile + j);
                 const int b = j % STAGES;
                 const uint32_t parity = uint32_t(j / STAGES) & 1u;
                 const bool prefix = cursor.segment == 0;
@@ -447,7 +423,6 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
                         tma_load_2d(v_smem + b * Shape::KV_BYTES + a * Shape::KV_ATOM_BYTES, v_map, v_full + 8 * b, a * 128, row);
                 }
                 __syncwarp();
-                if (j + 1 < num_tiles) cursor.next(start_tile + j + 1);
             }
             // every copy has landed before this CTA may leave (on the normal path the readers have long seen them)
             bool drain_failed = false;
@@ -474,71 +449,137 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
             tc_fence_after_sync();
             __syncwarp();
             if (elect_one()) {
-                const uint32_t d_tmem = tmem_base + uint32_t(d) * PA_KEYS;
+                const uint32_t d_tmem = tmem_base + Shape::TMEM_S + uint32_t(d) * PA_KEYS;
                 const uint32_t k_base = k_low + field(k_smem + b * Shape::KV_BYTES);
-                const uint32_t q_base = k_low + field(q_smem);
+                // 32 bytes along K per instruction: 8 columns of Q.  Quantised: first all of hi, then all of lo.
 #pragma unroll
-                for (int half = 0; half < (FP8 ? 2 : 1); ++half)
+                for (int a = 0; a < Shape::Q_ATOMS; ++a)
 #pragma unroll
-                    for (int a = 0; a < Shape::KV_ATOMS; ++a)
-#pragma unroll
-                        for (int s = 0; s < 4; ++s) {          // 32 bytes along K per instruction
-                            const uint64_t q_desc = desc_from_words(q_base + (half * Shape::KV_ATOMS + a) * (Shape::Q_ATOM_BYTES >> 4) + 2 * s, k_high);
-                            const uint64_t k_desc = desc_from_words(k_base + a * (Shape::KV_ATOM_BYTES >> 4) + 2 * s, k_high);
-                            if (FP8) mma_f8f6f4(d_tmem, q_desc, k_desc, idesc_scores, (half | a | s) != 0);
-                            else pa_mma_16bit(d_tmem, q_desc, k_desc, idesc_scores, (a | s) != 0);
-                        }
+                    for (int s = 0; s < 4; ++s) {
+                        const uint64_t k_desc = desc_from_words(k_base + (a % Shape::KV_ATOMS) * (Shape::KV_ATOM_BYTES >> 4) + 2 * s, k_high);
+                        if (a < Shape::Q_TMEM_ATOMS) pa_mma<FP8>(d_tmem, tmem_base + Shape::TMEM_Q + uint32_t((a * 4 + s) * 8), k_desc, idesc_scores, (a | s) != 0);
+                        else pa_mma_shared<FP8>(d_tmem, desc_from_words(k_low + field(q_smem) + 2 * s, k_high), k_desc, idesc_scores, 1u);
+                    }
                 tc_commit(k_empty + 8 * b);
                 tc_commit(s_full + 8 * d);
             }
             __syncwarp();
         };
         auto output = [&](int j) {          // O += P V_j
-            const int b = FP8 ? (j & 1) : j % STAGES;
+            const int b = FP8 ? (j & 1) : j % STAGES, d = j & 1;
             const uint32_t parity = uint32_t(FP8 ? j >> 1 : j / STAGES) & 1u;
             mbar_wait(value_full + 8 * b, parity, failed, args.status, STATUS_WAIT_MMA_FULL);
-            mbar_wait(p_ready, uint32_t(j) & 1u, failed, args.status, STATUS_WAIT_MMA_TMEM);
+            mbar_wait(p_ready + 8 * d, uint32_t(j >> 1) & 1u, failed, args.status, STATUS_WAIT_MMA_TMEM);
+            // One output at a time: who has seen the output of tile j - 2 done can tell by its parity whether that of j - 1 is.  The
+            // scores issued in between keep the tensor core busy.
+            if (j > 0) mbar_wait(o_done + 8 * (d ^ 1), uint32_t((j - 1) >> 1) & 1u, failed, args.status, STATUS_WAIT_MMA_TMEM);
             tc_fence_after_sync();
             __syncwarp();
             if (elect_one()) {
-                const uint32_t p_base = k_low + field(p_smem);
+                const uint32_t p_tmem = tmem_base + Shape::TMEM_P + uint32_t(d % Shape::P_BUFFERS) * 32;
                 const uint32_t v_base = mn_low + field(FP8 ? values_smem + b * Shape::VALUE_BYTES : v_smem + b * Shape::KV_BYTES);
 #pragma unroll
-                for (int s = 0; s < PA_KEYS / 16; ++s)          // 16 keys per instruction: 32 bytes along a row of P, 16 rows (2048 bytes) of V
-                    pa_mma_16bit(tmem_base + Shape::TMEM_O, desc_from_words(p_base + 2 * s, k_high), desc_from_words(v_base + s * (2048 >> 4), mn_high),
-                                 idesc_output, (j | s) != 0);
+                for (int s = 0; s < PA_KEYS / 16; ++s)          // 16 keys per instruction: 8 columns of P, 16 rows (2048 bytes) of V
+                    pa_mma<false>(tmem_base + Shape::TMEM_O, p_tmem + 8 * s, desc_from_words(v_base + s * (2048 >> 4), mn_high), idesc_output, (j | s) != 0);
                 tc_commit((FP8 ? value_empty : v_empty) + 8 * b);
-                tc_commit(o_done);
+                tc_commit(o_done + 8 * d);
             }
             __syncwarp();
         };
         if (num_tiles > 0) scores(0);
+        if (num_tiles > 1) scores(1);
         for (int j = 0; j < num_tiles; ++j) {
-            if (j + 1 < num_tiles) scores(j + 1);
+            if (j + 2 < num_tiles) scores(j + 2);          // as soon as its group has the scores of tile j in registers
             output(j);
         }
-    } else if (warp < 6) {
-        // ------------------------------------------------------------- one thread per query row
+        if (num_tiles > 0 && elect_one()) tc_commit(all_done);
+        __syncwarp();
+    } else if (warp < PA_VALUE_WARP) {
+        // ------------------------------------------------------------- one thread per query row and tile parity
         const int quarter = warp & 3, row = quarter * 32 + lane;          // row of the tile = tensor-memory lane
+        const int parity_group = (warp - PA_SOFTMAX_WARP) >> 2;           // 0: even tiles, 1: odd tiles
         const uint32_t lane_address = tmem_base + (uint32_t(quarter * 32) << 16);
         const bool exists = row < w.rows;
         int my_segment = -1, hidden = 0;          // the segment of this row's own keys; causal: how many of them lie behind the query
         int64_t out_offset = -1;
+        const __nv_bfloat16* query_row = args.q;
         if (exists) {
             const int member = (w.row0 + row) / args.rows_per_member, inside = w.row0 + row - member * args.rows_per_member;
-            const int head = inside / args.queries, query = inside - head * args.queries;
+            const int head_in_group = inside / args.queries, query = inside - head_in_group * args.queries;
+            const int head = kv_head * (args.heads / args.kv_heads) + head_in_group;
             my_segment = member - w.first_segment_member + 1;
             hidden = args.causal ? args.queries - 1 - query : 0;
-            out_offset = ((int64_t(w.first_member + member) * args.heads + int64_t(kv_head) * (args.heads / args.kv_heads) + head) * args.queries + query) * D;
+            out_offset = ((int64_t(w.first_member + member) * args.heads + head) * args.queries + query) * D;
+            query_row += int64_t(w.first_member + member) * args.q_stride[0] + head * args.q_stride[1] + query * args.q_stride[2];
         }
-        float running_max = -INFINITY, running_sum = 0.0f, factor = 0.0f;
+        // ---- the queries into tensor memory: each group brings one half of the columns
+        float factor = args.scale_log2;
         if (num_tiles > 0) {
-            mbar_wait(q_ready, 0u, failed, args.status, STATUS_WAIT_EPILOGUE);
-            factor = row_factor[row];
+            constexpr int WORDS = D / 4;          // 32-bit words of half a bf16 row
+            uint32_t words[WORDS];
+            const uint4* source = reinterpret_cast<const uint4*>(query_row + parity_group * (D / 2));
+#pragma unroll
+            for (int i = 0; i < WORDS / 4; ++i) {
+                const uint4 v = exists ? source[i] : make_uint4(0, 0, 0, 0);
+                words[4 * i] = v.x; words[4 * i + 1] = v.y; words[4 * i + 2] = v.z; words[4 * i + 3] = v.w;
+            }
+            // atom `a` of Q: 32 words of this row
+            auto store_atom = [&](int a, const uint32_t* atom) {
+                if (a < Shape::Q_TMEM_ATOMS) {
+                    pa_tmem_store(lane_address + Shape::TMEM_Q + uint32_t(a) * 32, *reinterpret_cast<const uint32_t(*)[32]>(atom));
+                    return;
+                }
+                const uint32_t line = q_smem + uint32_t(row >> 3) * 1024u + uint32_t(row & 7) * 128u;
+#pragma unroll
+                for (int c = 0; c < 8; ++c) sts_u4(line + uint32_t((c ^ (row & 7)) * 16), atom[4 * c], atom[4 * c + 1], atom[4 * c + 2], atom[4 * c + 3]);
+                fence_async_shared();
+            };
+            if (!FP8) {
+#pragma unroll
+                for (int i = 0; i < WORDS / 32; ++i) store_atom(parity_group * (WORDS / 32) + i, words + 32 * i);
+            } else {
+                uint32_t largest = 0;      // bf16 magnitude bits: NaN and infinities order above numbers
+#pragma unroll
+                for (int i = 0; i < WORDS; ++i) largest = max(largest, max(words[i] & 0x7fffu, (words[i] >> 16) & 0x7fffu));
+                row_exchange[parity_group * PA_ROWS + row] = __uint_as_float(largest);
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                largest = max(largest, __float_as_uint(row_exchange[(parity_group ^ 1) * PA_ROWS + row]));
+                // 2^e that brings the largest magnitude into [128, 256), kept a normal number
+                int exponent = int(largest >> 7) - 127;
+                exponent = exponent < -110 ? -110 : (exponent > 120 ? 120 : exponent);
+                const float up = largest == 0u ? 1.0f : __uint_as_float(uint32_t(127 + 7 - exponent) << 23);
+                const float down = largest == 0u ? 1.0f : __uint_as_float(uint32_t(127 - 7 + exponent) << 23);
+                // a row with an infinity or a NaN: every score is NaN
+                factor = largest >= 0x7f80u ? __uint_as_float(0x7fc00000u) : args.scale_log2 * down;
+                uint32_t high[WORDS / 2], low[WORDS / 2];
+#pragma unroll
+                for (int i = 0; i < WORDS; ++i) {
+                    const float2 value = bf16x2_to_float2(words[i]);
+                    const float2 scaled = make_float2(value.x * up, value.y * up);
+                    const uint32_t h = __nv_cvt_float2_to_fp8x2(scaled, __NV_SATFINITE, __NV_E4M3);
+                    const float2 back = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(h), __NV_E4M3)));
+                    const uint32_t l = __nv_cvt_float2_to_fp8x2(make_float2(scaled.x - back.x, scaled.y - back.y), __NV_SATFINITE, __NV_E4M3);
+                    high[i >> 1] = (i & 1) ? high[i >> 1] | (h << 16) : h;
+                    low[i >> 1] = (i & 1) ? low[i >> 1] | (l << 16) : l;
+                }
+                if (D == 256) {          // the half row is one atom of hi and one of lo
+                    store_atom(parity_group, high);
+                    store_atom(2 + parity_group, low);
+                } else {
+                    pa_tmem_store16(lane_address + Shape::TMEM_Q + parity_group * 16, high);
+                    pa_tmem_store16(lane_address + Shape::TMEM_Q + 32 + parity_group * 16, low);
+                }
+            }
+            pa_tmem_store_wait();
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_ready);
         }
-        PaCursor cursor(segment_first, segment_length, w.segments, start_tile);
-        for (int j = 0; j < num_tiles; ++j) {
-            const int d = j & 1;
+        float reference = -INFINITY, running_sum = 0.0f;          // of this group's tiles so far: the sum in units of 2^reference
+        PaCursor cursor(segment_first, w.segments, start_tile);
+        for (int j = parity_group; j < num_tiles; j += 2) {
+            cursor.seek(start_tile + j);
+            const uint32_t s_tmem = lane_address + Shape::TMEM_S + uint32_t(parity_group) * PA_KEYS;
             // keys of this tile that this row sees: the first `valid`
             int valid = 0;
             if (exists) {
@@ -546,36 +587,31 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
                 else if (cursor.segment == my_segment) valid = segment_length[cursor.segment] - hidden - cursor.offset * PA_KEYS;
             }
             const bool whole = __all_sync(0xffffffffu, valid >= PA_KEYS), none = __all_sync(0xffffffffu, valid <= 0);
-            mbar_wait(s_full + 8 * d, uint32_t(j >> 1) & 1u, failed, args.status, STATUS_WAIT_EPILOGUE);
+            mbar_wait(s_full + 8 * parity_group, uint32_t(j >> 1) & 1u, failed, args.status, STATUS_WAIT_EPILOGUE);
             tc_fence_after_sync();
             uint32_t raw[2][32];
-            if (!none) {
-                tmem_load_32x32(lane_address + uint32_t(d) * PA_KEYS, raw[0]);
-                tmem_load_32x32(lane_address + uint32_t(d) * PA_KEYS + 32, raw[1]);
-                tmem_load_wait();
-            }
-            tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(s_free + 8 * d);
             const int stage = j % PA_SCALE_STAGES;
             const uint32_t tile_scales = scales_smem + uint32_t(stage) * PA_SCALE_FLOATS * 4;
+            if (!none) {
+                tmem_load_32x32(s_tmem, raw[0]);
+                tmem_load_32x32(s_tmem + 32, raw[1]);
+            }
             if (FP8) mbar_wait(scale_full + 8 * stage, uint32_t(j / PA_SCALE_STAGES) & 1u, failed, args.status, STATUS_WAIT_EPILOGUE);
-            float correction = 1.0f;
-            uint32_t packed[2][16];
-            if (none) {
-#pragma unroll
-                for (int i = 0; i < 32; ++i) packed[i >> 4][i & 15] = 0u;
-            } else {
-                // in units of log2: score, quantised also + log2 vs
-                if (FP8) {
+            float tile_max = -INFINITY;
+            if (!none) tmem_load_wait();
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(s_free + 8 * parity_group);
+            if (!none) {
+                if (FP8) {      // score in units of log2, + log2 vs
+                    const float2 factor2 = make_float2(factor, factor);
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const float4 ks = lds_f4(tile_scales + i * 16), lv = lds_f4(tile_scales + PA_KEYS * 4 + i * 16);
                         uint32_t* r = &raw[i >> 3][(i & 7) * 4];
-                        r[0] = __float_as_uint(__fmaf_rn(__uint_as_float(r[0]) * ks.x, factor, lv.x));
-                        r[1] = __float_as_uint(__fmaf_rn(__uint_as_float(r[1]) * ks.y, factor, lv.y));
-                        r[2] = __float_as_uint(__fmaf_rn(__uint_as_float(r[2]) * ks.z, factor, lv.z));
-                        r[3] = __float_as_uint(__fmaf_rn(__uint_as_float(r[3]) * ks.w, factor, lv.w));
+                        const float2 a = __ffma2_rn(__fmul2_rn(make_float2(__uint_as_float(r[0]), __uint_as_float(r[1])), make_float2(ks.x, ks.y)), factor2, make_float2(lv.x, lv.y));
+                        const float2 c = __ffma2_rn(__fmul2_rn(make_float2(__uint_as_float(r[2]), __uint_as_float(r[3])), make_float2(ks.z, ks.w)), factor2, make_float2(lv.z, lv.w));
+                        r[0] = __float_as_uint(a.x); r[1] = __float_as_uint(a.y); r[2] = __float_as_uint(c.x); r[3] = __float_as_uint(c.y);
                     }
                 }
                 if (!whole) {
@@ -585,100 +621,129 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
                 }
                 float partial_max[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int i = 0; i < 64; ++i) partial_max[i & 3] = fmaxf(partial_max[i & 3], __uint_as_float(raw[i >> 5][i & 31]));
-                float tile_max = fmaxf(fmaxf(partial_max[0], partial_max[1]), fmaxf(partial_max[2], partial_max[3]));
+                for (int i = 0; i < 32; ++i)
+                    partial_max[i & 3] = fmaxf(fmaxf(partial_max[i & 3], __uint_as_float(raw[0][i])), __uint_as_float(raw[1][i]));
+                tile_max = fmaxf(fmaxf(partial_max[0], partial_max[1]), fmaxf(partial_max[2], partial_max[3]));
                 if (!FP8) tile_max *= factor;
-                // The reference follows the maximum lazily, as in attention.cu: weights stay below 2^8 and the accumulator is
-                // rescaled a few times per row.  A row that has seen no key yet has no reference; 0 stands in, its weights are 0.
-                const bool move = tile_max > running_max + 8.0f;
-                const float new_max = move ? tile_max : running_max;
-                correction = move ? pa_exp2(running_max - new_max) : 1.0f;
-                running_max = new_max;
-                const float reference = new_max == -INFINITY ? 0.0f : new_max;
-                float partial_sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            }
+            // The reference of the tile before comes from the other group.  It follows the maximum lazily: it moves only when the
+            // maximum has grown by more than 2^8 since it was set, so weights stay below 2^8 and the accumulator is rescaled a few
+            // times per row.  A row that has seen no key yet has none; 0 stands in, its weights are 0.
+            float previous = -INFINITY;
+            if (j > 0) {
+                const int other = parity_group ^ 1;
+                mbar_wait(reference_ready + 16 * quarter + 8 * other, uint32_t((j - 1) >> 1) & 1u, failed, args.status, STATUS_WAIT_EPILOGUE);
+                previous = *static_cast<volatile float*>(row_reference + other * PA_ROWS + row);
+            }
+            const float now = tile_max > previous + 8.0f ? tile_max : previous;
+            *static_cast<volatile float*>(row_reference + parity_group * PA_ROWS + row) = now;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(reference_ready + 16 * quarter + 8 * parity_group);
+            const float correction = now == previous ? 1.0f : pa_exp2(previous - now);
+            if (now != reference) running_sum *= pa_exp2(reference - now);
+            reference = now;
+            uint32_t packed[32];
+            if (none) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) packed[i] = 0u;
+            } else {
+                const float shift = now == -INFINITY ? 0.0f : -now;
+                const float2 shift2 = make_float2(shift, shift);
+                float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
                 if (FP8) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const float4 inverse = lds_f4(tile_scales + 2 * PA_KEYS * 4 + i * 16);
                         const uint32_t* r = &raw[i >> 3][(i & 7) * 4];
-                        const float p0 = pa_exp2(__uint_as_float(r[0]) - reference), p1 = pa_exp2(__uint_as_float(r[1]) - reference);
-                        const float p2 = pa_exp2(__uint_as_float(r[2]) - reference), p3 = pa_exp2(__uint_as_float(r[3]) - reference);
-                        partial_sum[0] = __fmaf_rn(p0, inverse.x, partial_sum[0]);
-                        partial_sum[1] = __fmaf_rn(p1, inverse.y, partial_sum[1]);
-                        partial_sum[2] = __fmaf_rn(p2, inverse.z, partial_sum[2]);
-                        partial_sum[3] = __fmaf_rn(p3, inverse.w, partial_sum[3]);
-                        packed[i >> 3][(i & 7) * 2] = float2_to_half2_bits(p0, p1);
-                        packed[i >> 3][(i & 7) * 2 + 1] = float2_to_half2_bits(p2, p3);
+                        const float2 a = __fadd2_rn(make_float2(__uint_as_float(r[0]), __uint_as_float(r[1])), shift2);
+                        const float2 c = __fadd2_rn(make_float2(__uint_as_float(r[2]), __uint_as_float(r[3])), shift2);
+                        const float2 p = make_float2(pa_exp2(a.x), pa_exp2(a.y)), q = make_float2(pa_exp2(c.x), pa_exp2(c.y));
+                        sum[0] = __ffma2_rn(p, make_float2(inverse.x, inverse.y), sum[0]);
+                        sum[1] = __ffma2_rn(q, make_float2(inverse.z, inverse.w), sum[1]);
+                        packed[2 * i] = float2_to_half2_bits(p.x, p.y);
+                        packed[2 * i + 1] = float2_to_half2_bits(q.x, q.y);
                     }
                 } else {
+                    const float2 factor2 = make_float2(factor, factor);
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
-                        const float p0 = pa_exp2(__fmaf_rn(__uint_as_float(raw[i >> 4][2 * (i & 15)]), factor, -reference));
-                        const float p1 = pa_exp2(__fmaf_rn(__uint_as_float(raw[i >> 4][2 * (i & 15) + 1]), factor, -reference));
-                        packed[i >> 4][i & 15] = float2_to_bf16x2(make_float2(p0, p1));
-                        partial_sum[i & 3] += p0 + p1;
+                        const float2 a = __ffma2_rn(make_float2(__uint_as_float(raw[i >> 4][2 * (i & 15)]), __uint_as_float(raw[i >> 4][2 * (i & 15) + 1])), factor2, shift2);
+                        const float2 p = make_float2(pa_exp2(a.x), pa_exp2(a.y));
+                        packed[i] = float2_to_bf16x2(p);
+                        sum[i & 1] = __fadd2_rn(sum[i & 1], p);
+                    }
+                    if (cursor.segment > 0) {
+                        mbar_wait(value_full + 8 * (j % STAGES), uint32_t(j / STAGES) & 1u, failed, args.status, STATUS_WAIT_EPILOGUE);
+                        const unsigned long long seen = valid >= PA_KEYS ? ~0ull : valid <= 0 ? 0ull : (1ull << valid) - 1ull;
+                        if ((*static_cast<volatile unsigned long long*>(bad_keys + j % STAGES) & seen) != 0ull) sum[0].x = __uint_as_float(0x7fc00000u);
                     }
                 }
-                if (!FP8 && cursor.segment > 0) {
-                    mbar_wait(value_full + 8 * (j % STAGES), uint32_t(j / STAGES) & 1u, failed, args.status, STATUS_WAIT_EPILOGUE);
-                    const unsigned long long seen = valid >= PA_KEYS ? ~0ull : valid <= 0 ? 0ull : (1ull << valid) - 1ull;
-                    if ((*static_cast<volatile unsigned long long*>(bad_keys + j % STAGES) & seen) != 0ull) partial_sum[0] = __uint_as_float(0x7fc00000u);
-                }
-                running_sum = running_sum * correction + ((partial_sum[0] + partial_sum[1]) + (partial_sum[2] + partial_sum[3]));
+                running_sum += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
             }
             if (FP8) {
                 __syncwarp();
                 if (lane == 0) mbar_arrive(scale_empty + 8 * stage);
             }
-            // the product of the tile before has read P and added to O
-            if (j > 0) {
-                mbar_wait(o_done, uint32_t(j - 1) & 1u, failed, args.status, STATUS_WAIT_EPILOGUE);
+            // the P that lies where this one goes has been read: that of the tile before, or of this group's last
+            if (j >= Shape::P_BUFFERS) {
+                const int last = j - Shape::P_BUFFERS;
+                mbar_wait(o_done + 8 * (last & 1), uint32_t(last >> 1) & 1u, failed, args.status, STATUS_WAIT_EPILOGUE);
                 tc_fence_after_sync();
-                if (__any_sync(0xffffffffu, correction != 1.0f)) {
+            }
+            pa_tmem_store(lane_address + Shape::TMEM_P + uint32_t(parity_group % Shape::P_BUFFERS) * 32, packed);      // 64 keys in 32 columns
+            if (j > 0 && __any_sync(0xffffffffu, correction != 1.0f)) {
+                // O holds the tiles before this one in units of the reference before: wait for the last of them
+                if (Shape::P_BUFFERS > 1) mbar_wait(o_done + 8 * (parity_group ^ 1), uint32_t((j - 1) >> 1) & 1u, failed, args.status, STATUS_WAIT_EPILOGUE);
+                tc_fence_after_sync();
 #pragma unroll 1
-                    for (int chunk = 0; chunk < D / 32; ++chunk) {
-                        uint32_t o[32];
-                        tmem_load_32x32(lane_address + Shape::TMEM_O + chunk * 32, o);
-                        tmem_load_wait();
+                for (int chunk = 0; chunk < D / 32; ++chunk) {
+                    uint32_t o[32];
+                    tmem_load_32x32(lane_address + Shape::TMEM_O + chunk * 32, o);
+                    tmem_load_wait();
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * correction);
-                        pa_tmem_store(lane_address + Shape::TMEM_O + chunk * 32, o);
-                    }
-                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * correction);
+                    pa_tmem_store(lane_address + Shape::TMEM_O + chunk * 32, o);
                 }
             }
-            // P: row `row`, 64 keys = 8 chunks of 16 bytes, chunk c stored at c ^ (row % 8)
-            const uint32_t p_row = p_smem + uint32_t(row >> 3) * 1024u + uint32_t(row & 7) * 128u;
-#pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                const uint32_t* four = &packed[c >> 2][(c & 3) * 4];
-                sts_u4(p_row + uint32_t((c ^ (row & 7)) * 16), four[0], four[1], four[2], four[3]);
-            }
-            fence_async_shared();
+            pa_tmem_store_wait();
             tc_fence_before_sync();
             __syncwarp();
-            if (lane == 0) mbar_arrive(p_ready);
-            if (j + 1 < num_tiles) cursor.next(start_tile + j + 1);
+            if (lane == 0) mbar_arrive(p_ready + 8 * parity_group);
         }
+        // ---- the two groups' sums; the later reference is the one O is held in
         if (num_tiles > 0) {
-            mbar_wait(o_done, uint32_t(num_tiles - 1) & 1u, failed, args.status, STATUS_WAIT_EPILOGUE);
+            mbar_wait(all_done, 0u, failed, args.status, STATUS_WAIT_EPILOGUE);
             tc_fence_after_sync();
+        }
+        row_reference[parity_group * PA_ROWS + row] = reference;      // what the last tile of this group left there, or -inf
+        row_exchange[parity_group * PA_ROWS + row] = running_sum;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        {
+            const float other_reference = row_reference[(parity_group ^ 1) * PA_ROWS + row], other_sum = row_exchange[(parity_group ^ 1) * PA_ROWS + row];
+            const float last = fmaxf(reference, other_reference);
+            if (other_reference != last) running_sum += other_sum * pa_exp2(other_reference - last);
+            else if (reference != last) running_sum = running_sum * pa_exp2(reference - last) + other_sum;
+            else running_sum += other_sum;
+            reference = last;
         }
         // the codes reached the tensor core as values times 2^-8
         constexpr float UNIT = FP8 ? 256.0f : 1.0f;
         const int work_index = kv_head * args.tiles + tile;
+        const int first_column = parity_group * (D / 2);          // each group stores half of the columns
         if (args.splits > 1) {
             const int64_t partial_row = (int64_t(work_index) * args.splits + split) * PA_ROWS + row;
             const int64_t total_rows = int64_t(args.tiles) * args.kv_heads * args.splits * PA_ROWS;
-            if (split == 0) args.row_offsets[int64_t(work_index) * PA_ROWS + row] = out_offset;
-            if (exists) *reinterpret_cast<float2*>(args.partial + total_rows * D + partial_row * 2) = make_float2(running_max, running_sum);
+            if (parity_group == 0) {
+                if (split == 0) args.row_offsets[int64_t(work_index) * PA_ROWS + row] = out_offset;
+                if (exists) *reinterpret_cast<float2*>(args.partial + total_rows * D + partial_row * 2) = make_float2(reference, running_sum);
+            }
             if (num_tiles > 0) {
-                float* destination = args.partial + partial_row * D;
+                float* destination = args.partial + partial_row * D + first_column;
 #pragma unroll 1
-                for (int chunk = 0; chunk < D / 64; ++chunk) {
+                for (int chunk = 0; chunk < D / 128; ++chunk) {
                     uint32_t o[2][32];
-                    tmem_load_32x32(lane_address + Shape::TMEM_O + chunk * 64, o[0]);
-                    tmem_load_32x32(lane_address + Shape::TMEM_O + chunk * 64 + 32, o[1]);
+                    tmem_load_32x32(lane_address + Shape::TMEM_O + first_column + chunk * 64, o[0]);
+                    tmem_load_32x32(lane_address + Shape::TMEM_O + first_column + chunk * 64 + 32, o[1]);
                     tmem_load_wait();
                     if (exists) {
 #pragma unroll
@@ -696,11 +761,11 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
             const bool empty = running_sum == 0.0f;
             const float inverse = UNIT / running_sum;
 #pragma unroll 1
-            for (int chunk = 0; chunk < D / 64; ++chunk) {
+            for (int chunk = 0; chunk < D / 128; ++chunk) {
                 uint32_t o[2][32];
                 if (num_tiles > 0) {
-                    tmem_load_32x32(lane_address + Shape::TMEM_O + chunk * 64, o[0]);
-                    tmem_load_32x32(lane_address + Shape::TMEM_O + chunk * 64 + 32, o[1]);
+                    tmem_load_32x32(lane_address + Shape::TMEM_O + first_column + chunk * 64, o[0]);
+                    tmem_load_32x32(lane_address + Shape::TMEM_O + first_column + chunk * 64 + 32, o[1]);
                     tmem_load_wait();
                 }
                 if (exists) {
@@ -713,8 +778,9 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
                             const float c = __uint_as_float(o[i >> 1][(i & 1) * 16 + 2 * v + 1]) * inverse;
                             words[v] = empty ? 0u : float2_to_bf16x2(make_float2(a, c));
                         }
-                        *reinterpret_cast<uint4*>(args.out + out_offset + chunk * 64 + i * 16) = make_uint4(words[0], words[1], words[2], words[3]);
-                        *reinterpret_cast<uint4*>(args.out + out_offset + chunk * 64 + i * 16 + 8) = make_uint4(words[4], words[5], words[6], words[7]);
+                        __nv_bfloat16* destination = args.out + out_offset + first_column + chunk * 64 + i * 16;
+                        *reinterpret_cast<uint4*>(destination) = make_uint4(words[0], words[1], words[2], words[3]);
+                        *reinterpret_cast<uint4*>(destination + 8) = make_uint4(words[4], words[5], words[6], words[7]);
                     }
                 }
             }
@@ -723,9 +789,10 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
         // ------------------------------------------------------------- bf16: values the tensor core must not see
         if (num_tiles > 0) {
             constexpr int CHUNKS = Shape::KV_ATOMS * 8;          // 16-byte chunks of a row
-            const int thread = (warp - 6) * 32 + lane;
-            PaCursor cursor(segment_first, segment_length, w.segments, start_tile);
+            const int thread = (warp - PA_VALUE_WARP) * 32 + lane;
+            PaCursor cursor(segment_first, w.segments, start_tile);
             for (int j = 0; j < num_tiles; ++j) {
+                cursor.seek(start_tile + j);
                 const int b = j % STAGES;
                 mbar_wait(v_full + 8 * b, uint32_t(j / STAGES) & 1u, failed, args.status, STATUS_WAIT_PRODUCER);
                 int valid = segment_length[cursor.segment] - cursor.offset * PA_KEYS;
@@ -735,7 +802,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
                     sts_u4(stage + uint32_t((i & (CHUNKS - 1)) >> 3) * Shape::KV_ATOM_BYTES + uint32_t(i / CHUNKS) * 128u + uint32_t(i & 7) * 16u, 0u, 0u, 0u, 0u);
                 if (cursor.segment > 0) {
                     if (thread == 0) bad_keys[b] = 0ull;
-                    asm volatile("bar.sync 1, %0;" ::"n"(32 * Shape::VALUE_WARPS) : "memory");
+                    asm volatile("bar.sync 2, %0;" ::"n"(32 * Shape::VALUE_WARPS) : "memory");
 #pragma unroll 4
                     for (int i = thread; i < valid * CHUNKS; i += 32 * Shape::VALUE_WARPS) {
                         const int key = i / CHUNKS;
@@ -750,15 +817,14 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
                 fence_async_shared();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(value_full + 8 * b);
-                if (j + 1 < num_tiles) cursor.next(start_tile + j + 1);
             }
         }
-    } else if (warp < 6 + Shape::VALUE_WARPS) {
+    } else if (warp < PA_VALUE_WARP + Shape::VALUE_WARPS) {
         // ------------------------------------------------------------- codes of the value tile -> f16 operand
         // 16 codes of a key per thread and step: chunk `piece` of its row (stored at piece ^ (key % 8) inside its 128-byte group)
         // becomes two 16-byte chunks of the 64-column group they belong to.
         constexpr int PIECES = D / 16;
-        const int thread = (warp - 6) * 32 + lane;
+        const int thread = (warp - PA_VALUE_WARP) * 32 + lane;
         for (int j = 0; j < num_tiles; ++j) {
             const int b = j % STAGES, c = j & 1;
             mbar_wait(v_full + 8 * b, uint32_t(j / STAGES) & 1u, failed, args.status, STATUS_WAIT_PRODUCER);
@@ -784,35 +850,40 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
             }
         }
     } else if (num_tiles > 0) {
-        // ------------------------------------------------------------- scales of the key tile
-        PaCursor cursor(segment_first, segment_length, w.segments, start_tile);
-        for (int j = 0; j < num_tiles; ++j) {
-            const int stage = j % PA_SCALE_STAGES;
+        // ------------------------------------------------------------- scales of the key tile, loaded a tile ahead
+        PaCursor cursor(segment_first, w.segments, start_tile);
+        float ks[2], vs[2];
+        auto load = [&](int j) {
+            cursor.seek(start_tile + j);
             const bool prefix = cursor.segment == 0;
             const int sequence = prefix ? w.group : w.first_member + w.first_segment_member + cursor.segment - 1;
             const int64_t first = (int64_t(sequence) * args.kv_heads + kv_head) * (prefix ? args.prefix_capacity : args.own_capacity) + cursor.offset * PA_KEYS;
             const int valid = segment_length[cursor.segment] - cursor.offset * PA_KEYS;
             const float* key_scales = (prefix ? args.prefix_scales[0] : args.own_scales[0]) + first;
             const float* value_scales = (prefix ? args.prefix_scales[1] : args.own_scales[1]) + first;
-            float ks[2], vs[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const bool inside = lane + 32 * i < valid;
                 ks[i] = inside ? __ldg(key_scales + lane + 32 * i) : 0.0f;
                 vs[i] = inside ? __ldg(value_scales + lane + 32 * i) : 0.0f;
             }
+        };
+        load(0);
+        for (int j = 0; j < num_tiles; ++j) {
+            const int stage = j % PA_SCALE_STAGES;
+            const float key_scale[2] = {ks[0], ks[1]}, value_scale[2] = {vs[0], vs[1]};
+            if (j + 1 < num_tiles) load(j + 1);
             mbar_wait(scale_empty + 8 * stage, (uint32_t(j / PA_SCALE_STAGES) & 1u) ^ 1u, failed, args.status, STATUS_WAIT_PRODUCER);
             float* out = reinterpret_cast<float*>(generic + Shape::OFF_SCALES) + stage * PA_SCALE_FLOATS;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const float value = vs[i] == 0.0f ? PA_ZERO_ROW_SCALE : vs[i];
-                out[lane + 32 * i] = ks[i];
+                const float value = value_scale[i] == 0.0f ? PA_ZERO_ROW_SCALE : value_scale[i];
+                out[lane + 32 * i] = key_scale[i];
                 out[PA_KEYS + lane + 32 * i] = log2f(value);
                 out[2 * PA_KEYS + lane + 32 * i] = value == value ? 1.0f / value : 0.0f;      // NaN reaches the rows that see it by its logarithm
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(scale_full + 8 * stage);
-            if (j + 1 < num_tiles) cursor.next(start_tile + j + 1);
         }
     }
 
@@ -820,7 +891,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
     __syncthreads();
     if (warp == 1) {
         tc_fence_after_sync();
-        tmem_dealloc(tmem_base, Shape::TMEM_COLUMNS_USED);
+        tmem_dealloc(tmem_base, TMEM_COLUMNS);
     }
 }
 
