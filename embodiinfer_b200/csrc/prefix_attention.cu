@@ -30,14 +30,13 @@
 //   2^e bringing the row's largest value into [128, 256): a bf16 value has 8 significant bits, hi takes 4 and lo the rest,
 //   exactly, down to 2^-18 of the row's largest value.  Two products at twice the bf16 rate cost what one bf16 product
 //   would, and no key is ever converted.  ks multiplies the score.
-//   Output.  The four value warps turn the codes into f16 (exact: the code's bits shifted into place are the value times
-//   2^-8).  vs cannot be divided out afterwards, so it joins the probability:
-//       w = 2^(s + log2 vs - M),   O = sum w v,   L = sum w / vs,   out = O / L
-//   with M the running reference of s + log2 vs: the weights that meet the values are at most 2^8, whatever the spread of the
-//   scales, and f16 with its 11 bits is enough (bf16 probabilities would double the error of the result; two e4m3 halves, which
+//   Output.  The four value warps turn the codes into f16, exactly, and multiply by vs 2^-E: one rounding of 2^-11 for the scale and one for the product, beside the 2^-9 of the result.  2^E is the unit
+//   of the accumulator, the same for all rows: it follows the largest vs of a key tile when that leaves [2^-10, 2^6) units, and
+//   the accumulator is rescaled then as it is for a new reference.  A value keeps its precision as long as its scale is within
+//   2^-20 of the largest in its tile of 64 keys, whatever the scales of other tiles are.  P is f16 as well: with its 11 bits the
+//   result is as exact as its own rounding allows (bf16 probabilities would add as much error again; two e4m3 halves, which
 //   would spare the conversion of V, have no room for a long tail of weights 2^-15 below the largest).
-//   A row whose scale is 0 holds zeros; it takes part in L alone, with a vs below every scale that the cache's write leaves
-//   (2^-59 to 2^32), so that it never sets M.
+//   A scale that is not finite zeroes its row of values and marks the key: rows that see it get NaN from their sum.
 //
 // Few CTAs: the key tiles of a row tile are cut across `splits` CTAs, which leave O, M and L in fp32 in the workspace; a second
 // launch joins them in split order (no atomics: the result does not depend on timing).
@@ -46,16 +45,23 @@
 #include <cuda.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 namespace b2 {
 
 namespace {
 
 constexpr int PA_ROWS = 128;                     // query rows per CTA
 constexpr int PA_KEYS = 64;                      // keys per tile
-constexpr int PA_SOFTMAX_WARP = 2, PA_VALUE_WARP = 10;      // first softmax warp (of 8), first value warp
-constexpr int PA_SCALE_STAGES = 4;
-constexpr int PA_SCALE_FLOATS = 3 * PA_KEYS;     // ks, log2 vs, 1 / vs of a key tile
-constexpr float PA_ZERO_ROW_SCALE = 8.6736173798840355e-19f;      // 2^-60
+constexpr int PA_LOAD_WARP = 8, PA_SCORES_WARP = 9, PA_OUTPUT_WARP = 10, PA_SCALE_WARP = 11, PA_VALUE_WARP = 12, PA_WARPS = 16;      // 0-7: softmax
+// Registers per thread: 128 at launch (512 threads); the softmax warpgroups take what the others give up.
+constexpr int PA_SOFTMAX_REGISTERS = 168, PA_OTHER_REGISTERS = 88;
+static_assert(256 * PA_SOFTMAX_REGISTERS + (PA_WARPS * 32 - 256) * PA_OTHER_REGISTERS <= PA_WARPS * 32 * 128, "registers of the launch");
+constexpr int PA_PATIENCE = 1 << 24;              // tries of a wait: some 30 cycles each at least, half a second in all
+constexpr int PA_SCALE_STAGES = 4, PA_RAW_STAGES = 8;      // of the quantised cache's scales: as the softmax reads them; as they come
+// A key tile's scales as the roles read them: ks, vs in units as pairs of halves, then bits of keys whose vs is not finite (2 words), the
+// unit, and the unit of the tile before less this one (exponents).
+constexpr int PA_SCALE_FLOATS = 2 * PA_KEYS + 4;
 constexpr int PA_MAX_SEGMENTS = PA_ROWS + 1;     // the prefix and at most one member per row
 
 template <int D, bool FP8>
@@ -68,20 +74,22 @@ struct PaShape {
     static constexpr int STAGES = D == 256 ? (FP8 ? 4 : 3) : (FP8 ? 8 : 6); // of the K and the V ring each
     static constexpr int VALUE_STAGES = FP8 ? 2 : 0;                        // converted value tiles
     static constexpr uint32_t VALUE_BYTES = PA_KEYS * D * 2;
-    static constexpr int VALUE_WARPS = FP8 ? 4 : 2;
-    static constexpr int WARPS = PA_VALUE_WARP + VALUE_WARPS + (FP8 ? 1 : 0);   // + the scale warp
-    static constexpr int THREADS = WARPS * 32;
-    // Q: atoms of 32 columns (64 bf16 or 128 e4m3 values of a row).  With D = 256 there is room for three of the four, and for one P;
-    // the last atom of Q lies in shared memory.
-    static constexpr int Q_ATOMS = D / 64, Q_TMEM_ATOMS = Q_ATOMS < 3 ? Q_ATOMS : 3, P_BUFFERS = D == 256 ? 1 : 2;
-    static constexpr uint32_t TMEM_S = 0, TMEM_O = 2 * PA_KEYS, TMEM_Q = TMEM_O + D, TMEM_P = TMEM_Q + Q_TMEM_ATOMS * 32;
+    static constexpr int VALUE_WARPS = 4;
+    static constexpr int THREADS = PA_WARPS * 32;
+    // With D = 128 each softmax group has an accumulator of its own and never meets the other before the end; with D = 256 there is
+    // room for one accumulator and one P, and for three of Q's four atoms (32 columns: 64 bf16 or 128 e4m3 values of a row): the last one
+    // lies in shared memory.
+    static constexpr bool SHARED = D == 256;
+    static constexpr int Q_ATOMS = D / 64, Q_TMEM_ATOMS = Q_ATOMS < 3 ? Q_ATOMS : 3, P_BUFFERS = SHARED ? 1 : 2, O_BUFFERS = SHARED ? 1 : 2;
+    static constexpr uint32_t TMEM_S = 0, TMEM_O = 2 * PA_KEYS, TMEM_Q = TMEM_O + O_BUFFERS * D, TMEM_P = TMEM_Q + Q_TMEM_ATOMS * 32;
     static_assert(TMEM_P + P_BUFFERS * 32 <= TMEM_COLUMNS, "tensor memory");
     static constexpr uint32_t OFF_K = 0;
     static constexpr uint32_t OFF_V = OFF_K + STAGES * KV_BYTES;
     static constexpr uint32_t OFF_VALUES = OFF_V + STAGES * KV_BYTES;
     static constexpr uint32_t OFF_Q = OFF_VALUES + VALUE_STAGES * VALUE_BYTES;
     static constexpr uint32_t OFF_SCALES = OFF_Q + (Q_ATOMS - Q_TMEM_ATOMS) * PA_ROWS * 128;
-    static constexpr uint32_t OFF_ROWS = OFF_SCALES + (FP8 ? PA_SCALE_STAGES * PA_SCALE_FLOATS * 4 : 0);      // float [2][128], twice
+    static constexpr uint32_t OFF_RAW_SCALES = OFF_SCALES + (FP8 ? PA_SCALE_STAGES * PA_SCALE_FLOATS * 4 : 0);
+    static constexpr uint32_t OFF_ROWS = OFF_RAW_SCALES + (FP8 ? PA_RAW_STAGES * 2 * PA_KEYS * 4 : 0);      // float [2][128], twice
     static constexpr uint32_t OFF_SEGMENTS = OFF_ROWS + 4 * PA_ROWS * 4;
     static constexpr uint32_t OFF_BARS = OFF_SEGMENTS + (PA_MAX_SEGMENTS + 3) * 8;
     static constexpr int SHARED_BYTES = 1024 + int(OFF_BARS) + 768;
@@ -198,12 +206,6 @@ __device__ __forceinline__ uint4 lds_u4(uint32_t address) {
     return v;
 }
 
-__device__ __forceinline__ float4 lds_f4(uint32_t address) {
-    float4 v;
-    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(address) : "memory");
-    return v;
-}
-
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 __device__ __forceinline__ uint32_t float2_to_half2_bits(float a, float b) {
@@ -211,11 +213,14 @@ __device__ __forceinline__ uint32_t float2_to_half2_bits(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&pair);
 }
 
-// Two e4m3 codes in the low half of `codes` -> two f16 holding the values times 2^-8: sign to the top bit, the other seven
-// bits under the f16 exponent's top bit (subnormal codes are subnormal halves).
-__device__ __forceinline__ uint32_t codes_to_halves(uint32_t codes, uint32_t selector) {
-    const uint32_t spread = __byte_perm(codes, 0u, selector);          // code 0 in byte 1, code 1 in byte 3
-    return (spread & 0x80008000u) | ((spread & 0x7f007f00u) >> 1);
+// Two e4m3 codes in the low half of `codes` -> two f16 of the values times `scale`.  CLEAN: codes that are NaN become 448, for tiles
+// with rows that some queries pass over with probability zero.
+template <bool CLEAN>
+__device__ __forceinline__ uint32_t codes_to_halves(uint32_t codes, __half2 scale) {
+    __half2 value(__nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(codes), __NV_E4M3));
+    if (CLEAN) value = __hmin2(value, __float2half2_rn(448.0f));
+    value = __hmul2(value, scale);
+    return *reinterpret_cast<const uint32_t*>(&value);
 }
 
 // Whether one of the two bf16 values of a word is an infinity or a NaN.
@@ -223,23 +228,53 @@ __device__ __forceinline__ bool has_not_finite(uint32_t word) {
     return (word & 0x7f80u) == 0x7f80u || (word & 0x7f800000u) == 0x7f800000u;
 }
 
+// Bounded wait, as small as it can be made: the roles' loops have to share the instruction caches.  `patience` is the number of tries; once
+// they have run out it stays 0, every later wait of the thread gives up at once, and the role reports it when it ends.
+__device__ __forceinline__ void pa_wait(uint32_t bar, uint32_t parity, int& patience) {
+    int tries = patience;
+    while (!mbar_try_wait(bar, parity))
+        if (--tries <= 0) {
+            patience = 0;
+            break;
+        }
+}
+
 // Walks the key tiles of a CTA: the prefix (segment 0), then the own keys of its members.
 struct PaCursor {
     const int* first_tile;      // [segments + 1], shared memory
-    int segment, offset;        // offset: key tile inside the segment
-    __device__ __forceinline__ PaCursor(const int* first, int segments, int tile) : first_tile(first), segment(0), offset(0) {
-        int low = 0, high = segments;      // the last segment that starts at or before `tile`; empty ones are passed over
-        while (high - low > 1) {
-            const int middle = (low + high) >> 1;
-            if (first[middle] <= tile) low = middle;
-            else high = middle;
-        }
-        segment = low;
-        offset = tile - first[low];
+    const int* length;          // [segments]
+    int segment, start, end, keys_left;      // of the segment: its tiles and the keys from its tile `start` on
+    __device__ __forceinline__ PaCursor(const int* first, const int* lengths, int tile) : first_tile(first), length(lengths), segment(-1), start(0), end(-1), keys_left(0) {
+        seek(tile);
     }
-    __device__ __forceinline__ void seek(int tile) {          // forward to `tile`, which exists
-        while (first_tile[segment + 1] <= tile) ++segment;
-        offset = tile - first_tile[segment];
+    __device__ __forceinline__ void seek(int tile) {          // forward to `tile`; empty segments are passed over
+        while (tile >= end) {
+            ++segment;
+            start = first_tile[segment];
+            end = first_tile[segment + 1];
+            keys_left = length[segment];
+        }
+    }
+    __device__ __forceinline__ int first_key(int tile) const { return (tile - start) * PA_KEYS; }
+    __device__ __forceinline__ int keys(int tile) const {          // of this tile: 1 to PA_KEYS
+        const int left = keys_left - first_key(tile);
+        return left < PA_KEYS ? left : PA_KEYS;
+    }
+};
+
+// A place in a ring of slots and the parity of its current use.
+template <int SLOTS>
+struct PaRing {
+    int slot = 0;
+    uint32_t parity = 0;
+    __device__ __forceinline__ void next() {
+        if (++slot == SLOTS) {
+            slot = 0;
+            parity ^= 1u;
+        }
+    }
+    __device__ __forceinline__ void next(int count) {
+        for (int i = 0; i < count; ++i) next();
     }
 };
 
@@ -254,9 +289,10 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
     const uint32_t base = (smem_u32(shared_raw) + 1023u) & ~1023u;
     uint8_t* const generic = shared_raw + (base - smem_u32(shared_raw));
     const uint32_t k_smem = base + Shape::OFF_K, v_smem = base + Shape::OFF_V, values_smem = base + Shape::OFF_VALUES;
-    const uint32_t q_smem = base + Shape::OFF_Q, scales_smem = base + Shape::OFF_SCALES;
+    const uint32_t q_smem = base + Shape::OFF_Q;
     float* const row_reference = reinterpret_cast<float*>(generic + Shape::OFF_ROWS);           // [2][128]: of the latest even and odd tile
     float* const row_exchange = row_reference + 2 * PA_ROWS;                                    // [2][128]: row maxima of Q, then the sums
+    int* const group_unit = reinterpret_cast<int*>(generic + Shape::OFF_BARS + 720);          // [2]: last units of the accumulators, as exponents
     int* const segment_first = reinterpret_cast<int*>(generic + Shape::OFF_SEGMENTS);
     int* const segment_length = segment_first + PA_MAX_SEGMENTS + 3;
     const uint32_t bars = base + Shape::OFF_BARS;
@@ -296,7 +332,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
         }
         for (int i = 0; i < PA_SCALE_STAGES; ++i) {
             mbar_init(scale_full + 8 * i, 1);
-            mbar_init(scale_empty + 8 * i, 4);
+            mbar_init(scale_empty + 8 * i, 4 + Shape::VALUE_WARPS);
         }
         for (int i = 0; i < 8; ++i) mbar_init(reference_ready + 8 * i, 1);
         mbar_init(all_done, 1);
@@ -307,12 +343,12 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
         tma_prefetch_descriptor(&own_k_map);
         tma_prefetch_descriptor(&own_v_map);
     }
-    if (warp == 1) {
+    if (warp == PA_SCORES_WARP) {
         tmem_alloc(tmem_slot, TMEM_COLUMNS);
         tmem_relinquish();
     }
     pdl_wait();
-    if (warp == 0) {
+    if (warp == PA_LOAD_WARP) {
         // ---- which rows, which keys
         int group = -1, first = 0, count = 0, group_tile = 0;
         if (args.members == nullptr) {
@@ -393,111 +429,12 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
     const int start_tile = int(int64_t(w.key_tiles) * split / args.splits);
     const int num_tiles = int(int64_t(w.key_tiles) * (split + 1) / args.splits) - start_tile;
 
-    bool failed = false;
-    if (warp == 0) {
-        // ------------------------------------------------------------- TMA producer
-        if (num_tiles > 0) {
-            PaCursor cursor(segment_first, w.segments, start_tile);
-            for (int j = 0; j < num_tiles; ++j) {
-                cursor.seek(start_tile + j);
-                const int b = j % STAGES;
-                const uint32_t parity = uint32_t(j / STAGES) & 1u;
-                const bool prefix = cursor.segment == 0;
-                const CUtensorMap* k_map = prefix ? &prefix_k_map : &own_k_map;
-                const CUtensorMap* v_map = prefix ? &prefix_v_map : &own_v_map;
-                const int sequence = prefix ? w.group : w.first_member + w.first_segment_member + cursor.segment - 1;
-                const int row = (sequence * args.kv_heads + kv_head) * (prefix ? args.prefix_capacity : args.own_capacity) + cursor.offset * PA_KEYS;
-                mbar_wait(k_empty + 8 * b, parity ^ 1u, failed, args.status, STATUS_WAIT_PRODUCER);
-                __syncwarp();
-                if (elect_one()) {
-                    mbar_expect_tx(k_full + 8 * b, Shape::KV_BYTES);
-                    for (int a = 0; a < Shape::KV_ATOMS; ++a)
-                        tma_load_2d(k_smem + b * Shape::KV_BYTES + a * Shape::KV_ATOM_BYTES, k_map, k_full + 8 * b, a * 128, row);
-                }
-                __syncwarp();
-                mbar_wait(v_empty + 8 * b, parity ^ 1u, failed, args.status, STATUS_WAIT_PRODUCER);
-                __syncwarp();
-                if (elect_one()) {
-                    mbar_expect_tx(v_full + 8 * b, Shape::KV_BYTES);
-                    for (int a = 0; a < Shape::KV_ATOMS; ++a)
-                        tma_load_2d(v_smem + b * Shape::KV_BYTES + a * Shape::KV_ATOM_BYTES, v_map, v_full + 8 * b, a * 128, row);
-                }
-                __syncwarp();
-            }
-            // every copy has landed before this CTA may leave (on the normal path the readers have long seen them)
-            bool drain_failed = false;
-            for (int b = 0; b < STAGES && b < num_tiles; ++b) {
-                const int last = ((num_tiles - 1 - b) / STAGES) * STAGES + b;
-                mbar_wait(k_full + 8 * b, uint32_t(last / STAGES) & 1u, drain_failed, args.status, STATUS_WAIT_DRAIN);
-                mbar_wait(v_full + 8 * b, uint32_t(last / STAGES) & 1u, drain_failed, args.status, STATUS_WAIT_DRAIN);
-            }
-        }
-    } else if (warp == 1) {
-        // ------------------------------------------------------------- MMA issuer
-        const uint32_t idesc_scores = FP8 ? idesc_f8(PA_ROWS, PA_KEYS) : pa_idesc_16bit(PA_ROWS, PA_KEYS, true, false);
-        const uint32_t idesc_output = pa_idesc_16bit(PA_ROWS, D, !FP8, true);
-        const uint64_t k_major = smem_desc_sw128(0), mn_major = pa_desc_mn(Shape::KV_ATOM_BYTES);
-        const uint32_t k_low = uint32_t(k_major), k_high = uint32_t(k_major >> 32);
-        const uint32_t mn_low = uint32_t(mn_major), mn_high = uint32_t(mn_major >> 32);
-        auto field = [](uint32_t address) { return (address & 0x3FFFFu) >> 4; };
-        if (num_tiles > 0) mbar_wait(q_ready, 0u, failed, args.status, STATUS_WAIT_MMA_FULL);
-        tc_fence_after_sync();
-        auto scores = [&](int j) {          // S[j & 1] = Q K_j^T
-            const int b = j % STAGES, d = j & 1;
-            mbar_wait(k_full + 8 * b, uint32_t(j / STAGES) & 1u, failed, args.status, STATUS_WAIT_MMA_FULL);
-            mbar_wait(s_free + 8 * d, (uint32_t(j >> 1) & 1u) ^ 1u, failed, args.status, STATUS_WAIT_MMA_TMEM);
-            tc_fence_after_sync();
-            __syncwarp();
-            if (elect_one()) {
-                const uint32_t d_tmem = tmem_base + Shape::TMEM_S + uint32_t(d) * PA_KEYS;
-                const uint32_t k_base = k_low + field(k_smem + b * Shape::KV_BYTES);
-                // 32 bytes along K per instruction: 8 columns of Q.  Quantised: first all of hi, then all of lo.
-#pragma unroll
-                for (int a = 0; a < Shape::Q_ATOMS; ++a)
-#pragma unroll
-                    for (int s = 0; s < 4; ++s) {
-                        const uint64_t k_desc = desc_from_words(k_base + (a % Shape::KV_ATOMS) * (Shape::KV_ATOM_BYTES >> 4) + 2 * s, k_high);
-                        if (a < Shape::Q_TMEM_ATOMS) pa_mma<FP8>(d_tmem, tmem_base + Shape::TMEM_Q + uint32_t((a * 4 + s) * 8), k_desc, idesc_scores, (a | s) != 0);
-                        else pa_mma_shared<FP8>(d_tmem, desc_from_words(k_low + field(q_smem) + 2 * s, k_high), k_desc, idesc_scores, 1u);
-                    }
-                tc_commit(k_empty + 8 * b);
-                tc_commit(s_full + 8 * d);
-            }
-            __syncwarp();
-        };
-        auto output = [&](int j) {          // O += P V_j
-            const int b = FP8 ? (j & 1) : j % STAGES, d = j & 1;
-            const uint32_t parity = uint32_t(FP8 ? j >> 1 : j / STAGES) & 1u;
-            mbar_wait(value_full + 8 * b, parity, failed, args.status, STATUS_WAIT_MMA_FULL);
-            mbar_wait(p_ready + 8 * d, uint32_t(j >> 1) & 1u, failed, args.status, STATUS_WAIT_MMA_TMEM);
-            // One output at a time: who has seen the output of tile j - 2 done can tell by its parity whether that of j - 1 is.  The
-            // scores issued in between keep the tensor core busy.
-            if (j > 0) mbar_wait(o_done + 8 * (d ^ 1), uint32_t((j - 1) >> 1) & 1u, failed, args.status, STATUS_WAIT_MMA_TMEM);
-            tc_fence_after_sync();
-            __syncwarp();
-            if (elect_one()) {
-                const uint32_t p_tmem = tmem_base + Shape::TMEM_P + uint32_t(d % Shape::P_BUFFERS) * 32;
-                const uint32_t v_base = mn_low + field(FP8 ? values_smem + b * Shape::VALUE_BYTES : v_smem + b * Shape::KV_BYTES);
-#pragma unroll
-                for (int s = 0; s < PA_KEYS / 16; ++s)          // 16 keys per instruction: 8 columns of P, 16 rows (2048 bytes) of V
-                    pa_mma<false>(tmem_base + Shape::TMEM_O, p_tmem + 8 * s, desc_from_words(v_base + s * (2048 >> 4), mn_high), idesc_output, (j | s) != 0);
-                tc_commit((FP8 ? value_empty : v_empty) + 8 * b);
-                tc_commit(o_done + 8 * d);
-            }
-            __syncwarp();
-        };
-        if (num_tiles > 0) scores(0);
-        if (num_tiles > 1) scores(1);
-        for (int j = 0; j < num_tiles; ++j) {
-            if (j + 2 < num_tiles) scores(j + 2);          // as soon as its group has the scores of tile j in registers
-            output(j);
-        }
-        if (num_tiles > 0 && elect_one()) tc_commit(all_done);
-        __syncwarp();
-    } else if (warp < PA_VALUE_WARP) {
+    int patience = PA_PATIENCE;
+    if (warp < 8) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PA_SOFTMAX_REGISTERS));
         // ------------------------------------------------------------- one thread per query row and tile parity
         const int quarter = warp & 3, row = quarter * 32 + lane;          // row of the tile = tensor-memory lane
-        const int parity_group = (warp - PA_SOFTMAX_WARP) >> 2;           // 0: even tiles, 1: odd tiles
+        const int parity_group = warp >> 2;           // 0: even tiles, 1: odd tiles
         const uint32_t lane_address = tmem_base + (uint32_t(quarter * 32) << 16);
         const bool exists = row < w.rows;
         int my_segment = -1, hidden = 0;          // the segment of this row's own keys; causal: how many of them lie behind the query
@@ -576,41 +513,45 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
             if (lane == 0) mbar_arrive(q_ready);
         }
         float reference = -INFINITY, running_sum = 0.0f;          // of this group's tiles so far: the sum in units of 2^reference
-        PaCursor cursor(segment_first, w.segments, start_tile);
-        for (int j = parity_group; j < num_tiles; j += 2) {
+        int unit = 0;                                             // of the values in its accumulator, as an exponent
+        const uint32_t s_tmem = lane_address + Shape::TMEM_S + uint32_t(parity_group) * PA_KEYS;
+        const uint32_t p_tmem = lane_address + Shape::TMEM_P + uint32_t(parity_group % Shape::P_BUFFERS) * 32;
+        const uint32_t o_tmem = lane_address + Shape::TMEM_O + uint32_t(parity_group % Shape::O_BUFFERS) * D;
+        PaCursor cursor(segment_first, segment_length, parity_group < num_tiles ? start_tile + parity_group : -1);
+        uint32_t phase = 0;                                       // of this group's barriers: (j / 2) % 2
+        for (int j = parity_group; j < num_tiles; j += 2, phase ^= 1u) {
             cursor.seek(start_tile + j);
-            const uint32_t s_tmem = lane_address + Shape::TMEM_S + uint32_t(parity_group) * PA_KEYS;
             // keys of this tile that this row sees: the first `valid`
-            int valid = 0;
-            if (exists) {
-                if (cursor.segment == 0) valid = segment_length[0] - cursor.offset * PA_KEYS;
-                else if (cursor.segment == my_segment) valid = segment_length[cursor.segment] - hidden - cursor.offset * PA_KEYS;
+            int valid = cursor.keys_left - cursor.first_key(start_tile + j);
+            bool whole = valid >= PA_KEYS, none = false;
+            if (cursor.segment > 0) {
+                valid = cursor.segment == my_segment ? valid - hidden : 0;
+                whole = __all_sync(0xffffffffu, valid >= PA_KEYS);
+                none = __all_sync(0xffffffffu, valid <= 0);
             }
-            const bool whole = __all_sync(0xffffffffu, valid >= PA_KEYS), none = __all_sync(0xffffffffu, valid <= 0);
-            mbar_wait(s_full + 8 * parity_group, uint32_t(j >> 1) & 1u, failed, args.status, STATUS_WAIT_EPILOGUE);
+            const int stage = j % PA_SCALE_STAGES;
+            const float4* tile_scales = reinterpret_cast<const float4*>(generic + Shape::OFF_SCALES) + stage * (PA_SCALE_FLOATS / 4);
+            if (FP8) pa_wait(scale_full + 8 * stage, uint32_t(j / PA_SCALE_STAGES) & 1u, patience);
+            pa_wait(s_full + 8 * parity_group, phase, patience);
             tc_fence_after_sync();
             uint32_t raw[2][32];
-            const int stage = j % PA_SCALE_STAGES;
-            const uint32_t tile_scales = scales_smem + uint32_t(stage) * PA_SCALE_FLOATS * 4;
             if (!none) {
                 tmem_load_32x32(s_tmem, raw[0]);
                 tmem_load_32x32(s_tmem + 32, raw[1]);
+                tmem_load_wait();
             }
-            if (FP8) mbar_wait(scale_full + 8 * stage, uint32_t(j / PA_SCALE_STAGES) & 1u, failed, args.status, STATUS_WAIT_EPILOGUE);
-            float tile_max = -INFINITY;
-            if (!none) tmem_load_wait();
             tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(s_free + 8 * parity_group);
+            float tile_max = -INFINITY;
             if (!none) {
-                if (FP8) {      // score in units of log2, + log2 vs
-                    const float2 factor2 = make_float2(factor, factor);
+                if (FP8) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const float4 ks = lds_f4(tile_scales + i * 16), lv = lds_f4(tile_scales + PA_KEYS * 4 + i * 16);
+                        const float4 ks = tile_scales[i];
                         uint32_t* r = &raw[i >> 3][(i & 7) * 4];
-                        const float2 a = __ffma2_rn(__fmul2_rn(make_float2(__uint_as_float(r[0]), __uint_as_float(r[1])), make_float2(ks.x, ks.y)), factor2, make_float2(lv.x, lv.y));
-                        const float2 c = __ffma2_rn(__fmul2_rn(make_float2(__uint_as_float(r[2]), __uint_as_float(r[3])), make_float2(ks.z, ks.w)), factor2, make_float2(lv.z, lv.w));
+                        const float2 a = __fmul2_rn(make_float2(__uint_as_float(r[0]), __uint_as_float(r[1])), make_float2(ks.x, ks.y));
+                        const float2 c = __fmul2_rn(make_float2(__uint_as_float(r[2]), __uint_as_float(r[3])), make_float2(ks.z, ks.w));
                         r[0] = __float_as_uint(a.x); r[1] = __float_as_uint(a.y); r[2] = __float_as_uint(c.x); r[3] = __float_as_uint(c.y);
                     }
                 }
@@ -623,111 +564,128 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
 #pragma unroll
                 for (int i = 0; i < 32; ++i)
                     partial_max[i & 3] = fmaxf(fmaxf(partial_max[i & 3], __uint_as_float(raw[0][i])), __uint_as_float(raw[1][i]));
-                tile_max = fmaxf(fmaxf(partial_max[0], partial_max[1]), fmaxf(partial_max[2], partial_max[3]));
-                if (!FP8) tile_max *= factor;
+                tile_max = fmaxf(fmaxf(partial_max[0], partial_max[1]), fmaxf(partial_max[2], partial_max[3])) * factor;
             }
-            // The reference of the tile before comes from the other group.  It follows the maximum lazily: it moves only when the
-            // maximum has grown by more than 2^8 since it was set, so weights stay below 2^8 and the accumulator is rescaled a few
-            // times per row.  A row that has seen no key yet has none; 0 stands in, its weights are 0.
-            float previous = -INFINITY;
-            if (j > 0) {
+            // The reference follows the maximum lazily: it moves only when the maximum has grown by more than 2^8 since it was set, so
+            // weights stay below 2^8 and the accumulator is rescaled a few times per row.  A row that has seen no key yet has none; 0
+            // stands in, its weights are 0.  With one accumulator the reference of the tile before comes from the other group.
+            float previous = reference;
+            if (Shape::SHARED && j > 0) {
                 const int other = parity_group ^ 1;
-                mbar_wait(reference_ready + 16 * quarter + 8 * other, uint32_t((j - 1) >> 1) & 1u, failed, args.status, STATUS_WAIT_EPILOGUE);
+                pa_wait(reference_ready + 16 * quarter + 8 * other, parity_group == 0 ? phase ^ 1u : phase, patience);
                 previous = *static_cast<volatile float*>(row_reference + other * PA_ROWS + row);
             }
             const float now = tile_max > previous + 8.0f ? tile_max : previous;
-            *static_cast<volatile float*>(row_reference + parity_group * PA_ROWS + row) = now;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(reference_ready + 16 * quarter + 8 * parity_group);
-            const float correction = now == previous ? 1.0f : pa_exp2(previous - now);
-            if (now != reference) running_sum *= pa_exp2(reference - now);
+            if (Shape::SHARED) {
+                *static_cast<volatile float*>(row_reference + parity_group * PA_ROWS + row) = now;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(reference_ready + 16 * quarter + 8 * parity_group);
+            }
+            // what O holds is in units of the reference before (a row without one has nothing but zeros there) and of the values' unit before
+            float correction = now == previous || previous == -INFINITY ? 1.0f : pa_exp2(previous - now);
+            running_sum *= Shape::SHARED ? (now == reference ? 1.0f : pa_exp2(reference - now)) : correction;
             reference = now;
+            unsigned long long bad = 0ull;          // keys that give NaN to the rows that see them
+            if (FP8) {
+                const float4 entry = tile_scales[2 * PA_KEYS / 4];
+                bad = __float_as_uint(entry.x) | (static_cast<unsigned long long>(__float_as_uint(entry.y)) << 32);
+                const int tile_unit = __float_as_int(Shape::SHARED ? entry.w : entry.z);
+                if (Shape::SHARED) {          // the change from the tile before
+                    if (tile_unit != 0) correction *= exp2f(float(tile_unit));
+                } else {
+                    if (j >= 2 && tile_unit != unit) correction *= exp2f(float(unit - tile_unit));
+                    unit = tile_unit;
+                }
+            }
             uint32_t packed[32];
             if (none) {
 #pragma unroll
                 for (int i = 0; i < 32; ++i) packed[i] = 0u;
             } else {
                 const float shift = now == -INFINITY ? 0.0f : -now;
-                const float2 shift2 = make_float2(shift, shift);
+                const float2 shift2 = make_float2(shift, shift), factor2 = make_float2(factor, factor);
                 float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-                if (FP8) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float4 inverse = lds_f4(tile_scales + 2 * PA_KEYS * 4 + i * 16);
-                        const uint32_t* r = &raw[i >> 3][(i & 7) * 4];
-                        const float2 a = __fadd2_rn(make_float2(__uint_as_float(r[0]), __uint_as_float(r[1])), shift2);
-                        const float2 c = __fadd2_rn(make_float2(__uint_as_float(r[2]), __uint_as_float(r[3])), shift2);
-                        const float2 p = make_float2(pa_exp2(a.x), pa_exp2(a.y)), q = make_float2(pa_exp2(c.x), pa_exp2(c.y));
-                        sum[0] = __ffma2_rn(p, make_float2(inverse.x, inverse.y), sum[0]);
-                        sum[1] = __ffma2_rn(q, make_float2(inverse.z, inverse.w), sum[1]);
-                        packed[2 * i] = float2_to_half2_bits(p.x, p.y);
-                        packed[2 * i + 1] = float2_to_half2_bits(q.x, q.y);
-                    }
-                } else {
-                    const float2 factor2 = make_float2(factor, factor);
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const float2 a = __ffma2_rn(make_float2(__uint_as_float(raw[i >> 4][2 * (i & 15)]), __uint_as_float(raw[i >> 4][2 * (i & 15) + 1])), factor2, shift2);
-                        const float2 p = make_float2(pa_exp2(a.x), pa_exp2(a.y));
-                        packed[i] = float2_to_bf16x2(p);
-                        sum[i & 1] = __fadd2_rn(sum[i & 1], p);
-                    }
-                    if (cursor.segment > 0) {
-                        mbar_wait(value_full + 8 * (j % STAGES), uint32_t(j / STAGES) & 1u, failed, args.status, STATUS_WAIT_EPILOGUE);
-                        const unsigned long long seen = valid >= PA_KEYS ? ~0ull : valid <= 0 ? 0ull : (1ull << valid) - 1ull;
-                        if ((*static_cast<volatile unsigned long long*>(bad_keys + j % STAGES) & seen) != 0ull) sum[0].x = __uint_as_float(0x7fc00000u);
-                    }
+                for (int i = 0; i < 32; ++i) {
+                    const float2 a = __ffma2_rn(make_float2(__uint_as_float(raw[i >> 4][2 * (i & 15)]), __uint_as_float(raw[i >> 4][2 * (i & 15) + 1])), factor2, shift2);
+                    const float2 p = make_float2(pa_exp2(a.x), pa_exp2(a.y));
+                    packed[i] = FP8 ? float2_to_half2_bits(p.x, p.y) : float2_to_bf16x2(p);
+                    sum[i & 1] = __fadd2_rn(sum[i & 1], p);
                 }
                 running_sum += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+                if (!FP8 && cursor.segment > 0) {
+                    pa_wait(value_full + 8 * (j % STAGES), uint32_t(j / STAGES) & 1u, patience);
+                    bad = *static_cast<volatile unsigned long long*>(bad_keys + j % STAGES);
+                }
+                if (bad != 0ull) {
+                    const unsigned long long seen = valid >= PA_KEYS ? ~0ull : valid <= 0 ? 0ull : (1ull << valid) - 1ull;
+                    if ((bad & seen) != 0ull) running_sum = __uint_as_float(0x7fc00000u);
+                }
             }
             if (FP8) {
                 __syncwarp();
                 if (lane == 0) mbar_arrive(scale_empty + 8 * stage);
             }
-            // the P that lies where this one goes has been read: that of the tile before, or of this group's last
+            // the P that lies where this one goes has been read, and O holds everything before this tile: the product of the tile before, or
+            // of this group's last, is done
             if (j >= Shape::P_BUFFERS) {
-                const int last = j - Shape::P_BUFFERS;
-                mbar_wait(o_done + 8 * (last & 1), uint32_t(last >> 1) & 1u, failed, args.status, STATUS_WAIT_EPILOGUE);
+                if (Shape::SHARED) pa_wait(o_done + 8 * (parity_group ^ 1), parity_group == 0 ? phase ^ 1u : phase, patience);
+                else pa_wait(o_done + 8 * parity_group, phase ^ 1u, patience);
                 tc_fence_after_sync();
-            }
-            pa_tmem_store(lane_address + Shape::TMEM_P + uint32_t(parity_group % Shape::P_BUFFERS) * 32, packed);      // 64 keys in 32 columns
-            if (j > 0 && __any_sync(0xffffffffu, correction != 1.0f)) {
-                // O holds the tiles before this one in units of the reference before: wait for the last of them
-                if (Shape::P_BUFFERS > 1) mbar_wait(o_done + 8 * (parity_group ^ 1), uint32_t((j - 1) >> 1) & 1u, failed, args.status, STATUS_WAIT_EPILOGUE);
-                tc_fence_after_sync();
+                if (__any_sync(0xffffffffu, correction != 1.0f)) {
 #pragma unroll 1
-                for (int chunk = 0; chunk < D / 32; ++chunk) {
-                    uint32_t o[32];
-                    tmem_load_32x32(lane_address + Shape::TMEM_O + chunk * 32, o);
-                    tmem_load_wait();
+                    for (int chunk = 0; chunk < D / 32; ++chunk) {
+                        uint32_t o[32];
+                        tmem_load_32x32(o_tmem + chunk * 32, o);
+                        tmem_load_wait();
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * correction);
-                    pa_tmem_store(lane_address + Shape::TMEM_O + chunk * 32, o);
+                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * correction);
+                        pa_tmem_store(o_tmem + chunk * 32, o);
+                    }
                 }
             }
+            pa_tmem_store(p_tmem, packed);          // 64 keys in 32 columns
             pa_tmem_store_wait();
             tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(p_ready + 8 * parity_group);
         }
-        // ---- the two groups' sums; the later reference is the one O is held in
+        // ---- the two groups' results.  One accumulator is in units of the later reference; two have one each.
         if (num_tiles > 0) {
-            mbar_wait(all_done, 0u, failed, args.status, STATUS_WAIT_EPILOGUE);
+            pa_wait(all_done, 0u, patience);
             tc_fence_after_sync();
         }
-        row_reference[parity_group * PA_ROWS + row] = reference;      // what the last tile of this group left there, or -inf
+        row_reference[parity_group * PA_ROWS + row] = reference;      // what its last tile left there, or -inf
         row_exchange[parity_group * PA_ROWS + row] = running_sum;
+        if (!Shape::SHARED && row == 0) group_unit[parity_group] = unit;
         asm volatile("bar.sync 1, 256;" ::: "memory");
-        {
-            const float other_reference = row_reference[(parity_group ^ 1) * PA_ROWS + row], other_sum = row_exchange[(parity_group ^ 1) * PA_ROWS + row];
-            const float last = fmaxf(reference, other_reference);
-            if (other_reference != last) running_sum += other_sum * pa_exp2(other_reference - last);
-            else if (reference != last) running_sum = running_sum * pa_exp2(reference - last) + other_sum;
-            else running_sum += other_sum;
-            reference = last;
+        const float last = fmaxf(row_reference[row], row_reference[PA_ROWS + row]);
+        float weight[2];          // of the groups' sums, and of their accumulators
+#pragma unroll
+        for (int g = 0; g < 2; ++g) weight[g] = row_reference[g * PA_ROWS + row] == last ? 1.0f : pa_exp2(row_reference[g * PA_ROWS + row] - last);
+        running_sum = weight[0] * row_exchange[row] + weight[1] * row_exchange[PA_ROWS + row];
+        reference = last;
+        if (FP8) {
+            if (Shape::SHARED) weight[0] = exp2f(float(num_tiles > 0 ? group_unit[0] : 0));
+            else weight[0] *= exp2f(float(group_unit[0])), weight[1] *= exp2f(float(group_unit[1]));
+        } else if (Shape::SHARED) {
+            weight[0] = 1.0f;
         }
-        // the codes reached the tensor core as values times 2^-8
-        constexpr float UNIT = FP8 ? 256.0f : 1.0f;
+        // 32 columns of the row in units of the reference
+        auto output_columns = [&](int column, uint32_t (&o)[32]) {
+            tmem_load_32x32(lane_address + Shape::TMEM_O + column, o);
+            if (!Shape::SHARED && num_tiles > 1) {
+                uint32_t other[32];
+                tmem_load_32x32(lane_address + Shape::TMEM_O + D + column, other);
+                tmem_load_wait();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * weight[0] + __uint_as_float(other[i]) * weight[1]);
+            } else {
+                tmem_load_wait();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * weight[0]);
+            }
+        };
         const int work_index = kv_head * args.tiles + tile;
         const int first_column = parity_group * (D / 2);          // each group stores half of the columns
         if (args.splits > 1) {
@@ -740,18 +698,14 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
             if (num_tiles > 0) {
                 float* destination = args.partial + partial_row * D + first_column;
 #pragma unroll 1
-                for (int chunk = 0; chunk < D / 128; ++chunk) {
-                    uint32_t o[2][32];
-                    tmem_load_32x32(lane_address + Shape::TMEM_O + first_column + chunk * 64, o[0]);
-                    tmem_load_32x32(lane_address + Shape::TMEM_O + first_column + chunk * 64 + 32, o[1]);
-                    tmem_load_wait();
+                for (int column = 0; column < D / 2; column += 32) {
+                    uint32_t o[32];
+                    output_columns(first_column + column, o);
                     if (exists) {
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            uint32_t eight[8];
-#pragma unroll
-                            for (int v = 0; v < 8; ++v) eight[v] = __float_as_uint(__uint_as_float(o[i >> 2][(i & 3) * 8 + v]) * UNIT);
-                            st_u8(destination + chunk * 64 + i * 8, eight);
+                        for (int i = 0; i < 4; ++i) {
+                            const uint32_t eight[8] = {o[8 * i], o[8 * i + 1], o[8 * i + 2], o[8 * i + 3], o[8 * i + 4], o[8 * i + 5], o[8 * i + 6], o[8 * i + 7]};
+                            st_u8(destination + column + i * 8, eight);
                         }
                     }
                 }
@@ -759,43 +713,132 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
         } else {
             // sum 0: the row sees no key
             const bool empty = running_sum == 0.0f;
-            const float inverse = UNIT / running_sum;
+            const float inverse = 1.0f / running_sum;
 #pragma unroll 1
-            for (int chunk = 0; chunk < D / 128; ++chunk) {
-                uint32_t o[2][32];
-                if (num_tiles > 0) {
-                    tmem_load_32x32(lane_address + Shape::TMEM_O + first_column + chunk * 64, o[0]);
-                    tmem_load_32x32(lane_address + Shape::TMEM_O + first_column + chunk * 64 + 32, o[1]);
-                    tmem_load_wait();
-                }
+            for (int column = 0; column < D / 2; column += 32) {
+                uint32_t o[32], words[16];
+                if (num_tiles > 0) output_columns(first_column + column, o);
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    words[i] = empty ? 0u : float2_to_bf16x2(make_float2(__uint_as_float(o[2 * i]) * inverse, __uint_as_float(o[2 * i + 1]) * inverse));
                 if (exists) {
+                    uint4* destination = reinterpret_cast<uint4*>(args.out + out_offset + first_column + column);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint32_t words[8];
-#pragma unroll
-                        for (int v = 0; v < 8; ++v) {
-                            const float a = __uint_as_float(o[i >> 1][(i & 1) * 16 + 2 * v]) * inverse;
-                            const float c = __uint_as_float(o[i >> 1][(i & 1) * 16 + 2 * v + 1]) * inverse;
-                            words[v] = empty ? 0u : float2_to_bf16x2(make_float2(a, c));
-                        }
-                        __nv_bfloat16* destination = args.out + out_offset + first_column + chunk * 64 + i * 16;
-                        *reinterpret_cast<uint4*>(destination) = make_uint4(words[0], words[1], words[2], words[3]);
-                        *reinterpret_cast<uint4*>(destination + 8) = make_uint4(words[4], words[5], words[6], words[7]);
-                    }
+                    for (int i = 0; i < 4; ++i) destination[i] = make_uint4(words[4 * i], words[4 * i + 1], words[4 * i + 2], words[4 * i + 3]);
                 }
             }
         }
-    } else if (!FP8) {
+    } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PA_OTHER_REGISTERS));
+    if (warp == PA_LOAD_WARP) {
+        // ------------------------------------------------------------- TMA producer
+        if (num_tiles > 0) {
+            PaCursor cursor(segment_first, segment_length, start_tile);
+            for (int j = 0; j < num_tiles; ++j) {
+                cursor.seek(start_tile + j);
+                const int b = j % STAGES;
+                const uint32_t parity = uint32_t(j / STAGES) & 1u;
+                const bool prefix = cursor.segment == 0;
+                const CUtensorMap* k_map = prefix ? &prefix_k_map : &own_k_map;
+                const CUtensorMap* v_map = prefix ? &prefix_v_map : &own_v_map;
+                const int sequence = prefix ? w.group : w.first_member + w.first_segment_member + cursor.segment - 1;
+                const int row = (sequence * args.kv_heads + kv_head) * (prefix ? args.prefix_capacity : args.own_capacity) + cursor.first_key(start_tile + j);
+                pa_wait(k_empty + 8 * b, parity ^ 1u, patience);
+                __syncwarp();
+                if (elect_one()) {
+                    mbar_expect_tx(k_full + 8 * b, Shape::KV_BYTES);
+                    for (int a = 0; a < Shape::KV_ATOMS; ++a)
+                        tma_load_2d(k_smem + b * Shape::KV_BYTES + a * Shape::KV_ATOM_BYTES, k_map, k_full + 8 * b, a * 128, row);
+                }
+                __syncwarp();
+                pa_wait(v_empty + 8 * b, parity ^ 1u, patience);
+                __syncwarp();
+                if (elect_one()) {
+                    mbar_expect_tx(v_full + 8 * b, Shape::KV_BYTES);
+                    for (int a = 0; a < Shape::KV_ATOMS; ++a)
+                        tma_load_2d(v_smem + b * Shape::KV_BYTES + a * Shape::KV_ATOM_BYTES, v_map, v_full + 8 * b, a * 128, row);
+                }
+                __syncwarp();
+            }
+            // every copy has landed before this CTA may leave (on the normal path the readers have long seen them)
+            for (int b = 0; b < STAGES && b < num_tiles; ++b) {
+                const int last = ((num_tiles - 1 - b) / STAGES) * STAGES + b;
+                pa_wait(k_full + 8 * b, uint32_t(last / STAGES) & 1u, patience);
+                pa_wait(v_full + 8 * b, uint32_t(last / STAGES) & 1u, patience);
+            }
+        }
+    } else if (warp == PA_SCORES_WARP) {
+        // ------------------------------------------------------------- MMA issuer: S[j & 1] = Q K_j^T
+        // Products into different accumulators are ordered by nothing but the barriers, so each kind has a warp that issues it: neither
+        // waits behind the other's operands, and the tensor core finds the next product queued.
+        const uint32_t idesc = FP8 ? idesc_f8(PA_ROWS, PA_KEYS) : pa_idesc_16bit(PA_ROWS, PA_KEYS, true, false);
+        const uint64_t k_major = smem_desc_sw128(0);
+        const uint32_t k_low = uint32_t(k_major), k_high = uint32_t(k_major >> 32);
+        auto field = [](uint32_t address) { return (address & 0x3FFFFu) >> 4; };
+        if (num_tiles > 0) pa_wait(q_ready, 0u, patience);
+        PaRing<STAGES> ring;
+        for (int j = 0; j < num_tiles; ++j) {
+            const int d = j & 1;
+            pa_wait(s_free + 8 * d, (uint32_t(j >> 1) & 1u) ^ 1u, patience);
+            pa_wait(k_full + 8 * ring.slot, ring.parity, patience);
+            tc_fence_after_sync();
+            __syncwarp();
+            if (elect_one()) {
+                const uint32_t d_tmem = tmem_base + Shape::TMEM_S + uint32_t(d) * PA_KEYS;
+                const uint32_t k_base = k_low + field(k_smem + ring.slot * Shape::KV_BYTES);
+                // 32 bytes along K per instruction: 8 columns of Q.  Quantised: first all of hi, then all of lo.
+#pragma unroll
+                for (int a = 0; a < Shape::Q_ATOMS; ++a)
+#pragma unroll
+                    for (int s = 0; s < 4; ++s) {
+                        const uint64_t k_desc = desc_from_words(k_base + (a % Shape::KV_ATOMS) * (Shape::KV_ATOM_BYTES >> 4) + 2 * s, k_high);
+                        if (a < Shape::Q_TMEM_ATOMS) pa_mma<FP8>(d_tmem, tmem_base + Shape::TMEM_Q + uint32_t((a * 4 + s) * 8), k_desc, idesc, (a | s) != 0);
+                        else pa_mma_shared<FP8>(d_tmem, desc_from_words(k_low + field(q_smem) + 2 * s, k_high), k_desc, idesc, 1u);
+                    }
+                tc_commit(s_full + 8 * d);
+                tc_commit(k_empty + 8 * ring.slot);
+            }
+            __syncwarp();
+            ring.next();
+        }
+    } else if (warp == PA_OUTPUT_WARP) {
+        // ------------------------------------------------------------- MMA issuer: O += P V_j
+        const uint32_t idesc = pa_idesc_16bit(PA_ROWS, D, !FP8, true);
+        const uint64_t mn_major = pa_desc_mn(Shape::KV_ATOM_BYTES);
+        const uint32_t mn_low = uint32_t(mn_major), mn_high = uint32_t(mn_major >> 32);
+        auto field = [](uint32_t address) { return (address & 0x3FFFFu) >> 4; };
+        PaRing<FP8 ? 2 : STAGES> ring;
+        for (int j = 0; j < num_tiles; ++j) {
+            const int d = j & 1;
+            pa_wait(value_full + 8 * ring.slot, ring.parity, patience);
+            pa_wait(p_ready + 8 * d, uint32_t(j >> 1) & 1u, patience);
+            tc_fence_after_sync();
+            __syncwarp();
+            if (elect_one()) {
+                const uint32_t p_tmem = tmem_base + Shape::TMEM_P + uint32_t(d % Shape::P_BUFFERS) * 32;
+                const uint32_t v_base = mn_low + field(FP8 ? values_smem + ring.slot * Shape::VALUE_BYTES : v_smem + ring.slot * Shape::KV_BYTES);
+#pragma unroll
+                for (int s = 0; s < PA_KEYS / 16; ++s)          // 16 keys per instruction: 8 columns of P, 16 rows (2048 bytes) of V
+                    pa_mma<false>(tmem_base + Shape::TMEM_O + uint32_t(d % Shape::O_BUFFERS) * D, p_tmem + 8 * s, desc_from_words(v_base + s * (2048 >> 4), mn_high), idesc,
+                                  j >= Shape::O_BUFFERS || s > 0);
+                tc_commit(o_done + 8 * d);
+                tc_commit((FP8 ? value_empty : v_empty) + 8 * ring.slot);
+                if (j == num_tiles - 1) tc_commit(all_done);
+            }
+            __syncwarp();
+            ring.next();
+        }
+    } else if (warp >= PA_VALUE_WARP && !FP8) {
         // ------------------------------------------------------------- bf16: values the tensor core must not see
         if (num_tiles > 0) {
             constexpr int CHUNKS = Shape::KV_ATOMS * 8;          // 16-byte chunks of a row
             const int thread = (warp - PA_VALUE_WARP) * 32 + lane;
-            PaCursor cursor(segment_first, w.segments, start_tile);
+            PaCursor cursor(segment_first, segment_length, start_tile);
             for (int j = 0; j < num_tiles; ++j) {
                 cursor.seek(start_tile + j);
                 const int b = j % STAGES;
-                mbar_wait(v_full + 8 * b, uint32_t(j / STAGES) & 1u, failed, args.status, STATUS_WAIT_PRODUCER);
-                int valid = segment_length[cursor.segment] - cursor.offset * PA_KEYS;
+                pa_wait(v_full + 8 * b, uint32_t(j / STAGES) & 1u, patience);
+                int valid = cursor.keys_left - cursor.first_key(start_tile + j);
                 valid = valid < PA_KEYS ? valid : PA_KEYS;
                 const uint32_t stage = v_smem + b * Shape::KV_BYTES;
                 for (int i = valid * CHUNKS + thread; i < PA_KEYS * CHUNKS; i += 32 * Shape::VALUE_WARPS)
@@ -819,77 +862,137 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
                 if (lane == 0) mbar_arrive(value_full + 8 * b);
             }
         }
-    } else if (warp < PA_VALUE_WARP + Shape::VALUE_WARPS) {
+    } else if (warp >= PA_VALUE_WARP) {
         // ------------------------------------------------------------- codes of the value tile -> f16 operand
         // 16 codes of a key per thread and step: chunk `piece` of its row (stored at piece ^ (key % 8) inside its 128-byte group)
-        // becomes two 16-byte chunks of the 64-column group they belong to.
+        // becomes two 16-byte chunks of the 64-column group they belong to.  Odd groups store their two chunks in the other order: the
+        // eight lanes of a store then meet all banks.
         constexpr int PIECES = D / 16;
         const int thread = (warp - PA_VALUE_WARP) * 32 + lane;
+        PaRing<STAGES> ring;
+        PaCursor cursor(segment_first, segment_length, num_tiles > 0 ? start_tile : -1);
         for (int j = 0; j < num_tiles; ++j) {
-            const int b = j % STAGES, c = j & 1;
-            mbar_wait(v_full + 8 * b, uint32_t(j / STAGES) & 1u, failed, args.status, STATUS_WAIT_PRODUCER);
-            mbar_wait(value_empty + 8 * c, (uint32_t(j >> 1) & 1u) ^ 1u, failed, args.status, STATUS_WAIT_PRODUCER);
+            const int c = j & 1, stage = j % PA_SCALE_STAGES;
+            const uint32_t* value_scales = reinterpret_cast<const uint32_t*>(generic + Shape::OFF_SCALES) + stage * PA_SCALE_FLOATS + PA_KEYS;
+            cursor.seek(start_tile + j);
+            // prefix keys are seen by every row: what is not finite among them may reach all
+            const bool clean = cursor.segment > 0 || cursor.keys(start_tile + j) < PA_KEYS;
+            pa_wait(scale_full + 8 * stage, uint32_t(j / PA_SCALE_STAGES) & 1u, patience);
+            pa_wait(v_full + 8 * ring.slot, ring.parity, patience);
+            pa_wait(value_empty + 8 * c, (uint32_t(j >> 1) & 1u) ^ 1u, patience);
+            auto convert = [&](auto tag) {
+                constexpr bool CLEAN = decltype(tag)::value;
 #pragma unroll 4
-            for (int i = thread; i < PA_KEYS * PIECES; i += 32 * Shape::VALUE_WARPS) {
-                const uint32_t key = uint32_t(i) / PIECES, piece = uint32_t(i) % PIECES, swizzle = key & 7u;
-                const uint4 codes = lds_u4(v_smem + b * Shape::KV_BYTES + (piece >> 3) * Shape::KV_ATOM_BYTES + key * 128u + (((piece & 7u) ^ swizzle) << 4));
-                const uint32_t group = values_smem + c * Shape::VALUE_BYTES + (piece >> 2) * Shape::KV_ATOM_BYTES + key * 128u;
-                const uint32_t first = (piece & 3u) * 2u;
-                const uint32_t a0 = codes_to_halves(codes.x, 0x1404), a1 = codes_to_halves(codes.x, 0x3424);
-                const uint32_t a2 = codes_to_halves(codes.y, 0x1404), a3 = codes_to_halves(codes.y, 0x3424);
-                const uint32_t b0 = codes_to_halves(codes.z, 0x1404), b1 = codes_to_halves(codes.z, 0x3424);
-                const uint32_t b2 = codes_to_halves(codes.w, 0x1404), b3 = codes_to_halves(codes.w, 0x3424);
-                sts_u4(group + ((first ^ swizzle) << 4), a0, a1, a2, a3);
-                sts_u4(group + (((first + 1u) ^ swizzle) << 4), b0, b1, b2, b3);
-            }
+                for (int i = thread; i < PA_KEYS * PIECES; i += 32 * Shape::VALUE_WARPS) {
+                    const uint32_t key = uint32_t(i) / PIECES, piece = uint32_t(i) % PIECES, swizzle = key & 7u;
+                    const uint4 codes = lds_u4(v_smem + ring.slot * Shape::KV_BYTES + (piece >> 3) * Shape::KV_ATOM_BYTES + key * 128u + (((piece & 7u) ^ swizzle) << 4));
+                    const uint32_t scale_bits = value_scales[key];
+                    const __half2 scale = *reinterpret_cast<const __half2*>(&scale_bits);
+                    const uint32_t group = values_smem + c * Shape::VALUE_BYTES + (piece >> 2) * Shape::KV_ATOM_BYTES + key * 128u;
+                    const uint32_t odd = (piece >> 2) & 1u, left = (piece & 3u) * 2u;
+                    const uint32_t x = odd ? codes.z : codes.x, y = odd ? codes.w : codes.y, z = odd ? codes.x : codes.z, w = odd ? codes.y : codes.w;
+                    sts_u4(group + (((left + odd) ^ swizzle) << 4), codes_to_halves<CLEAN>(x, scale), codes_to_halves<CLEAN>(x >> 16, scale),
+                           codes_to_halves<CLEAN>(y, scale), codes_to_halves<CLEAN>(y >> 16, scale));
+                    sts_u4(group + (((left + 1u - odd) ^ swizzle) << 4), codes_to_halves<CLEAN>(z, scale), codes_to_halves<CLEAN>(z >> 16, scale),
+                           codes_to_halves<CLEAN>(w, scale), codes_to_halves<CLEAN>(w >> 16, scale));
+                }
+            };
+            if (clean) convert(std::true_type{});
+            else convert(std::false_type{});
             fence_async_shared();
             __syncwarp();
             if (lane == 0) {
-                mbar_arrive(v_empty + 8 * b);
+                mbar_arrive(v_empty + 8 * ring.slot);
                 mbar_arrive(value_full + 8 * c);
+                mbar_arrive(scale_empty + 8 * stage);
             }
+            ring.next();
         }
-    } else if (num_tiles > 0) {
-        // ------------------------------------------------------------- scales of the key tile, loaded a tile ahead
-        PaCursor cursor(segment_first, w.segments, start_tile);
-        float ks[2], vs[2];
-        auto load = [&](int j) {
-            cursor.seek(start_tile + j);
-            const bool prefix = cursor.segment == 0;
-            const int sequence = prefix ? w.group : w.first_member + w.first_segment_member + cursor.segment - 1;
-            const int64_t first = (int64_t(sequence) * args.kv_heads + kv_head) * (prefix ? args.prefix_capacity : args.own_capacity) + cursor.offset * PA_KEYS;
-            const int valid = segment_length[cursor.segment] - cursor.offset * PA_KEYS;
-            const float* key_scales = (prefix ? args.prefix_scales[0] : args.own_scales[0]) + first;
-            const float* value_scales = (prefix ? args.prefix_scales[1] : args.own_scales[1]) + first;
+    } else if (FP8 && warp == PA_SCALE_WARP) {
+        // ------------------------------------------------------------- scales of the key tiles
+        // Copied PA_RAW_STAGES - 1 tiles ahead, by the lane that converts them: a key tile's time is less than a load from memory takes.
+        if (num_tiles > 0) {
+            PaCursor cursor(segment_first, segment_length, start_tile);
+            const uint32_t raw_scales = base + Shape::OFF_RAW_SCALES;
+            int unit_exponent = 0;
+            auto copy = [&](int j) {
+                if (j < num_tiles) {
+                    cursor.seek(start_tile + j);
+                    const bool prefix = cursor.segment == 0;
+                    const int sequence = prefix ? w.group : w.first_member + w.first_segment_member + cursor.segment - 1;
+                    const int64_t first = (int64_t(sequence) * args.kv_heads + kv_head) * (prefix ? args.prefix_capacity : args.own_capacity) + cursor.first_key(start_tile + j);
+                    const int valid = cursor.keys(start_tile + j);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const bool inside = lane + 32 * i < valid;
-                ks[i] = inside ? __ldg(key_scales + lane + 32 * i) : 0.0f;
-                vs[i] = inside ? __ldg(value_scales + lane + 32 * i) : 0.0f;
-            }
-        };
-        load(0);
-        for (int j = 0; j < num_tiles; ++j) {
-            const int stage = j % PA_SCALE_STAGES;
-            const float key_scale[2] = {ks[0], ks[1]}, value_scale[2] = {vs[0], vs[1]};
-            if (j + 1 < num_tiles) load(j + 1);
-            mbar_wait(scale_empty + 8 * stage, (uint32_t(j / PA_SCALE_STAGES) & 1u) ^ 1u, failed, args.status, STATUS_WAIT_PRODUCER);
-            float* out = reinterpret_cast<float*>(generic + Shape::OFF_SCALES) + stage * PA_SCALE_FLOATS;
+                    for (int i = 0; i < PA_KEYS; i += 32) {
+                        // keys behind the end are not read: 0 takes their place
+                        const int bytes = lane + i < valid ? 4 : 0;
+                        const int64_t at = first + (lane + i < valid ? lane + i : 0);
+                        const uint32_t slot = raw_scales + uint32_t(((j % PA_RAW_STAGES) * 2 * PA_KEYS + lane + i) * 4);
+                        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(slot), "l"((prefix ? args.prefix_scales[0] : args.own_scales[0]) + at), "r"(bytes) : "memory");
+                        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(slot + PA_KEYS * 4), "l"((prefix ? args.prefix_scales[1] : args.own_scales[1]) + at), "r"(bytes) : "memory");
+                    }
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            };
+#pragma unroll 1
+            for (int j = 0; j < PA_RAW_STAGES - 1; ++j) copy(j);
+#pragma unroll 1
+            for (int j = 0; j < num_tiles; ++j) {
+                copy(j + PA_RAW_STAGES - 1);
+                asm volatile("cp.async.wait_group %0;" ::"n"(PA_RAW_STAGES - 1) : "memory");
+                const int stage = j % PA_SCALE_STAGES;
+                pa_wait(scale_empty + 8 * stage, (uint32_t(j / PA_SCALE_STAGES) & 1u) ^ 1u, patience);
+                const volatile float* raw = reinterpret_cast<const volatile float*>(generic + Shape::OFF_RAW_SCALES) + (j % PA_RAW_STAGES) * 2 * PA_KEYS + lane;
+                uint32_t* out = reinterpret_cast<uint32_t*>(generic + Shape::OFF_SCALES) + stage * PA_SCALE_FLOATS;
+                float vs[2];
+                uint32_t not_finite[2], largest = 0u;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const float value = value_scale[i] == 0.0f ? PA_ZERO_ROW_SCALE : value_scale[i];
-                out[lane + 32 * i] = key_scale[i];
-                out[PA_KEYS + lane + 32 * i] = log2f(value);
-                out[2 * PA_KEYS + lane + 32 * i] = value == value ? 1.0f / value : 0.0f;      // NaN reaches the rows that see it by its logarithm
+                for (int i = 0; i < 2; ++i) {
+                    vs[i] = raw[PA_KEYS + 32 * i];
+                    const uint32_t bits = __float_as_uint(vs[i]) & 0x7fffffffu;
+                    not_finite[i] = __ballot_sync(0xffffffffu, bits >= 0x7f800000u);
+                    if (bits >= 0x7f800000u) vs[i] = 0.0f;
+                    else largest = max(largest, bits);
+                }
+                largest = __reduce_max_sync(0xffffffffu, largest);
+                // the unit 2^E: kept unless the tile's largest scale is outside [2^-10, 2^6) of it (a tile of zeros fits any)
+                const int exponent = int(largest >> 23) - 127, relative = exponent - unit_exponent;
+                int change = 0;
+                if (largest != 0u && (j == 0 || relative > 5 || relative < -10)) {
+                    int next = exponent < -60 ? -60 : (exponent > 60 ? 60 : exponent);
+                    if (j > 0) {
+                        next = next < unit_exponent - 60 ? unit_exponent - 60 : next;          // the accumulator grows by the step
+                        change = unit_exponent - next;
+                    }
+                    unit_exponent = next;
+                }
+                const float up = __uint_as_float(uint32_t(127 - unit_exponent) << 23);          // 2^-E
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    out[lane + 32 * i] = __float_as_uint(raw[32 * i]);
+                    const __half2 pair = __float2half2_rn(vs[i] * up);
+                    out[PA_KEYS + lane + 32 * i] = *reinterpret_cast<const uint32_t*>(&pair);
+                }
+                if (lane == 0) {
+                    out[2 * PA_KEYS] = not_finite[0];
+                    out[2 * PA_KEYS + 1] = not_finite[1];
+                    out[2 * PA_KEYS + 2] = uint32_t(unit_exponent);
+                    out[2 * PA_KEYS + 3] = uint32_t(change);
+                    if (Shape::SHARED) group_unit[0] = unit_exponent;
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(scale_full + 8 * stage);
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(scale_full + 8 * stage);
+            asm volatile("cp.async.wait_all;" ::: "memory");
         }
     }
+    }
 
+    if (patience == 0 && args.status != nullptr)
+        atomicCAS(args.status, 0u, warp < 8 ? STATUS_WAIT_EPILOGUE : warp == PA_SCORES_WARP || warp == PA_OUTPUT_WARP ? STATUS_WAIT_MMA_FULL : STATUS_WAIT_PRODUCER);
     tc_fence_before_sync();
     __syncthreads();
-    if (warp == 1) {
+    if (warp == PA_SCORES_WARP) {
         tc_fence_after_sync();
         tmem_dealloc(tmem_base, TMEM_COLUMNS);
     }
