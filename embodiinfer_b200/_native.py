@@ -134,11 +134,11 @@ SIGNATURES: dict[str, list] = {
     "b2_attention": [_P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P],
     "b2_attention_fp8": [_P, _P, _P, _P, _F, _I, _I, _I, _I, _I, _P, _P],
     "b2_attention_nvfp4": [_P, _P, _P, _P, _P, _P, _F, _I, _I, _I, _I, _I, _P, _P],
-    "b2_rope_axes": [_P, _I, ctypes.POINTER(ctypes.c_int32), _I, _I64, _I, _D, _I, _P, _P, _P],
-    "b2_kv_cache_write": [ctypes.POINTER(KVCacheDesc), _P],
-    "b2_kv_cache_read": [ctypes.POINTER(KVCacheDesc), _P],
-    "b2_prefix_attention": [ctypes.POINTER(PrefixAttentionDesc), _P],
-    "b2_prefix_attention_workspace_bytes": [ctypes.POINTER(PrefixAttentionDesc)],
+    "b2_rope_axes": [_P, _I, _P, _I, _I64, _I, _D, _I, _P, _P, _P],
+    "b2_kv_cache_write": [_P, _P],
+    "b2_kv_cache_read": [_P, _P],
+    "b2_prefix_attention": [_P, _P],
+    "b2_prefix_attention_workspace_bytes": [_P],
 }
 RESULT_TYPES = {"b2_linear_workspace_bytes": ctypes.c_int64, "b2_prefix_attention_workspace_bytes": ctypes.c_int64}
 

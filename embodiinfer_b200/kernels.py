@@ -9,6 +9,7 @@ These are the calls the plan objects (``embodiinfer_b200.backend``) and the regi
 from __future__ import annotations
 
 import ctypes
+import struct
 from contextlib import nullcontext
 
 import torch
@@ -18,7 +19,8 @@ from .kv_cache import QuantizedKVCache
 
 
 def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    # the handle alone: building the Stream object around it takes some 2 us
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device.index is None else device.index)
 
 
 def _ptr(tensor: torch.Tensor | None) -> int | None:
@@ -26,19 +28,20 @@ def _ptr(tensor: torch.Tensor | None) -> int | None:
 
 
 def _require_cuda(*tensors: torch.Tensor | None) -> torch.device:
-    device = None
+    first, index = None, -1
     for tensor in tensors:
         if tensor is None:
             continue
-        if not tensor.is_cuda:
+        own = tensor.get_device()          # -1: not on a GPU
+        if own < 0 or not tensor.is_cuda:
             raise ValueError("embodiinfer_b200 kernels require CUDA tensors; there is no CPU fallback")
-        if device is None:
-            device = tensor.device
-        elif tensor.device != device:
+        if first is None:
+            first, index = tensor, own
+        elif own != index:
             raise ValueError("all operands must live on one CUDA device")
-    if device is None:
+    if first is None:
         raise ValueError("no tensor operands")
-    return device
+    return first.device
 
 
 def _on(device: torch.device):
@@ -273,58 +276,69 @@ def rope_axes(positions: torch.Tensor, sections: tuple[int, ...], sine: torch.Te
     device = _require_cuda(positions, sine, cosine)
     if positions.dtype not in (torch.int32, torch.int64) or positions.ndim < 2 or not positions.is_contiguous():
         raise ValueError("rope_axes requires contiguous int32 or int64 positions [axes, ..., tokens]")
-    axes, half = positions.shape[0], sum(sections)
+    shape = positions.shape
+    axes, half = shape[0], sum(sections)
     if len(sections) != axes or any(type(section) is not int or section <= 0 for section in sections):
         raise ValueError("rope_axes requires one positive section for each axis")
-    shape = (*positions.shape[1:], half)
+    shape = (*shape[1:], half)
     if sine is None and cosine is None:
-        sine, cosine = (torch.empty(shape, device=device, dtype=torch.float32) for _ in range(2))
-    for table in (sine, cosine):
-        if table is None or table.dtype != torch.float32 or table.shape != shape or not table.is_contiguous():
-            raise ValueError("rope_axes requires contiguous fp32 tables [..., tokens, head_dim/2], both or neither")
+        sine = torch.empty(shape, device=device, dtype=torch.float32)
+        cosine = torch.empty_like(sine)
+    else:
+        for table in (sine, cosine):
+            if table is None or table.dtype != torch.float32 or table.shape != shape or not table.is_contiguous():
+                raise ValueError("rope_axes requires contiguous fp32 tables [..., tokens, head_dim/2], both or neither")
     tokens = positions.numel() // axes if axes else 0
     if tokens == 0:
         return sine, cosine
     with _on(device):
-        status = N.load().b2_rope_axes(positions.data_ptr(), positions.element_size(), (ctypes.c_int32 * axes)(*sections), axes, tokens,
+        status = N.load().b2_rope_axes(positions.data_ptr(), positions.element_size(), struct.pack(f"{axes}i", *sections), axes, tokens,
                                        2 * half, float(theta), N.ROPE_OWN_SPECTRUM if own_spectrum else 0, sine.data_ptr(),
                                        cosine.data_ptr(), _stream(device))
     N.check(status, "b2_rope_axes")
     return sine, cosine
 
 
+# The descriptors of the calls that a decoding step makes for every token, packed: filling the ctypes structures takes longer than
+# launching the kernel.
+_CACHE_DESC = struct.Struct("12P10q6i0q")
+_ATTENTION_DESC = struct.Struct("15P4qf10i0q")
+assert _CACHE_DESC.size == ctypes.sizeof(N.KVCacheDesc) and _ATTENTION_DESC.size == ctypes.sizeof(N.PrefixAttentionDesc)
+
+
+def _address(tensor: torch.Tensor | None) -> int:
+    return 0 if tensor is None else tensor.data_ptr()
+
+
 def _check_cache(cache: QuantizedKVCache, what: str) -> tuple[int, int, int, int]:
     """The (batch, kv_heads, capacity, head_dim) of a quantised cache."""
-    shape = cache.k_codes.shape
-    if len(shape) != 4 or cache.v_codes.shape != shape or cache.k_scales.shape != shape[:3] or cache.v_scales.shape != shape[:3]:
+    k_codes, k_scales, v_codes, v_scales = cache
+    shape = k_codes.shape
+    if len(shape) != 4 or v_codes.shape != shape or k_scales.shape != shape[:3] or v_scales.shape != shape[:3]:
         raise ValueError(f"{what} requires codes [batch, kv_heads, capacity, head_dim] and scales [batch, kv_heads, capacity]")
-    for codes, scales in ((cache.k_codes, cache.k_scales), (cache.v_codes, cache.v_scales)):
-        if codes.element_size() != 1 or scales.dtype != torch.float32 or not codes.is_contiguous() or not scales.is_contiguous():
-            raise ValueError(f"{what} requires contiguous one-byte codes and contiguous fp32 scales")
-    return tuple(shape)
+    if not (k_codes.element_size() == 1 == v_codes.element_size() and k_scales.dtype is torch.float32 is v_scales.dtype and k_codes.is_contiguous()
+            and v_codes.is_contiguous() and k_scales.is_contiguous() and v_scales.is_contiguous()):
+        raise ValueError(f"{what} requires contiguous one-byte codes and contiguous fp32 scales")
+    return shape
 
 
 def _check_whole(values: torch.Tensor | None, count: int, what: str) -> None:
-    if values is not None and (values.dtype != torch.int32 or values.shape != (count,) or not values.is_contiguous()):
+    if values is not None and (values.dtype is not torch.int32 or values.shape != (count,) or not values.is_contiguous()):
         raise ValueError(f"{what} must be a contiguous int32 tensor of {count} values")
 
 
-def _kv_cache_desc(rows: tuple[torch.Tensor, torch.Tensor], cache: QuantizedKVCache, offsets, lengths, what: str) -> "N.KVCacheDesc":
-    """The descriptor of a write or a read, without queries and tables; checks everything the two have in common."""
+def _check_cache_rows(k: torch.Tensor, v: torch.Tensor, cache: QuantizedKVCache, offsets, lengths, what: str) -> tuple:
+    """Everything that a write and a read have in common: (batch, kv_heads, capacity, head_dim, tokens, the strides of k and v)."""
     batch, kv_heads, capacity, head_dim = _check_cache(cache, what)
-    k, v = rows
-    if k.shape != v.shape or k.ndim != 4 or k.shape[0] != batch or k.shape[1] != kv_heads or k.shape[3] != head_dim:
+    shape = k.shape
+    if v.shape != shape or len(shape) != 4 or shape[0] != batch or shape[1] != kv_heads or shape[3] != head_dim:
         raise ValueError(f"{what} requires keys and values [batch, kv_heads, tokens, head_dim] that fit the cache")
-    for row in rows:
-        if row.dtype != torch.bfloat16 or row.stride(3) != 1:
-            raise ValueError(f"{what} requires bf16 keys and values whose last dimension is contiguous")
+    k_stride, v_stride = k.stride(), v.stride()
+    if not (k.dtype is torch.bfloat16 is v.dtype and k_stride[3] == 1 == v_stride[3]):
+        raise ValueError(f"{what} requires bf16 keys and values whose last dimension is contiguous")
     _check_whole(offsets, batch, "offsets")
     _check_whole(lengths, batch, "lengths")
-    return N.KVCacheDesc(
-        k=k.data_ptr(), v=v.data_ptr(), k_codes=cache.k_codes.data_ptr(), k_scales=cache.k_scales.data_ptr(),
-        v_codes=cache.v_codes.data_ptr(), v_scales=cache.v_scales.data_ptr(), offsets=_ptr(offsets), lengths=_ptr(lengths),
-        k_stride=k.stride()[:3], v_stride=v.stride()[:3], batch=batch, tokens=k.shape[2], kv_heads=kv_heads, head_dim=head_dim,
-        capacity=capacity)
+    return batch, kv_heads, capacity, head_dim, shape[2], (*k_stride[:3], *v_stride[:3])
 
 
 def kv_cache_write(k: torch.Tensor, v: torch.Tensor, cache: QuantizedKVCache, *, q: torch.Tensor | None = None,
@@ -335,27 +349,31 @@ def kv_cache_write(k: torch.Tensor, v: torch.Tensor, cache: QuantizedKVCache, *,
     rotated ``q`` [B, H, T, D] goes to ``q_out`` (contiguous).  k, v and q may be views of one packed projection.  See
     ``b2_kv_cache_write``; padded tokens and positions outside the cache are passed over."""
     device = _require_cuda(k, v, *cache, q, q_out, sine, cosine, offsets, lengths)
-    desc = _kv_cache_desc((k, v), cache, offsets, lengths, "kv_cache_write")
-    tokens, head_dim = k.shape[2], k.shape[3]
+    batch, kv_heads, capacity, head_dim, tokens, strides = _check_cache_rows(k, v, cache, offsets, lengths, "kv_cache_write")
     if (q is None) != (q_out is None) or (sine is None) != (cosine is None):
         raise ValueError("kv_cache_write takes q with q_out, and sine with cosine")
+    heads, q_stride, factor_stride = 0, (0, 0, 0), 0
     if q is not None:
-        if q.dtype != torch.bfloat16 or q.ndim != 4 or q.shape[0] != k.shape[0] or q.shape[2:] != k.shape[2:] or q.stride(3) != 1:
+        shape, q_stride = q.shape, q.stride()
+        if q.dtype is not torch.bfloat16 or len(shape) != 4 or shape[0] != batch or shape[2] != tokens or shape[3] != head_dim or q_stride[3] != 1:
             raise ValueError("q must be bf16 [batch, heads, tokens, head_dim] with a contiguous last dimension")
-        if q_out.dtype != torch.bfloat16 or q_out.shape != q.shape or not q_out.is_contiguous():
+        if q_out.dtype is not torch.bfloat16 or q_out.shape != shape or not q_out.is_contiguous():
             raise ValueError("q_out must be a contiguous bf16 tensor of q's shape")
-        desc.q, desc.q_out, desc.heads, desc.q_stride = q.data_ptr(), q_out.data_ptr(), q.shape[1], q.stride()[:3]
+        heads, q_stride = shape[1], q_stride[:3]
     if sine is not None:
-        for factor in (sine, cosine):
-            if factor.dtype != torch.float32 or not factor.is_contiguous() or factor.shape != sine.shape or \
-                    tuple(factor.shape) not in ((tokens, head_dim // 2), (k.shape[0], tokens, head_dim // 2)):
-                raise ValueError("kv_cache_write requires contiguous fp32 factors [tokens, head_dim/2] or [batch, tokens, head_dim/2]")
-        desc.sine, desc.cosine = sine.data_ptr(), cosine.data_ptr()
-        desc.factor_batch_stride = tokens * (head_dim // 2) if sine.ndim == 3 else 0
-    if k.numel() == 0 or desc.capacity == 0:
+        shape, half = sine.shape, head_dim // 2
+        if not (sine.dtype is torch.float32 is cosine.dtype and cosine.shape == shape and sine.is_contiguous() and cosine.is_contiguous()
+                and (shape == (tokens, half) or shape == (batch, tokens, half))):
+            raise ValueError("kv_cache_write requires contiguous fp32 factors [tokens, head_dim/2] or [batch, tokens, head_dim/2]")
+        factor_stride = tokens * half if len(shape) == 3 else 0
+    if not (batch and kv_heads and tokens and head_dim and capacity):
         return
+    k_codes, k_scales, v_codes, v_scales = cache
+    desc = _CACHE_DESC.pack(_address(q), _address(q_out), k.data_ptr(), v.data_ptr(), _address(sine), _address(cosine), k_codes.data_ptr(),
+                            k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(), _address(offsets), _address(lengths), *q_stride,
+                            *strides, factor_stride, batch, tokens, heads, kv_heads, head_dim, capacity)
     with _on(device):
-        status = N.load().b2_kv_cache_write(ctypes.byref(desc), _stream(device))
+        status = N.load().b2_kv_cache_write(desc, _stream(device))
     N.check(status, "b2_kv_cache_write")
 
 
@@ -364,31 +382,34 @@ def kv_cache_read(cache: QuantizedKVCache, k_out: torch.Tensor, v_out: torch.Ten
     """Positions ``offsets[b] + t`` of ``cache`` as bf16 into row ``t`` of ``k_out`` / ``v_out`` [B, kv_heads, T, D], for
     ``t < lengths[b]`` (defaults 0 and T); the other rows are left as they are.  See ``b2_kv_cache_read``."""
     device = _require_cuda(*cache, k_out, v_out, offsets, lengths)
-    desc = _kv_cache_desc((k_out, v_out), cache, offsets, lengths, "kv_cache_read")
-    if k_out.numel() != 0 and desc.capacity != 0:
+    batch, kv_heads, capacity, head_dim, tokens, strides = _check_cache_rows(k_out, v_out, cache, offsets, lengths, "kv_cache_read")
+    if batch and kv_heads and tokens and head_dim and capacity:
+        k_codes, k_scales, v_codes, v_scales = cache
+        desc = _CACHE_DESC.pack(0, 0, k_out.data_ptr(), v_out.data_ptr(), 0, 0, k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
+                                v_scales.data_ptr(), _address(offsets), _address(lengths), 0, 0, 0, *strides, 0, batch, tokens, 0, kv_heads,
+                                head_dim, capacity)
         with _on(device):
-            status = N.load().b2_kv_cache_read(ctypes.byref(desc), _stream(device))
+            status = N.load().b2_kv_cache_read(desc, _stream(device))
         N.check(status, "b2_kv_cache_read")
     return k_out, v_out
 
 
-def _cache_part(part, count: int, q: torch.Tensor, what: str) -> tuple[int, int, int, tuple]:
-    """(bits, kv_heads, capacity, the four pointers) of a prefix or own cache; bits 0 when there is none."""
-    if part is None:
-        return 0, 0, 0, (None, None, None, None)
+def _cache_part(part, count: int, width: int, what: str) -> tuple[int, int, int, int, tuple]:
+    """(bits, batch, kv_heads, capacity, the four pointers k, v, k_scales, v_scales) of a prefix or own cache."""
     if isinstance(part, QuantizedKVCache):
         batch, kv_heads, capacity, head_dim = _check_cache(part, "prefix_attention")
-        bits, pointers = 8, (part.k_codes.data_ptr(), part.v_codes.data_ptr(), part.k_scales.data_ptr(), part.v_scales.data_ptr())
+        k, k_scales, v, v_scales = part
+        bits, pointers = 8, (k.data_ptr(), v.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr())
     else:
         k, v = part
-        if k.ndim != 4 or k.shape != v.shape or k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16 or not k.is_contiguous() or \
-                not v.is_contiguous():
+        shape = k.shape
+        if not (len(shape) == 4 and v.shape == shape and k.dtype is torch.bfloat16 is v.dtype and k.is_contiguous() and v.is_contiguous()):
             raise ValueError("prefix_attention requires contiguous bf16 keys and values [n, kv_heads, capacity, head_dim], or quantised caches")
-        batch, kv_heads, capacity, head_dim = k.shape
-        bits, pointers = 16, (k.data_ptr(), v.data_ptr(), None, None)
-    if batch != count and count >= 0 or head_dim != q.shape[3]:
+        batch, kv_heads, capacity, head_dim = shape
+        bits, pointers = 16, (k.data_ptr(), v.data_ptr(), 0, 0)
+    if batch != count and count >= 0 or head_dim != width:
         raise ValueError(f"prefix_attention: the {what} cache does not fit the queries")
-    return bits, kv_heads, capacity, pointers if capacity else (None, None, None, None)
+    return bits, batch, kv_heads, capacity, pointers if capacity else (0, 0, 0, 0)
 
 
 def prefix_attention(q: torch.Tensor, prefix, own=None, *, members: torch.Tensor | None = None, prefix_lengths: torch.Tensor | None = None,
@@ -400,45 +421,47 @@ def prefix_attention(q: torch.Tensor, prefix, own=None, *, members: torch.Tensor
     [members[g], members[g + 1]); default B / G each.  ``prefix_lengths`` int32 [G], ``own_lengths`` int32 [B]: default the
     capacities.  ``causal``: query t sees all but the last T - 1 - t own keys.  ``scale`` defaults to 1 / sqrt(D).  Returns bf16
     [B, H, T, D]; rows that see no key are zero.  See ``b2_prefix_attention``."""
-    parts = tuple(t for part in (prefix, own) if part is not None for t in part)
-    device = _require_cuda(q, *parts, members, prefix_lengths, own_lengths, out, status)
-    if q.ndim != 4 or q.dtype != torch.bfloat16 or q.stride(3) != 1:
-        raise ValueError("prefix_attention requires bf16 queries [batch, heads, tokens, head_dim] with a contiguous last dimension")
-    batch, heads, queries, head_dim = q.shape
     if prefix is None:
         raise ValueError("prefix_attention requires a prefix cache (its capacity may be 0)")
-    bits, kv_heads, prefix_capacity, prefix_pointers = _cache_part(prefix, -1, q, "prefix")
-    own_bits, own_kv_heads, own_capacity, own_pointers = _cache_part(own, batch, q, "own")
-    if own is not None and (own_bits != bits or own_kv_heads != kv_heads):
-        raise ValueError("prefix_attention requires prefix and own caches of one kind with equal kv_heads")
-    groups = prefix[0].shape[0]
+    device = _require_cuda(q, *prefix, *(own or ()), members, prefix_lengths, own_lengths, out, status)
+    shape, q_stride = q.shape, q.stride()
+    if len(shape) != 4 or q.dtype is not torch.bfloat16 or q_stride[3] != 1:
+        raise ValueError("prefix_attention requires bf16 queries [batch, heads, tokens, head_dim] with a contiguous last dimension")
+    batch, heads, queries, head_dim = shape
+    bits, groups, kv_heads, prefix_capacity, prefix_pointers = _cache_part(prefix, -1, head_dim, "prefix")
+    own_capacity, own_pointers = 0, (0, 0, 0, 0)
+    if own is not None:
+        own_bits, _, own_kv_heads, own_capacity, own_pointers = _cache_part(own, batch, head_dim, "own")
+        if own_bits != bits or own_kv_heads != kv_heads:
+            raise ValueError("prefix_attention requires prefix and own caches of one kind with equal kv_heads")
     _check_whole(members, groups + 1, "members")
     _check_whole(prefix_lengths, groups, "prefix_lengths")
     _check_whole(own_lengths, batch, "own_lengths")
     if kv_heads == 0 or heads % kv_heads or groups == 0 or (members is None and batch % groups):
         raise ValueError("prefix_attention requires heads divisible by kv_heads, and a batch divisible by the groups unless members is given")
     if out is None:
-        out = torch.empty((batch, heads, queries, head_dim), device=device, dtype=torch.bfloat16)
-    elif out.shape != q.shape or out.dtype != torch.bfloat16 or not out.is_contiguous():
+        out = torch.empty(shape, device=device, dtype=torch.bfloat16)
+    elif out.shape != shape or out.dtype is not torch.bfloat16 or not out.is_contiguous():
         raise ValueError("attention output must be a contiguous bf16 tensor of the queries' shape")
-    if out.numel() == 0:
+    if not (batch and heads and queries and head_dim):
         return out
     if prefix_capacity == 0 and own_capacity == 0:
         return out.zero_()
     if status is None:
         status = status_word(device)
-    desc = N.PrefixAttentionDesc(
-        q.data_ptr(), out.data_ptr(), *prefix_pointers[:2], *prefix_pointers[2:], *own_pointers[:2], *own_pointers[2:], _ptr(members),
-        _ptr(prefix_lengths), _ptr(own_lengths), status.data_ptr(), None, 0, q.stride()[:3], head_dim ** -0.5 if scale is None else scale,
-        N.ATTENTION_CAUSAL if causal else 0, batch, groups, heads, kv_heads, queries, head_dim, prefix_capacity, own_capacity, bits)
+    pointers = (q.data_ptr(), out.data_ptr(), *prefix_pointers, *own_pointers, _address(members), _address(prefix_lengths),
+                _address(own_lengths), status.data_ptr())
+    sizes = (*q_stride[:3], head_dim ** -0.5 if scale is None else scale, N.ATTENTION_CAUSAL if causal else 0, batch, groups, heads,
+             kv_heads, queries, head_dim, prefix_capacity, own_capacity, bits)
+    desc = _ATTENTION_DESC.pack(*pointers, 0, 0, *sizes)
     library = N.load()
     with _on(device):
         # scratch of this call alone (also inside a captured graph: it is the graph's own)
-        size = library.b2_prefix_attention_workspace_bytes(ctypes.byref(desc))
-        workspace = torch.empty(size, device=device, dtype=torch.uint8) if size else None
+        size = library.b2_prefix_attention_workspace_bytes(desc)
         if size:
-            desc.workspace, desc.workspace_bytes = workspace.data_ptr(), size
-        code = library.b2_prefix_attention(ctypes.byref(desc), _stream(device))
+            workspace = torch.empty(size, device=device, dtype=torch.uint8)
+            desc = _ATTENTION_DESC.pack(*pointers, workspace.data_ptr(), size, *sizes)
+        code = library.b2_prefix_attention(desc, _stream(device))
     N.check(code, "b2_prefix_attention")
     return out
 
