@@ -57,7 +57,7 @@ constexpr int PA_LOAD_WARP = 8, PA_SCORES_WARP = 9, PA_OUTPUT_WARP = 10, PA_SCAL
 // Registers per thread: 128 at launch (512 threads); the softmax warpgroups take what the others give up.
 constexpr int PA_SOFTMAX_REGISTERS = 168, PA_OTHER_REGISTERS = 88;
 static_assert(256 * PA_SOFTMAX_REGISTERS + (PA_WARPS * 32 - 256) * PA_OTHER_REGISTERS <= PA_WARPS * 32 * 128, "registers of the launch");
-constexpr int PA_PATIENCE = 1 << 24;              // tries of a wait: some 30 cycles each at least, half a second in all
+constexpr uint32_t PA_PATIENCE = 1400000000u;     // cycles of a wait
 constexpr int PA_SCALE_STAGES = 4, PA_RAW_STAGES = 8;      // of the quantised cache's scales: as the softmax reads them; as they come
 // A key tile's scales as the roles read them: ks, vs in units as pairs of halves, then bits of keys whose vs is not finite (2 words), the
 // unit, and the unit of the tile before less this one (exponents).
@@ -72,6 +72,7 @@ struct PaShape {
     static constexpr uint32_t KV_ATOM_BYTES = PA_KEYS * 128;
     static constexpr uint32_t KV_BYTES = KV_ATOMS * KV_ATOM_BYTES;
     static constexpr int STAGES = D == 256 ? (FP8 ? 4 : 3) : (FP8 ? 8 : 6); // of the K and the V ring each
+    static constexpr int FREE_V_STAGES = FP8 ? STAGES : STAGES - int(PA_ROWS * D * 2 / KV_BYTES);      // of V: not under the queries as they come in
     static constexpr int VALUE_STAGES = FP8 ? 2 : 0;                        // converted value tiles
     static constexpr uint32_t VALUE_BYTES = PA_KEYS * D * 2;
     static constexpr int VALUE_WARPS = 4;
@@ -90,7 +91,8 @@ struct PaShape {
     static constexpr uint32_t OFF_SCALES = OFF_Q + (Q_ATOMS - Q_TMEM_ATOMS) * PA_ROWS * 128;
     static constexpr uint32_t OFF_RAW_SCALES = OFF_SCALES + (FP8 ? PA_SCALE_STAGES * PA_SCALE_FLOATS * 4 : 0);
     static constexpr uint32_t OFF_ROWS = OFF_RAW_SCALES + (FP8 ? PA_RAW_STAGES * 2 * PA_KEYS * 4 : 0);      // float [2][128], twice
-    static constexpr uint32_t OFF_SEGMENTS = OFF_ROWS + 4 * PA_ROWS * 4;
+    static constexpr uint32_t OFF_ROW_OFFSETS = OFF_ROWS + 4 * PA_ROWS * 4;          // int64 [2][128]
+    static constexpr uint32_t OFF_SEGMENTS = OFF_ROW_OFFSETS + 2 * PA_ROWS * 8;
     static constexpr uint32_t OFF_BARS = OFF_SEGMENTS + (PA_MAX_SEGMENTS + 3) * 8;
     static constexpr int SHARED_BYTES = 1024 + int(OFF_BARS) + 768;
 };
@@ -206,6 +208,12 @@ __device__ __forceinline__ uint4 lds_u4(uint32_t address) {
     return v;
 }
 
+template <int ID, int THREADS>
+__device__ __forceinline__ void named_barrier() {
+    __syncwarp();
+    __barrier_sync_count(ID, THREADS);
+}
+
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 __device__ __forceinline__ uint32_t float2_to_half2_bits(float a, float b) {
@@ -228,12 +236,13 @@ __device__ __forceinline__ bool has_not_finite(uint32_t word) {
     return (word & 0x7f80u) == 0x7f80u || (word & 0x7f800000u) == 0x7f800000u;
 }
 
-// Bounded wait, as small as it can be made: the roles' loops have to share the instruction caches.  `patience` is the number of tries; once
-// they have run out it stays 0, every later wait of the thread gives up at once, and the role reports it when it ends.
-__device__ __forceinline__ void pa_wait(uint32_t bar, uint32_t parity, int& patience) {
-    int tries = patience;
+// Bounded wait, as small as it can be made: the roles' loops have to share the instruction caches.  `patience` is its limit in cycles (0.7
+// seconds or more); once a wait has run out it stays 0, every later wait of the thread gives up at once, and the role reports it when it ends.
+__device__ __forceinline__ void pa_wait(uint32_t bar, uint32_t parity, uint32_t& patience) {
+    if (mbar_try_wait(bar, parity)) return;
+    const uint32_t start = uint32_t(clock());
     while (!mbar_try_wait(bar, parity))
-        if (--tries <= 0) {
+        if (uint32_t(clock()) - start >= patience) {
             patience = 0;
             break;
         }
@@ -289,7 +298,10 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
     const uint32_t base = (smem_u32(shared_raw) + 1023u) & ~1023u;
     uint8_t* const generic = shared_raw + (base - smem_u32(shared_raw));
     const uint32_t k_smem = base + Shape::OFF_K, v_smem = base + Shape::OFF_V, values_smem = base + Shape::OFF_VALUES;
-    const uint32_t q_smem = base + Shape::OFF_Q;
+    // the queries come in where the values, or the last value tiles, will lie
+    const uint32_t q_smem = base + Shape::OFF_Q, staging_smem = FP8 ? values_smem : v_smem + Shape::FREE_V_STAGES * Shape::KV_BYTES;
+    int64_t* const row_output = reinterpret_cast<int64_t*>(generic + Shape::OFF_ROW_OFFSETS);          // [128]: element offset of the row's output, -1: no row
+    int64_t* const row_query = row_output + PA_ROWS;                                                   // [128]: of its query
     float* const row_reference = reinterpret_cast<float*>(generic + Shape::OFF_ROWS);           // [2][128]: of the latest even and odd tile
     float* const row_exchange = row_reference + 2 * PA_ROWS;                                    // [2][128]: row maxima of Q, then the sums
     int* const group_unit = reinterpret_cast<int*>(generic + Shape::OFF_BARS + 720);          // [2]: last units of the accumulators, as exponents
@@ -313,31 +325,19 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
     const int kv_head = (int(blockIdx.x) / args.tiles) % args.kv_heads;
     const int split = int(blockIdx.x) / (args.tiles * args.kv_heads);
 
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < STAGES; ++i) {
-            mbar_init(k_full + 8 * i, 1);
-            mbar_init(k_empty + 8 * i, 1);
-            mbar_init(v_full + 8 * i, 1);
-            mbar_init(v_empty + 8 * i, FP8 ? Shape::VALUE_WARPS : 1);
+    if (warp == 0) {          // one lane per barrier (8 bytes each, in the order above); unused places of the arrays are barriers too
+        for (int i = lane; i < 74; i += 32) {
+            int count = 1;
+            if (i >= 24 && i < 32 && FP8) count = Shape::VALUE_WARPS;                 // v_empty
+            else if (i >= 32 && i < 40) count = Shape::VALUE_WARPS;                   // value_full
+            else if (i >= 50 && i < 54) count = 4;                                    // s_free, p_ready
+            else if (i >= 60 && i < 64) count = 4 + Shape::VALUE_WARPS;               // scale_empty
+            else if (i == 73) count = 8;                                              // q_ready
+            mbar_init(bars + 8 * i, count);
         }
-        for (int i = 0; i < (FP8 ? 2 : STAGES); ++i) {
-            mbar_init(value_full + 8 * i, Shape::VALUE_WARPS);
-            mbar_init(value_empty + 8 * i, 1);
-        }
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(s_full + 8 * i, 1);
-            mbar_init(s_free + 8 * i, 4);
-            mbar_init(p_ready + 8 * i, 4);
-            mbar_init(o_done + 8 * i, 1);
-        }
-        for (int i = 0; i < PA_SCALE_STAGES; ++i) {
-            mbar_init(scale_full + 8 * i, 1);
-            mbar_init(scale_empty + 8 * i, 4 + Shape::VALUE_WARPS);
-        }
-        for (int i = 0; i < 8; ++i) mbar_init(reference_ready + 8 * i, 1);
-        mbar_init(all_done, 1);
-        mbar_init(q_ready, 8);
         fence_barrier_init();
+    }
+    if (threadIdx.x == 32) {
         tma_prefetch_descriptor(&prefix_k_map);
         tma_prefetch_descriptor(&prefix_v_map);
         tma_prefetch_descriptor(&own_k_map);
@@ -429,7 +429,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
     const int start_tile = int(int64_t(w.key_tiles) * split / args.splits);
     const int num_tiles = int(int64_t(w.key_tiles) * (split + 1) / args.splits) - start_tile;
 
-    int patience = PA_PATIENCE;
+    uint32_t patience = PA_PATIENCE;
     if (warp < 8) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PA_SOFTMAX_REGISTERS));
         // ------------------------------------------------------------- one thread per query row and tile parity
@@ -438,8 +438,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
         const uint32_t lane_address = tmem_base + (uint32_t(quarter * 32) << 16);
         const bool exists = row < w.rows;
         int my_segment = -1, hidden = 0;          // the segment of this row's own keys; causal: how many of them lie behind the query
-        int64_t out_offset = -1;
-        const __nv_bfloat16* query_row = args.q;
+        int64_t out_offset = -1, query_offset = -1;
         if (exists) {
             const int member = (w.row0 + row) / args.rows_per_member, inside = w.row0 + row - member * args.rows_per_member;
             const int head_in_group = inside / args.queries, query = inside - head_in_group * args.queries;
@@ -447,39 +446,61 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
             my_segment = member - w.first_segment_member + 1;
             hidden = args.causal ? args.queries - 1 - query : 0;
             out_offset = ((int64_t(w.first_member + member) * args.heads + head) * args.queries + query) * D;
-            query_row += int64_t(w.first_member + member) * args.q_stride[0] + head * args.q_stride[1] + query * args.q_stride[2];
+            query_offset = int64_t(w.first_member + member) * args.q_stride[0] + head * args.q_stride[1] + query * args.q_stride[2];
         }
-        // ---- the queries into tensor memory: each group brings one half of the columns
+        if (parity_group == 0) row_output[row] = out_offset;          // read behind the barrier at the end
+        // ---- the queries into tensor memory: rows come to shared memory as they lie (16 bytes per thread), each thread then takes one half of
+        // the columns of its row
         float factor = args.scale_log2;
         if (num_tiles > 0) {
-            constexpr int WORDS = D / 4;          // 32-bit words of half a bf16 row
-            uint32_t words[WORDS];
-            const uint4* source = reinterpret_cast<const uint4*>(query_row + parity_group * (D / 2));
-#pragma unroll
-            for (int i = 0; i < WORDS / 4; ++i) {
-                const uint4 v = exists ? source[i] : make_uint4(0, 0, 0, 0);
-                words[4 * i] = v.x; words[4 * i + 1] = v.y; words[4 * i + 2] = v.z; words[4 * i + 3] = v.w;
+            constexpr int CHUNKS = D / 128;          // of 32 words (64 values) of half a bf16 row
+            constexpr int PIECES = D / 8;            // 16-byte pieces of a row; piece p lies at p ^ (row % 8)
+            if (parity_group == 1) row_query[row] = query_offset;
+            named_barrier<1, 256>();
+#pragma unroll 4
+            for (int i = int(threadIdx.x); i < PA_ROWS * PIECES; i += 256) {
+                const int r = i / PIECES, piece = i % PIECES;
+                const int64_t from = row_query[r];
+                const uint32_t to = staging_smem + uint32_t(r * D * 2 + ((piece ^ (r & 7)) << 4));
+                const __nv_bfloat16* source = args.q + (from < 0 ? 0 : from) + piece * 8;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(source), "r"(from < 0 ? 0 : 16) : "memory");
             }
-            // atom `a` of Q: 32 words of this row
-            auto store_atom = [&](int a, const uint32_t* atom) {
-                if (a < Shape::Q_TMEM_ATOMS) {
-                    pa_tmem_store(lane_address + Shape::TMEM_Q + uint32_t(a) * 32, *reinterpret_cast<const uint32_t(*)[32]>(atom));
-                    return;
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            named_barrier<1, 256>();
+            auto load = [&](int chunk, uint32_t (&words)[32]) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int piece = (parity_group * CHUNKS + chunk) * 8 + i;
+                    const uint4 v = lds_u4(staging_smem + uint32_t(row * D * 2 + ((piece ^ (row & 7)) << 4)));
+                    words[4 * i] = v.x; words[4 * i + 1] = v.y; words[4 * i + 2] = v.z; words[4 * i + 3] = v.w;
                 }
-                const uint32_t line = q_smem + uint32_t(row >> 3) * 1024u + uint32_t(row & 7) * 128u;
-#pragma unroll
-                for (int c = 0; c < 8; ++c) sts_u4(line + uint32_t((c ^ (row & 7)) * 16), atom[4 * c], atom[4 * c + 1], atom[4 * c + 2], atom[4 * c + 3]);
-                fence_async_shared();
             };
+            const uint32_t line = q_smem + uint32_t(row >> 3) * 1024u + uint32_t(row & 7) * 128u;          // of the atom in shared memory
+            auto store_line = [&](int c, const uint32_t* four) { sts_u4(line + uint32_t((c ^ (row & 7)) * 16), four[0], four[1], four[2], four[3]); };
             if (!FP8) {
+#pragma unroll 1
+                for (int chunk = 0; chunk < CHUNKS; ++chunk) {
+                    uint32_t words[32];
+                    load(chunk, words);
+                    const int atom = parity_group * CHUNKS + chunk;
+                    if (atom < Shape::Q_TMEM_ATOMS) {
+                        pa_tmem_store(lane_address + Shape::TMEM_Q + uint32_t(atom) * 32, words);
+                    } else {
 #pragma unroll
-                for (int i = 0; i < WORDS / 32; ++i) store_atom(parity_group * (WORDS / 32) + i, words + 32 * i);
+                        for (int c = 0; c < 8; ++c) store_line(c, words + 4 * c);
+                    }
+                }
             } else {
                 uint32_t largest = 0;      // bf16 magnitude bits: NaN and infinities order above numbers
+#pragma unroll 1
+                for (int chunk = 0; chunk < CHUNKS; ++chunk) {
+                    uint32_t words[32];
+                    load(chunk, words);
 #pragma unroll
-                for (int i = 0; i < WORDS; ++i) largest = max(largest, max(words[i] & 0x7fffu, (words[i] >> 16) & 0x7fffu));
+                    for (int i = 0; i < 32; ++i) largest = max(largest, max(words[i] & 0x7fffu, (words[i] >> 16) & 0x7fffu));
+                }
                 row_exchange[parity_group * PA_ROWS + row] = __uint_as_float(largest);
-                asm volatile("bar.sync 1, 256;" ::: "memory");
+                named_barrier<1, 256>();
                 largest = max(largest, __float_as_uint(row_exchange[(parity_group ^ 1) * PA_ROWS + row]));
                 // 2^e that brings the largest magnitude into [128, 256), kept a normal number
                 int exponent = int(largest >> 7) - 127;
@@ -488,25 +509,33 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
                 const float down = largest == 0u ? 1.0f : __uint_as_float(uint32_t(127 - 7 + exponent) << 23);
                 // a row with an infinity or a NaN: every score is NaN
                 factor = largest >= 0x7f80u ? __uint_as_float(0x7fc00000u) : args.scale_log2 * down;
-                uint32_t high[WORDS / 2], low[WORDS / 2];
+                // hi of this half is columns [HALF_COLUMNS * group, ..), lo the same behind all of hi
+                constexpr uint32_t HALF_COLUMNS = D / 8;
+#pragma unroll 1
+                for (int chunk = 0; chunk < CHUNKS; ++chunk) {
+                    uint32_t words[32], high[16], low[16];
+                    load(chunk, words);
 #pragma unroll
-                for (int i = 0; i < WORDS; ++i) {
-                    const float2 value = bf16x2_to_float2(words[i]);
-                    const float2 scaled = make_float2(value.x * up, value.y * up);
-                    const uint32_t h = __nv_cvt_float2_to_fp8x2(scaled, __NV_SATFINITE, __NV_E4M3);
-                    const float2 back = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(h), __NV_E4M3)));
-                    const uint32_t l = __nv_cvt_float2_to_fp8x2(make_float2(scaled.x - back.x, scaled.y - back.y), __NV_SATFINITE, __NV_E4M3);
-                    high[i >> 1] = (i & 1) ? high[i >> 1] | (h << 16) : h;
-                    low[i >> 1] = (i & 1) ? low[i >> 1] | (l << 16) : l;
-                }
-                if (D == 256) {          // the half row is one atom of hi and one of lo
-                    store_atom(parity_group, high);
-                    store_atom(2 + parity_group, low);
-                } else {
-                    pa_tmem_store16(lane_address + Shape::TMEM_Q + parity_group * 16, high);
-                    pa_tmem_store16(lane_address + Shape::TMEM_Q + 32 + parity_group * 16, low);
+                    for (int i = 0; i < 32; ++i) {
+                        const float2 value = bf16x2_to_float2(words[i]);
+                        const float2 scaled = make_float2(value.x * up, value.y * up);
+                        const uint32_t h = __nv_cvt_float2_to_fp8x2(scaled, __NV_SATFINITE, __NV_E4M3);
+                        const float2 back = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(h), __NV_E4M3)));
+                        const uint32_t l = __nv_cvt_float2_to_fp8x2(make_float2(scaled.x - back.x, scaled.y - back.y), __NV_SATFINITE, __NV_E4M3);
+                        high[i >> 1] = (i & 1) ? high[i >> 1] | (h << 16) : h;
+                        low[i >> 1] = (i & 1) ? low[i >> 1] | (l << 16) : l;
+                    }
+                    const uint32_t column = uint32_t(parity_group) * HALF_COLUMNS + uint32_t(chunk) * 16;
+                    pa_tmem_store16(lane_address + Shape::TMEM_Q + column, high);
+                    if (2 * HALF_COLUMNS + column < Shape::Q_TMEM_ATOMS * 32) {
+                        pa_tmem_store16(lane_address + Shape::TMEM_Q + 2 * HALF_COLUMNS + column, low);
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) store_line(4 * chunk + c, low + 4 * c);
+                    }
                 }
             }
+            fence_async_shared();          // the atom in shared memory; and the staging area is the copies' or the values' again
             pa_tmem_store_wait();
             tc_fence_before_sync();
             __syncwarp();
@@ -653,12 +682,13 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
         // ---- the two groups' results.  One accumulator is in units of the later reference; two have one each.
         if (num_tiles > 0) {
             pa_wait(all_done, 0u, patience);
+            __syncwarp();
             tc_fence_after_sync();
         }
         row_reference[parity_group * PA_ROWS + row] = reference;      // what its last tile left there, or -inf
         row_exchange[parity_group * PA_ROWS + row] = running_sum;
         if (!Shape::SHARED && row == 0) group_unit[parity_group] = unit;
-        asm volatile("bar.sync 1, 256;" ::: "memory");
+        named_barrier<1, 256>();
         const float last = fmaxf(row_reference[row], row_reference[PA_ROWS + row]);
         float weight[2];          // of the groups' sums, and of their accumulators
 #pragma unroll
@@ -688,45 +718,56 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
         };
         const int work_index = kv_head * args.tiles + tile;
         const int first_column = parity_group * (D / 2);          // each group stores half of the columns
-        if (args.splits > 1) {
-            const int64_t partial_row = (int64_t(work_index) * args.splits + split) * PA_ROWS + row;
+        const bool stored = args.splits == 1;
+        const int64_t first_partial = (int64_t(work_index) * args.splits + split) * PA_ROWS;
+        if (!stored && parity_group == 0) {
             const int64_t total_rows = int64_t(args.tiles) * args.kv_heads * args.splits * PA_ROWS;
-            if (parity_group == 0) {
-                if (split == 0) args.row_offsets[int64_t(work_index) * PA_ROWS + row] = out_offset;
-                if (exists) *reinterpret_cast<float2*>(args.partial + total_rows * D + partial_row * 2) = make_float2(reference, running_sum);
-            }
+            if (split == 0) args.row_offsets[int64_t(work_index) * PA_ROWS + row] = out_offset;
+            if (exists) *reinterpret_cast<float2*>(args.partial + total_rows * D + (first_partial + row) * 2) = make_float2(reference, running_sum);
+        }
+        // Rows go out through shared memory (the rings are empty now): a thread has a row of the accumulator, a warp stores whole rows.
+        const float inverse = stored ? (running_sum == 0.0f ? 0.0f : 1.0f / running_sum) : 1.0f;          // sum 0: the row sees no key
+        const uint32_t out_row = base + uint32_t(row) * (stored ? D * 2 : D * 4), row_swizzle = uint32_t(row & 7);
+#pragma unroll 1
+        for (int column = 0; column < D / 2; column += 32) {
+            uint32_t o[32];
             if (num_tiles > 0) {
-                float* destination = args.partial + partial_row * D + first_column;
-#pragma unroll 1
-                for (int column = 0; column < D / 2; column += 32) {
-                    uint32_t o[32];
-                    output_columns(first_column + column, o);
-                    if (exists) {
+                output_columns(first_column + column, o);
+            } else {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const uint32_t eight[8] = {o[8 * i], o[8 * i + 1], o[8 * i + 2], o[8 * i + 3], o[8 * i + 4], o[8 * i + 5], o[8 * i + 6], o[8 * i + 7]};
-                            st_u8(destination + column + i * 8, eight);
-                        }
-                    }
+                for (int i = 0; i < 32; ++i) o[i] = 0u;
+            }
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = running_sum == 0.0f ? 0u : o[i];
+            if (stored) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t words[4];
+#pragma unroll
+                    for (int v = 0; v < 4; ++v)
+                        words[v] = float2_to_bf16x2(make_float2(__uint_as_float(o[8 * i + 2 * v]) * inverse, __uint_as_float(o[8 * i + 2 * v + 1]) * inverse));
+                    const uint32_t piece = uint32_t(first_column + column) / 8 + i;
+                    sts_u4(out_row + ((piece ^ row_swizzle) << 4), words[0], words[1], words[2], words[3]);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const uint32_t piece = uint32_t(first_column + column) / 4 + i;
+                    sts_u4(out_row + ((piece ^ row_swizzle) << 4), o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
                 }
             }
-        } else {
-            // sum 0: the row sees no key
-            const bool empty = running_sum == 0.0f;
-            const float inverse = 1.0f / running_sum;
-#pragma unroll 1
-            for (int column = 0; column < D / 2; column += 32) {
-                uint32_t o[32], words[16];
-                if (num_tiles > 0) output_columns(first_column + column, o);
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    words[i] = empty ? 0u : float2_to_bf16x2(make_float2(__uint_as_float(o[2 * i]) * inverse, __uint_as_float(o[2 * i + 1]) * inverse));
-                if (exists) {
-                    uint4* destination = reinterpret_cast<uint4*>(args.out + out_offset + first_column + column);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) destination[i] = make_uint4(words[4 * i], words[4 * i + 1], words[4 * i + 2], words[4 * i + 3]);
-                }
-            }
+        }
+        named_barrier<1, 256>();
+        constexpr int ROW_SHIFT = D == 256 ? 5 : 4;
+        const int pieces = 1 << (stored ? ROW_SHIFT : ROW_SHIFT + 1);          // 16-byte pieces of a row
+#pragma unroll 4
+        for (int i = int(threadIdx.x); i < PA_ROWS * pieces; i += 256) {
+            const int r = i >> (stored ? ROW_SHIFT : ROW_SHIFT + 1), piece = i & (pieces - 1);
+            const int64_t at = row_output[r];
+            if (at < 0) continue;
+            const uint4 v = lds_u4(base + uint32_t(r * pieces + (piece ^ (r & 7))) * 16);
+            if (stored) *reinterpret_cast<uint4*>(args.out + at + piece * 8) = v;
+            else *reinterpret_cast<uint4*>(args.partial + (first_partial + r) * D + piece * 4) = v;
         }
     } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PA_OTHER_REGISTERS));
@@ -752,6 +793,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
                 }
                 __syncwarp();
                 pa_wait(v_empty + 8 * b, parity ^ 1u, patience);
+                if (j == Shape::FREE_V_STAGES && j < STAGES) pa_wait(q_ready, 0u, patience);          // the queries came through this place
                 __syncwarp();
                 if (elect_one()) {
                     mbar_expect_tx(v_full + 8 * b, Shape::KV_BYTES);
@@ -845,7 +887,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
                     sts_u4(stage + uint32_t((i & (CHUNKS - 1)) >> 3) * Shape::KV_ATOM_BYTES + uint32_t(i / CHUNKS) * 128u + uint32_t(i & 7) * 16u, 0u, 0u, 0u, 0u);
                 if (cursor.segment > 0) {
                     if (thread == 0) bad_keys[b] = 0ull;
-                    asm volatile("bar.sync 2, %0;" ::"n"(32 * Shape::VALUE_WARPS) : "memory");
+                    named_barrier<2, 32 * Shape::VALUE_WARPS>();
 #pragma unroll 4
                     for (int i = thread; i < valid * CHUNKS; i += 32 * Shape::VALUE_WARPS) {
                         const int key = i / CHUNKS;
@@ -871,6 +913,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
         const int thread = (warp - PA_VALUE_WARP) * 32 + lane;
         PaRing<STAGES> ring;
         PaCursor cursor(segment_first, segment_length, num_tiles > 0 ? start_tile : -1);
+        if (num_tiles > 0) pa_wait(q_ready, 0u, patience);          // the queries came through this place
         for (int j = 0; j < num_tiles; ++j) {
             const int c = j & 1, stage = j % PA_SCALE_STAGES;
             const uint32_t* value_scales = reinterpret_cast<const uint32_t*>(generic + Shape::OFF_SCALES) + stage * PA_SCALE_FLOATS + PA_KEYS;
@@ -1043,9 +1086,10 @@ PaPlan pa_plan(const b2_prefix_attention_desc* d) {
     PaPlan plan;
     const int64_t per_member = int64_t(d->heads / d->kv_heads) * d->queries;
     const int64_t per_group = d->batch / d->groups;
-    // unequal groups (their bounds are device data): one partly filled tile per group more than the rows fill
+    // unequal groups (their bounds are device data): n rows have 1 + (n - 1) / 128 tiles, and as many groups as can be have rows
+    const int64_t filled = d->groups < d->batch ? d->groups : d->batch;
     const int64_t tiles = d->members == nullptr ? d->groups * ((per_group * per_member + PA_ROWS - 1) / PA_ROWS)
-                                                : d->batch * per_member / PA_ROWS + (d->groups < d->batch ? d->groups : d->batch);
+                                                : filled + (d->batch * per_member - filled) / PA_ROWS;
     plan.tiles = int(tiles);
     // key tiles of a row tile: the prefix, and the own keys of the members that 128 rows can belong to
     int64_t sharing = (PA_ROWS + per_member - 2) / per_member + 1;
@@ -1078,6 +1122,11 @@ int pa_launch(const b2_prefix_attention_desc* d, const PaPlan& plan, PaArgs& arg
     if (device < 0 || device >= 64 || !configured[device]) {
         const cudaError_t error = cudaFuncSetAttribute(prefix_attention_kernel<D, FP8>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::SHARED_BYTES);
         if (error != cudaSuccess) return int(error);
+        // the softmax warps' registers come out of those that the launch has
+        cudaFuncAttributes attributes{};
+        const cudaError_t found = cudaFuncGetAttributes(&attributes, prefix_attention_kernel<D, FP8>);
+        if (found != cudaSuccess) return int(found);
+        if (attributes.numRegs * Shape::THREADS < 256 * PA_SOFTMAX_REGISTERS + (Shape::THREADS - 256) * PA_OTHER_REGISTERS) return B2_E_UNSUPPORTED;
         if (device >= 0 && device < 64) configured[device] = true;
     }
     // a part that is not there is never read; its map describes the other part
