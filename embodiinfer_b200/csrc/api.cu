@@ -192,7 +192,7 @@ int b2_rope_split(const void* qkv, const void* sine, const void* cosine, void* q
 int b2_rope_axes(const void* positions, int32_t position_bytes, const int32_t* sections, int32_t axes, int64_t tokens,
                  int32_t head_dim, double theta, int32_t flags, void* sine, void* cosine, void* stream) {
     if (positions == nullptr || sections == nullptr || sine == nullptr || cosine == nullptr) return B2_E_INVALID;
-    if (tokens <= 0 || head_dim <= 0 || (flags & ~B2_ROPE_OWN_SPECTRUM) || !(theta > 0.0) || theta > 1.0e300) return B2_E_INVALID;
+    if (tokens <= 0 || head_dim <= 0 || (flags & ~B2_ROPE_OWN_SPECTRUM) || !(theta >= 1.0e-300) || theta > 1.0e300) return B2_E_INVALID;
     if (position_bytes != 4 && position_bytes != 8) return B2_E_INVALID;
     if (axes < 1 || axes > 4 || head_dim % 2 != 0 || head_dim > 1024) return B2_E_UNSUPPORTED;
     int64_t sum = 0;

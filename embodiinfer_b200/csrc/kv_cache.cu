@@ -36,6 +36,7 @@ struct CacheArgs {
     int64_t q_stride[3], stride[2][3];      // elements: batch, head, token
     int64_t factor_batch_stride;
     int batch, tokens, heads, kv_heads, capacity, slots;
+    bool wide;                   // read: every output row starts on 32 bytes
 };
 
 // Cache position of token t of sequence b, or -1: beyond the sequence's length or outside the cache.
@@ -63,7 +64,6 @@ __global__ void __launch_bounds__(CACHE_THREADS) kv_cache_write_kernel(const __g
     const int all_heads = args.heads + 2 * args.kv_heads;
 
     uint4 first[HEADS], second[HEADS];
-    bool any_stored = false;
 #pragma unroll
     for (int i = 0; i < HEADS; ++i) {
         const int head = slot + i * args.slots;
@@ -76,7 +76,6 @@ __global__ void __launch_bounds__(CACHE_THREADS) kv_cache_write_kernel(const __g
             const int which = head >= args.heads + args.kv_heads;
             const int kv_head = head - args.heads - which * args.kv_heads;
             source = args.rows[which] + b * args.stride[which][0] + kv_head * args.stride[which][1] + t * args.stride[which][2];
-            any_stored = true;
         }
         first[i] = ld_nc_u4(reinterpret_cast<const uint4*>(source + lane * 8));
         second[i] = ld_nc_u4(reinterpret_cast<const uint4*>(source + HALF + lane * 8));
@@ -90,7 +89,6 @@ __global__ void __launch_bounds__(CACHE_THREADS) kv_cache_write_kernel(const __g
         s[0] = s0.x; s[1] = s0.y; s[2] = s0.z; s[3] = s0.w; s[4] = s1.x; s[5] = s1.y; s[6] = s1.z; s[7] = s1.w;
         c[0] = c0.x; c[1] = c0.y; c[2] = c0.z; c[3] = c0.w; c[4] = c1.x; c[5] = c1.y; c[6] = c1.z; c[7] = c1.w;
     }
-    any_stored = __any_sync(0xffffffffu, any_stored);
 #pragma unroll
     for (int i = 0; i < HEADS; ++i) {
         const int head = slot + i * args.slots;
@@ -102,7 +100,7 @@ __global__ void __launch_bounds__(CACHE_THREADS) kv_cache_write_kernel(const __g
         unpack_bf16x8(second[i], y);
         if (args.sine != nullptr && exists && which == 0) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
+            for (int j = 0; j < 8; ++j) {          // (the packed multiply and add would be contracted to one rounding)
                 const float low = __fsub_rn(__fmul_rn(x[j], c[j]), __fmul_rn(y[j], s[j]));
                 const float high = __fadd_rn(__fmul_rn(y[j], c[j]), __fmul_rn(x[j], s[j]));
                 x[j] = low;
@@ -116,7 +114,7 @@ __global__ void __launch_bounds__(CACHE_THREADS) kv_cache_write_kernel(const __g
             *reinterpret_cast<uint4*>(out + HALF) = make_uint4(float2_to_bf16x2(make_float2(y[0], y[1])), float2_to_bf16x2(make_float2(y[2], y[3])),
                                                                float2_to_bf16x2(make_float2(y[4], y[5])), float2_to_bf16x2(make_float2(y[6], y[7])));
         }
-        if (!any_stored) continue;      // a warp of queries only
+        if (!__any_sync(0xffffffffu, exists && !is_query)) continue;      // a warp of queries only
         // the largest magnitude as bits: infinities and NaN order above every number
         uint32_t largest = 0;
 #pragma unroll
@@ -200,8 +198,12 @@ __global__ void __launch_bounds__(CACHE_THREADS) kv_cache_read_kernel(const __gr
             values[2 * j] = decode_pair(words[j], scale[i]);
             values[2 * j + 1] = decode_pair(words[j] >> 16, scale[i]);
         }
-        reinterpret_cast<uint4*>(out[i])[0] = make_uint4(values[0], values[1], values[2], values[3]);
-        reinterpret_cast<uint4*>(out[i])[1] = make_uint4(values[4], values[5], values[6], values[7]);
+        if (args.wide) {
+            st_u8(out[i], values);
+        } else {
+            reinterpret_cast<uint4*>(out[i])[0] = make_uint4(values[0], values[1], values[2], values[3]);
+            reinterpret_cast<uint4*>(out[i])[1] = make_uint4(values[4], values[5], values[6], values[7]);
+        }
     }
 }
 
@@ -253,7 +255,9 @@ int launch_kv_cache_write(const b2_kv_cache_desc* desc, cudaStream_t stream) {
 }
 
 int launch_kv_cache_read(const b2_kv_cache_desc* desc, cudaStream_t stream) {
-    const CacheArgs args = cache_args(desc);
+    CacheArgs args = cache_args(desc);
+    args.wide = ((reinterpret_cast<uintptr_t>(desc->k) | reinterpret_cast<uintptr_t>(desc->v)) & 31u) == 0;
+    for (int i = 0; i < 3; ++i) args.wide = args.wide && (desc->k_stride[i] | desc->v_stride[i]) % 16 == 0;
     const int64_t rows = int64_t(args.batch) * args.kv_heads * args.tokens;
     const int64_t block_rows = CACHE_THREADS / (desc->head_dim / 16);
     // as in the write: four rows per thread once the launch fills the device with them

@@ -5,10 +5,11 @@
 //   f_i = theta^(-j / section)         a spectrum of its own for each axis, j counted inside its section
 //   sine[t, i] = sin(position[a(i), t] f_i), cosine likewise, fp32
 //
-// Angles of far positions (a video's 2.6e5th frame at f = 1) have no fraction left in fp32, so the angle is counted in whole
-// turns in 64 bits -- position * (f / 2 pi), of which only the fraction goes on to fp32 -- and sine and cosine are
-// sincospif of twice the fraction: no range reduction by a rounded pi.  Rounding the fraction to fp32 moves the angle by at most
-// pi 2^-25 (9e-8), about the rounding of the result.
+// Angles are counted in turns and in whole numbers: a frequency is held as the fraction of f / 2 pi in 64 bits (2^64 = one turn), and
+// position * fraction modulo 2^64 is the angle's fraction of a turn with nothing lost, however far the position (a video's
+// 2.6e5th frame at f = 1 has no fraction left in fp32).  The top bits name the quadrant, the rest, in [-1/8, 1/8) turns, goes to fp32
+// (an error of 2^-28 turns, 2.3e-8) and into the Taylor series of sine (to the 9th power) and cosine (to the 10th), both at
+// once on the packed fp32 pipe.  Frequencies are formed in fp64, to a few 2^-53 of themselves.
 //
 // Each thread keeps the frequencies of VECTOR neighbouring columns and walks down the tokens: one 16-byte store per table
 // and token, bound by those stores.
@@ -24,43 +25,79 @@ struct AxesArgs {
     const void* positions;
     float* sine;
     float* cosine;
-    double log2_theta;
+    double log2_step[4], step[4];      // of an axis: frequencies are 2^-log2_step, `step`, apart
     int64_t tokens;
     int32_t section[4];
     int32_t axes, half, own_spectrum;
 };
 
+// Sine and cosine of `angle` / 2^64 turns.
+__device__ __forceinline__ void sincos_turns(uint64_t angle, float& sine, float& cosine) {
+    const uint32_t high = uint32_t(angle >> 32), quadrant = (high + 0x20000000u) >> 30;
+    const float r = __fmaf_rn(float(uint32_t(angle)), 5.4210108624275222e-20f, float(int32_t(high - (quadrant << 30))) * 2.3283064365386963e-10f);
+    const float z = r * r;
+    // (2 pi)^n / n! with alternating signs: n = 9, 7, 5, 3, 1 and 10, 8, 6, 4, 2, 0
+    const float2 z2 = make_float2(z, z);
+    float2 sum = make_float2(42.058693944897634f, __fmaf_rn(z, -26.426256783374388f, 60.244641371876661f));
+    sum = __ffma2_rn(sum, z2, make_float2(-76.705859753061360f, -85.456817206693727f));
+    sum = __ffma2_rn(sum, z2, make_float2(81.605249276075040f, 64.939394022668292f));
+    sum = __ffma2_rn(sum, z2, make_float2(-41.341702240399755f, -19.739208802178717f));
+    sum = __ffma2_rn(sum, z2, make_float2(6.2831853071795865f, 1.0f));
+    const float s = sum.x * r;
+    const bool swapped = (quadrant & 1u) != 0;
+    sine = __uint_as_float(__float_as_uint(swapped ? sum.y : s) ^ ((quadrant & 2u) << 30));
+    cosine = __uint_as_float(__float_as_uint(swapped ? s : sum.y) ^ (((quadrant + 1u) & 2u) << 30));
+}
+
 template <typename Position, int VECTOR>
 __global__ void __launch_bounds__(AXES_THREADS) rope_axes_kernel(const __grid_constant__ AxesArgs args, int columns_per_row, int rows_per_block,
                                                                  int64_t row_step) {
     pdl_launch_dependents();
-    const int column = int(threadIdx.x) % columns_per_row;
+    const int column = (blockIdx.y * columns_per_row + int(threadIdx.x) % columns_per_row) * VECTOR;
     const int row = int(threadIdx.x) / columns_per_row;
-    double turns[VECTOR];
+    if (row >= rows_per_block || column >= args.half) return;
+    uint64_t frequency[VECTOR];          // turns of one position, as a fraction of 2^64
     const Position* source[VECTOR];
+    double turns = 0.0;
 #pragma unroll
     for (int v = 0; v < VECTOR; ++v) {
-        const int i = (blockIdx.y * columns_per_row + column) * VECTOR + v;
+        const int i = column + v;
         int axis = 0, start = 0;
         while (axis + 1 < args.axes && i >= start + args.section[axis]) start += args.section[axis++];
-        const double power = args.own_spectrum ? double(i - start) / double(args.section[axis]) : double(i) / double(args.half);
-        turns[v] = exp2(-power * args.log2_theta) * 0.15915494309189535;      // 1 / (2 pi)
+        // neighbours are one ratio apart; an axis' own spectrum begins with 1
+        const int power = args.own_spectrum ? i - start : i;
+        if (v == 0) turns = exp2(-double(power) * args.log2_step[axis]) * 0.15915494309189535;      // 1 / (2 pi)
+        else turns = power == 0 ? 0.15915494309189535 : turns * args.step[axis];
+        frequency[v] = uint64_t(__double2ll_rn((turns - rint(turns)) * 18446744073709551616.0));
         source[v] = static_cast<const Position*>(args.positions) + int64_t(axis) * args.tokens;
     }
-    if (row >= rows_per_block || (blockIdx.y * columns_per_row + column) * VECTOR >= args.half) return;
+    bool one_axis = true;
+#pragma unroll
+    for (int v = 1; v < VECTOR; ++v) one_axis = one_axis && source[v] == source[0];
     pdl_wait();
-    for (int64_t t = int64_t(blockIdx.x) * rows_per_block + row; t < args.tokens; t += row_step) {
-        float s[VECTOR], c[VECTOR];
-        Position position[VECTOR];
-        position[0] = __ldg(source[0] + t);
+    int64_t t = int64_t(blockIdx.x) * rows_per_block + row;
+    Position position[VECTOR];
+    auto load = [&](int64_t at) {
+        position[0] = __ldg(source[0] + at);
+        if (!one_axis) {
 #pragma unroll
-        for (int v = 1; v < VECTOR; ++v) position[v] = source[v] == source[0] ? position[0] : __ldg(source[v] + t);
+            for (int v = 1; v < VECTOR; ++v) position[v] = __ldg(source[v] + at);
+        } else {
 #pragma unroll
-        for (int v = 0; v < VECTOR; ++v) {
-            const double u = double(position[v]) * turns[v];
-            sincospif(2.0f * float(u - rint(u)), &s[v], &c[v]);
+            for (int v = 1; v < VECTOR; ++v) position[v] = position[0];
         }
-        const int64_t out = t * args.half + int64_t(blockIdx.y * columns_per_row + column) * VECTOR;
+    };
+    if (t < args.tokens) load(t);
+    while (t < args.tokens) {
+        uint64_t angle[VECTOR];
+#pragma unroll
+        for (int v = 0; v < VECTOR; ++v) angle[v] = uint64_t(int64_t(position[v])) * frequency[v];
+        const int64_t out = t * args.half + column;
+        t += row_step;
+        if (t < args.tokens) load(t);          // the next row's, while this one is computed
+        float s[VECTOR], c[VECTOR];
+#pragma unroll
+        for (int v = 0; v < VECTOR; ++v) sincos_turns(angle[v], s[v], c[v]);
         if (VECTOR == 4) {
             *reinterpret_cast<float4*>(args.sine + out) = make_float4(s[0], s[1 % VECTOR], s[2 % VECTOR], s[3 % VECTOR]);
             *reinterpret_cast<float4*>(args.cosine + out) = make_float4(c[0], c[1 % VECTOR], c[2 % VECTOR], c[3 % VECTOR]);
@@ -79,9 +116,12 @@ int launch_rope_axes(const void* positions, int position_bytes, const int32_t* s
     args.positions = positions;
     args.sine = static_cast<float*>(sine);
     args.cosine = static_cast<float*>(cosine);
-    args.log2_theta = log2(theta);
     args.tokens = tokens;
-    for (int a = 0; a < axes; ++a) args.section[a] = sections[a];
+    for (int a = 0; a < axes; ++a) {
+        args.section[a] = sections[a];
+        args.log2_step[a] = log2(theta) / (own_spectrum ? sections[a] : head_dim / 2);
+        args.step[a] = exp2(-args.log2_step[a]);
+    }
     args.axes = axes;
     args.half = head_dim / 2;
     args.own_spectrum = own_spectrum;
