@@ -28,20 +28,14 @@ def _ptr(tensor: torch.Tensor | None) -> int | None:
 
 
 def _require_cuda(*tensors: torch.Tensor | None) -> torch.device:
-    first, index = None, -1
-    for tensor in tensors:
-        if tensor is None:
-            continue
-        own = tensor.get_device()          # -1: not on a GPU
-        if own < 0 or not tensor.is_cuda:
+    indices = {tensor.get_device() for tensor in tensors if tensor is not None}          # -1: not on a GPU
+    if len(indices) != 1 or -1 in indices:
+        if -1 in indices:
             raise ValueError("embodiinfer_b200 kernels require CUDA tensors; there is no CPU fallback")
-        if first is None:
-            first, index = tensor, own
-        elif own != index:
-            raise ValueError("all operands must live on one CUDA device")
-    if first is None:
-        raise ValueError("no tensor operands")
-    return first.device
+        raise ValueError("all operands must live on one CUDA device" if indices else "no tensor operands")
+    for tensor in tensors:
+        if tensor is not None:
+            return tensor.device
 
 
 def _on(device: torch.device):
@@ -277,8 +271,13 @@ def rope_axes(positions: torch.Tensor, sections: tuple[int, ...], sine: torch.Te
     if positions.dtype not in (torch.int32, torch.int64) or positions.ndim < 2 or not positions.is_contiguous():
         raise ValueError("rope_axes requires contiguous int32 or int64 positions [axes, ..., tokens]")
     shape = positions.shape
-    axes, half = shape[0], sum(sections)
-    if len(sections) != axes or any(type(section) is not int or section <= 0 for section in sections):
+    axes, half = shape[0], 0
+    for section in sections:
+        if type(section) is not int or section <= 0:
+            axes = -1
+            break
+        half += section
+    if len(sections) != axes:
         raise ValueError("rope_axes requires one positive section for each axis")
     shape = (*shape[1:], half)
     if sine is None and cosine is None:
@@ -322,8 +321,8 @@ def _check_cache(cache: QuantizedKVCache, what: str) -> tuple[int, int, int, int
     return shape
 
 
-def _check_whole(values: torch.Tensor | None, count: int, what: str) -> None:
-    if values is not None and (values.dtype is not torch.int32 or values.shape != (count,) or not values.is_contiguous()):
+def _check_whole(values: torch.Tensor, count: int, what: str) -> None:
+    if values.dtype is not torch.int32 or values.shape != (count,) or not values.is_contiguous():
         raise ValueError(f"{what} must be a contiguous int32 tensor of {count} values")
 
 
@@ -336,8 +335,10 @@ def _check_cache_rows(k: torch.Tensor, v: torch.Tensor, cache: QuantizedKVCache,
     k_stride, v_stride = k.stride(), v.stride()
     if not (k.dtype is torch.bfloat16 is v.dtype and k_stride[3] == 1 == v_stride[3]):
         raise ValueError(f"{what} requires bf16 keys and values whose last dimension is contiguous")
-    _check_whole(offsets, batch, "offsets")
-    _check_whole(lengths, batch, "lengths")
+    if offsets is not None:
+        _check_whole(offsets, batch, "offsets")
+    if lengths is not None:
+        _check_whole(lengths, batch, "lengths")
     return batch, kv_heads, capacity, head_dim, shape[2], (*k_stride[:3], *v_stride[:3])
 
 
@@ -434,9 +435,9 @@ def prefix_attention(q: torch.Tensor, prefix, own=None, *, members: torch.Tensor
         own_bits, _, own_kv_heads, own_capacity, own_pointers = _cache_part(own, batch, head_dim, "own")
         if own_bits != bits or own_kv_heads != kv_heads:
             raise ValueError("prefix_attention requires prefix and own caches of one kind with equal kv_heads")
-    _check_whole(members, groups + 1, "members")
-    _check_whole(prefix_lengths, groups, "prefix_lengths")
-    _check_whole(own_lengths, batch, "own_lengths")
+    for values, count, name in ((members, groups + 1, "members"), (prefix_lengths, groups, "prefix_lengths"), (own_lengths, batch, "own_lengths")):
+        if values is not None:
+            _check_whole(values, count, name)
     if kv_heads == 0 or heads % kv_heads or groups == 0 or (members is None and batch % groups):
         raise ValueError("prefix_attention requires heads divisible by kv_heads, and a batch divisible by the groups unless members is given")
     if out is None:
