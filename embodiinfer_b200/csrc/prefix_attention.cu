@@ -84,6 +84,7 @@ struct PaShape {
     static constexpr int Q_ATOMS = D / 64, Q_TMEM_ATOMS = Q_ATOMS < 3 ? Q_ATOMS : 3, P_BUFFERS = SHARED ? 1 : 2, O_BUFFERS = SHARED ? 1 : 2;
     static constexpr uint32_t TMEM_S = 0, TMEM_O = 2 * PA_KEYS, TMEM_Q = TMEM_O + O_BUFFERS * D, TMEM_P = TMEM_Q + Q_TMEM_ATOMS * 32;
     static_assert(TMEM_P + P_BUFFERS * 32 <= TMEM_COLUMNS, "tensor memory");
+    static_assert(PA_ROWS * (D * 4 + 16) <= 2 * STAGES * KV_BYTES + VALUE_STAGES * VALUE_BYTES, "room of the output's rows");
     static constexpr uint32_t OFF_K = 0;
     static constexpr uint32_t OFF_V = OFF_K + STAGES * KV_BYTES;
     static constexpr uint32_t OFF_VALUES = OFF_V + STAGES * KV_BYTES;
@@ -300,8 +301,8 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
     const uint32_t k_smem = base + Shape::OFF_K, v_smem = base + Shape::OFF_V, values_smem = base + Shape::OFF_VALUES;
     // the queries come in where the values, or the last value tiles, will lie
     const uint32_t q_smem = base + Shape::OFF_Q, staging_smem = FP8 ? values_smem : v_smem + Shape::FREE_V_STAGES * Shape::KV_BYTES;
-    int64_t* const row_output = reinterpret_cast<int64_t*>(generic + Shape::OFF_ROW_OFFSETS);          // [128]: element offset of the row's output, -1: no row
-    int64_t* const row_query = row_output + PA_ROWS;                                                   // [128]: of its query
+    int64_t* const row_query = reinterpret_cast<int64_t*>(generic + Shape::OFF_ROW_OFFSETS);          // [128]: element offset of a row's query, -1: no row
+    int64_t* const row_output = row_query + PA_ROWS;                                                  // [128]: of its output
     float* const row_reference = reinterpret_cast<float*>(generic + Shape::OFF_ROWS);           // [2][128]: of the latest even and odd tile
     float* const row_exchange = row_reference + 2 * PA_ROWS;                                    // [2][128]: row maxima of Q, then the sums
     int* const group_unit = reinterpret_cast<int*>(generic + Shape::OFF_BARS + 720);          // [2]: last units of the accumulators, as exponents
@@ -389,6 +390,8 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
         int rows = group < 0 ? 0 : count * args.rows_per_member - row0;
         rows = rows < 0 ? 0 : (rows > PA_ROWS ? PA_ROWS : rows);
         const int first_own = row0 / args.rows_per_member;                      // first member with rows in this tile
+        if (lane == 0) *work = PaWork{group, first, count, row0, rows, 0, first_own, 0};
+        named_barrier<3, 288>();          // the softmax warps fetch the queries while the lengths come
         const int segments = rows == 0 ? 1 : (row0 + rows - 1) / args.rows_per_member - first_own + 2;
         int total = 0;
         for (int s0 = 0; s0 < segments; s0 += 32) {
@@ -417,7 +420,41 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
         }
         if (lane == 0) {
             segment_first[segments] = total;
-            *work = PaWork{group, first, count, row0, rows, segments, first_own, total};
+            work->segments = segments;
+            work->key_tiles = total;
+        }
+    }
+    // ---- softmax warps: which query a thread has, and all rows of queries on their way
+    bool exists = false;
+    int my_segment = -1, hidden = 0;          // the segment of this row's own keys; causal: how many of them lie behind the query
+    constexpr int PIECES = D / 8;             // 16-byte pieces of a row; in the staging area piece p lies at p ^ (row % 8)
+    if (warp < 8) {
+        named_barrier<3, 288>();
+        const PaWork found = *work;
+        const int row = int(threadIdx.x) & (PA_ROWS - 1);
+        int64_t query_offset = -1, out_offset = -1;
+        exists = row < found.rows;
+        if (exists) {
+            const int member = (found.row0 + row) / args.rows_per_member, inside = found.row0 + row - member * args.rows_per_member;
+            const int head_in_group = inside / args.queries, query = inside - head_in_group * args.queries;
+            const int head = kv_head * (args.heads / args.kv_heads) + head_in_group;
+            my_segment = member - found.first_segment_member + 1;
+            hidden = args.causal ? args.queries - 1 - query : 0;
+            out_offset = ((int64_t(found.first_member + member) * args.heads + head) * args.queries + query) * D;
+            query_offset = int64_t(found.first_member + member) * args.q_stride[0] + head * args.q_stride[1] + query * args.q_stride[2];
+        }
+        if (threadIdx.x < PA_ROWS) {
+            row_query[row] = query_offset;
+            row_output[row] = out_offset;
+        }
+        named_barrier<1, 256>();
+#pragma unroll 4
+        for (int i = int(threadIdx.x); i < PA_ROWS * PIECES; i += 256) {
+            const int r = i / PIECES, piece = i % PIECES;
+            const int64_t from = row_query[r];
+            const uint32_t to = staging_smem + uint32_t(r * D * 2 + ((piece ^ (r & 7)) << 4));
+            const __nv_bfloat16* source = args.q + (from < 0 ? 0 : from) + piece * 8;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(source), "r"(from < 0 ? 0 : 16) : "memory");
         }
     }
     tc_fence_before_sync();
@@ -436,36 +473,12 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
         const int quarter = warp & 3, row = quarter * 32 + lane;          // row of the tile = tensor-memory lane
         const int parity_group = warp >> 2;           // 0: even tiles, 1: odd tiles
         const uint32_t lane_address = tmem_base + (uint32_t(quarter * 32) << 16);
-        const bool exists = row < w.rows;
-        int my_segment = -1, hidden = 0;          // the segment of this row's own keys; causal: how many of them lie behind the query
-        int64_t out_offset = -1, query_offset = -1;
-        if (exists) {
-            const int member = (w.row0 + row) / args.rows_per_member, inside = w.row0 + row - member * args.rows_per_member;
-            const int head_in_group = inside / args.queries, query = inside - head_in_group * args.queries;
-            const int head = kv_head * (args.heads / args.kv_heads) + head_in_group;
-            my_segment = member - w.first_segment_member + 1;
-            hidden = args.causal ? args.queries - 1 - query : 0;
-            out_offset = ((int64_t(w.first_member + member) * args.heads + head) * args.queries + query) * D;
-            query_offset = int64_t(w.first_member + member) * args.q_stride[0] + head * args.q_stride[1] + query * args.q_stride[2];
-        }
-        if (parity_group == 0) row_output[row] = out_offset;          // read behind the barrier at the end
-        // ---- the queries into tensor memory: rows come to shared memory as they lie (16 bytes per thread), each thread then takes one half of
-        // the columns of its row
+        // ---- the queries into tensor memory: rows came to shared memory as they lie (16 bytes per thread), each thread takes one half of the
+        // columns of its row
         float factor = args.scale_log2;
+        asm volatile("cp.async.wait_all;" ::: "memory");
         if (num_tiles > 0) {
             constexpr int CHUNKS = D / 128;          // of 32 words (64 values) of half a bf16 row
-            constexpr int PIECES = D / 8;            // 16-byte pieces of a row; piece p lies at p ^ (row % 8)
-            if (parity_group == 1) row_query[row] = query_offset;
-            named_barrier<1, 256>();
-#pragma unroll 4
-            for (int i = int(threadIdx.x); i < PA_ROWS * PIECES; i += 256) {
-                const int r = i / PIECES, piece = i % PIECES;
-                const int64_t from = row_query[r];
-                const uint32_t to = staging_smem + uint32_t(r * D * 2 + ((piece ^ (r & 7)) << 4));
-                const __nv_bfloat16* source = args.q + (from < 0 ? 0 : from) + piece * 8;
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(source), "r"(from < 0 ? 0 : 16) : "memory");
-            }
-            asm volatile("cp.async.wait_all;" ::: "memory");
             named_barrier<1, 256>();
             auto load = [&](int chunk, uint32_t (&words)[32]) {
 #pragma unroll
@@ -497,8 +510,9 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
                     uint32_t words[32];
                     load(chunk, words);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) largest = max(largest, max(words[i] & 0x7fffu, (words[i] >> 16) & 0x7fffu));
+                    for (int i = 0; i < 32; ++i) largest = __vmaxu2(largest, words[i] & 0x7fff7fffu);
                 }
+                largest = max(largest & 0xffffu, largest >> 16);
                 row_exchange[parity_group * PA_ROWS + row] = __uint_as_float(largest);
                 named_barrier<1, 256>();
                 largest = max(largest, __float_as_uint(row_exchange[(parity_group ^ 1) * PA_ROWS + row]));
@@ -509,6 +523,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
                 const float down = largest == 0u ? 1.0f : __uint_as_float(uint32_t(127 - 7 + exponent) << 23);
                 // a row with an infinity or a NaN: every score is NaN
                 factor = largest >= 0x7f80u ? __uint_as_float(0x7fc00000u) : args.scale_log2 * down;
+                const __nv_bfloat162 up2 = __float2bfloat162_rn(up);
                 // hi of this half is columns [HALF_COLUMNS * group, ..), lo the same behind all of hi
                 constexpr uint32_t HALF_COLUMNS = D / 8;
 #pragma unroll 1
@@ -517,11 +532,12 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
                     load(chunk, words);
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
-                        const float2 value = bf16x2_to_float2(words[i]);
-                        const float2 scaled = make_float2(value.x * up, value.y * up);
-                        const uint32_t h = __nv_cvt_float2_to_fp8x2(scaled, __NV_SATFINITE, __NV_E4M3);
-                        const float2 back = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(h), __NV_E4M3)));
-                        const uint32_t l = __nv_cvt_float2_to_fp8x2(make_float2(scaled.x - back.x, scaled.y - back.y), __NV_SATFINITE, __NV_E4M3);
+                        // of the 8 significant bits hi takes the upper 4 and lo the lower: both exact above e4m3's smallest step
+                        const __nv_bfloat162 x = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&words[i]), up2);
+                        const uint32_t upper = *reinterpret_cast<const uint32_t*>(&x) & 0xfff0fff0u;
+                        const __nv_bfloat162 rest = __hsub2(x, *reinterpret_cast<const __nv_bfloat162*>(&upper));
+                        const uint32_t h = __nv_cvt_float2_to_fp8x2(bf16x2_to_float2(upper), __NV_SATFINITE, __NV_E4M3);
+                        const uint32_t l = __nv_cvt_float2_to_fp8x2(bf16x2_to_float2(*reinterpret_cast<const uint32_t*>(&rest)), __NV_SATFINITE, __NV_E4M3);
                         high[i >> 1] = (i & 1) ? high[i >> 1] | (h << 16) : h;
                         low[i >> 1] = (i & 1) ? low[i >> 1] | (l << 16) : l;
                     }
@@ -626,6 +642,8 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
                     unit = tile_unit;
                 }
             }
+            const uint32_t output_bar = o_done + 8 * (Shape::SHARED ? parity_group ^ 1 : parity_group);
+            const uint32_t output_phase = Shape::SHARED && parity_group == 1 ? phase : phase ^ 1u;
             uint32_t packed[32];
             if (none) {
 #pragma unroll
@@ -658,8 +676,8 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
             // the P that lies where this one goes has been read, and O holds everything before this tile: the product of the tile before, or
             // of this group's last, is done
             if (j >= Shape::P_BUFFERS) {
-                if (Shape::SHARED) pa_wait(o_done + 8 * (parity_group ^ 1), parity_group == 0 ? phase ^ 1u : phase, patience);
-                else pa_wait(o_done + 8 * parity_group, phase ^ 1u, patience);
+                pa_wait(output_bar, output_phase, patience);
+                __syncwarp();
                 tc_fence_after_sync();
                 if (__any_sync(0xffffffffu, correction != 1.0f)) {
 #pragma unroll 1
@@ -701,19 +719,24 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
         } else if (Shape::SHARED) {
             weight[0] = 1.0f;
         }
-        // 32 columns of the row in units of the reference
-        auto output_columns = [&](int column, uint32_t (&o)[32]) {
-            tmem_load_32x32(lane_address + Shape::TMEM_O + column, o);
-            if (!Shape::SHARED && num_tiles > 1) {
+        // 32 columns of the row (D = 256: 64) in units of the reference
+        auto output_columns = [&](int column, auto& o) {
+            tmem_load_32x32(lane_address + Shape::TMEM_O + column, o[0]);
+            if constexpr (Shape::SHARED) {
+                tmem_load_32x32(lane_address + Shape::TMEM_O + column + 32, o[1]);
+                tmem_load_wait();
+#pragma unroll
+                for (int i = 0; i < 64; ++i) o[i / 32][i % 32] = __float_as_uint(__uint_as_float(o[i / 32][i % 32]) * weight[0]);
+            } else if (num_tiles > 1) {
                 uint32_t other[32];
                 tmem_load_32x32(lane_address + Shape::TMEM_O + D + column, other);
                 tmem_load_wait();
 #pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * weight[0] + __uint_as_float(other[i]) * weight[1]);
+                for (int i = 0; i < 32; ++i) o[0][i] = __float_as_uint(__uint_as_float(o[0][i]) * weight[0] + __uint_as_float(other[i]) * weight[1]);
             } else {
                 tmem_load_wait();
 #pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * weight[0]);
+                for (int i = 0; i < 32; ++i) o[0][i] = __float_as_uint(__uint_as_float(o[0][i]) * weight[0]);
             }
         };
         const int work_index = kv_head * args.tiles + tile;
@@ -722,85 +745,86 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
         const int64_t first_partial = (int64_t(work_index) * args.splits + split) * PA_ROWS;
         if (!stored && parity_group == 0) {
             const int64_t total_rows = int64_t(args.tiles) * args.kv_heads * args.splits * PA_ROWS;
-            if (split == 0) args.row_offsets[int64_t(work_index) * PA_ROWS + row] = out_offset;
+            if (split == 0) args.row_offsets[int64_t(work_index) * PA_ROWS + row] = row_output[row];
             if (exists) *reinterpret_cast<float2*>(args.partial + total_rows * D + (first_partial + row) * 2) = make_float2(reference, running_sum);
         }
-        // Rows go out through shared memory (the rings are empty now): a thread has a row of the accumulator, a warp stores whole rows.
+        // Rows go out through shared memory (the rings are empty now), a bulk copy for each: a thread has a row of the accumulator, and its
+        // own stores would touch a sector at a time.  16 bytes between rows spread them over the banks.
         const float inverse = stored ? (running_sum == 0.0f ? 0.0f : 1.0f / running_sum) : 1.0f;          // sum 0: the row sees no key
-        const uint32_t out_row = base + uint32_t(row) * (stored ? D * 2 : D * 4), row_swizzle = uint32_t(row & 7);
+        const uint32_t row_bytes = stored ? D * 2 : D * 4, out_row = base + uint32_t(row) * (row_bytes + 16);
+        constexpr int BATCH = Shape::SHARED ? 2 : 1;          // of 32 columns
 #pragma unroll 1
-        for (int column = 0; column < D / 2; column += 32) {
-            uint32_t o[32];
+        for (int column = first_column; column < first_column + D / 2; column += 32 * BATCH) {
+            uint32_t o[BATCH][32];
             if (num_tiles > 0) {
-                output_columns(first_column + column, o);
+                output_columns(column, o);
             } else {
 #pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] = 0u;
+                for (int i = 0; i < 32 * BATCH; ++i) o[i / 32][i % 32] = 0u;
             }
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = running_sum == 0.0f ? 0u : o[i];
-            if (stored) {
+            for (int i = 0; i < 4 * BATCH; ++i) {
+                uint32_t eight[8];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int v = 0; v < 8; ++v) {
+                    const uint32_t value = o[i / 4][(8 * i + v) % 32];
+                    eight[v] = running_sum == 0.0f ? 0u : __float_as_uint(__uint_as_float(value) * inverse);
+                }
+                if (stored) {
                     uint32_t words[4];
 #pragma unroll
-                    for (int v = 0; v < 4; ++v)
-                        words[v] = float2_to_bf16x2(make_float2(__uint_as_float(o[8 * i + 2 * v]) * inverse, __uint_as_float(o[8 * i + 2 * v + 1]) * inverse));
-                    const uint32_t piece = uint32_t(first_column + column) / 8 + i;
-                    sts_u4(out_row + ((piece ^ row_swizzle) << 4), words[0], words[1], words[2], words[3]);
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const uint32_t piece = uint32_t(first_column + column) / 4 + i;
-                    sts_u4(out_row + ((piece ^ row_swizzle) << 4), o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                    for (int v = 0; v < 4; ++v) words[v] = float2_to_bf16x2(make_float2(__uint_as_float(eight[2 * v]), __uint_as_float(eight[2 * v + 1])));
+                    sts_u4(out_row + (column + 8 * i) * 2, words[0], words[1], words[2], words[3]);
+                } else {
+                    sts_u4(out_row + (column + 8 * i) * 4, eight[0], eight[1], eight[2], eight[3]);
+                    sts_u4(out_row + (column + 8 * i) * 4 + 16, eight[4], eight[5], eight[6], eight[7]);
                 }
             }
         }
+        fence_async_shared();
         named_barrier<1, 256>();
-        constexpr int ROW_SHIFT = D == 256 ? 5 : 4;
-        const int pieces = 1 << (stored ? ROW_SHIFT : ROW_SHIFT + 1);          // 16-byte pieces of a row
-#pragma unroll 4
-        for (int i = int(threadIdx.x); i < PA_ROWS * pieces; i += 256) {
-            const int r = i >> (stored ? ROW_SHIFT : ROW_SHIFT + 1), piece = i & (pieces - 1);
-            const int64_t at = row_output[r];
-            if (at < 0) continue;
-            const uint4 v = lds_u4(base + uint32_t(r * pieces + (piece ^ (r & 7))) * 16);
-            if (stored) *reinterpret_cast<uint4*>(args.out + at + piece * 8) = v;
-            else *reinterpret_cast<uint4*>(args.partial + (first_partial + r) * D + piece * 4) = v;
+        if (exists && parity_group == 0) {
+            const void* destination = stored ? static_cast<const void*>(args.out + row_output[row]) : static_cast<const void*>(args.partial + (first_partial + row) * D);
+            asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(destination), "r"(out_row), "r"(row_bytes) : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");          // the rows have been taken: the CTA may leave
         }
     } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PA_OTHER_REGISTERS));
     if (warp == PA_LOAD_WARP) {
         // ------------------------------------------------------------- TMA producer
         if (num_tiles > 0) {
-            PaCursor cursor(segment_first, segment_length, start_tile);
-            for (int j = 0; j < num_tiles; ++j) {
-                cursor.seek(start_tile + j);
+            auto load = [&](const PaCursor& cursor, const CUtensorMap& prefix_map, const CUtensorMap& own_map, uint32_t smem, uint32_t full, int j) {
                 const int b = j % STAGES;
-                const uint32_t parity = uint32_t(j / STAGES) & 1u;
                 const bool prefix = cursor.segment == 0;
-                const CUtensorMap* k_map = prefix ? &prefix_k_map : &own_k_map;
-                const CUtensorMap* v_map = prefix ? &prefix_v_map : &own_v_map;
                 const int sequence = prefix ? w.group : w.first_member + w.first_segment_member + cursor.segment - 1;
                 const int row = (sequence * args.kv_heads + kv_head) * (prefix ? args.prefix_capacity : args.own_capacity) + cursor.first_key(start_tile + j);
-                pa_wait(k_empty + 8 * b, parity ^ 1u, patience);
                 __syncwarp();
                 if (elect_one()) {
-                    mbar_expect_tx(k_full + 8 * b, Shape::KV_BYTES);
+                    mbar_expect_tx(full + 8 * b, Shape::KV_BYTES);
                     for (int a = 0; a < Shape::KV_ATOMS; ++a)
-                        tma_load_2d(k_smem + b * Shape::KV_BYTES + a * Shape::KV_ATOM_BYTES, k_map, k_full + 8 * b, a * 128, row);
+                        tma_load_2d(smem + b * Shape::KV_BYTES + a * Shape::KV_ATOM_BYTES, prefix ? &prefix_map : &own_map, full + 8 * b, a * 128, row);
                 }
                 __syncwarp();
-                pa_wait(v_empty + 8 * b, parity ^ 1u, patience);
-                if (j == Shape::FREE_V_STAGES && j < STAGES) pa_wait(q_ready, 0u, patience);          // the queries came through this place
-                __syncwarp();
-                if (elect_one()) {
-                    mbar_expect_tx(v_full + 8 * b, Shape::KV_BYTES);
-                    for (int a = 0; a < Shape::KV_ATOMS; ++a)
-                        tma_load_2d(v_smem + b * Shape::KV_BYTES + a * Shape::KV_ATOM_BYTES, v_map, v_full + 8 * b, a * 128, row);
+            };
+            // D = 256: keys go two tiles ahead of values, because the scores run ahead of the output and a value slot is free only behind
+            // the output (fifty-query chunks over 8192 keys: 213 us, in step 219).  D = 128 has the slots to go in step (a 32768-key prefix:
+            // 83 us, ahead 86).
+            constexpr int AHEAD = Shape::SHARED ? 2 : 0;
+            PaCursor key_cursor(segment_first, segment_length, start_tile), value_cursor(segment_first, segment_length, start_tile);
+            for (int i = 0; i < num_tiles + AHEAD; ++i) {
+                if (i < num_tiles) {
+                    key_cursor.seek(start_tile + i);
+                    pa_wait(k_empty + 8 * (i % STAGES), (uint32_t(i / STAGES) & 1u) ^ 1u, patience);
+                    load(key_cursor, prefix_k_map, own_k_map, k_smem, k_full, i);
                 }
-                __syncwarp();
+                const int j = i - AHEAD;
+                if (j >= 0) {
+                    if (AHEAD > 0) value_cursor.seek(start_tile + j);
+                    pa_wait(v_empty + 8 * (j % STAGES), (uint32_t(j / STAGES) & 1u) ^ 1u, patience);
+                    if (j == Shape::FREE_V_STAGES && j < STAGES) pa_wait(q_ready, 0u, patience);          // the queries came through this place
+                    load(AHEAD > 0 ? value_cursor : key_cursor, prefix_v_map, own_v_map, v_smem, v_full, j);
+                }
             }
             // every copy has landed before this CTA may leave (on the normal path the readers have long seen them)
             for (int b = 0; b < STAGES && b < num_tiles; ++b) {
@@ -909,7 +933,8 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
         // 16 codes of a key per thread and step: chunk `piece` of its row (stored at piece ^ (key % 8) inside its 128-byte group)
         // becomes two 16-byte chunks of the 64-column group they belong to.  Odd groups store their two chunks in the other order: the
         // eight lanes of a store then meet all banks.
-        constexpr int PIECES = D / 16;
+        constexpr int PIECES = D / 16, BATCH = 4;
+        static_assert(PA_KEYS * PIECES % (BATCH * 32 * Shape::VALUE_WARPS) == 0, "whole batches");
         const int thread = (warp - PA_VALUE_WARP) * 32 + lane;
         PaRing<STAGES> ring;
         PaCursor cursor(segment_first, segment_length, num_tiles > 0 ? start_tile : -1);
@@ -925,19 +950,29 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
             pa_wait(value_empty + 8 * c, (uint32_t(j >> 1) & 1u) ^ 1u, patience);
             auto convert = [&](auto tag) {
                 constexpr bool CLEAN = decltype(tag)::value;
-#pragma unroll 4
-                for (int i = thread; i < PA_KEYS * PIECES; i += 32 * Shape::VALUE_WARPS) {
-                    const uint32_t key = uint32_t(i) / PIECES, piece = uint32_t(i) % PIECES, swizzle = key & 7u;
-                    const uint4 codes = lds_u4(v_smem + ring.slot * Shape::KV_BYTES + (piece >> 3) * Shape::KV_ATOM_BYTES + key * 128u + (((piece & 7u) ^ swizzle) << 4));
-                    const uint32_t scale_bits = value_scales[key];
-                    const __half2 scale = *reinterpret_cast<const __half2*>(&scale_bits);
-                    const uint32_t group = values_smem + c * Shape::VALUE_BYTES + (piece >> 2) * Shape::KV_ATOM_BYTES + key * 128u;
-                    const uint32_t odd = (piece >> 2) & 1u, left = (piece & 3u) * 2u;
-                    const uint32_t x = odd ? codes.z : codes.x, y = odd ? codes.w : codes.y, z = odd ? codes.x : codes.z, w = odd ? codes.y : codes.w;
-                    sts_u4(group + (((left + odd) ^ swizzle) << 4), codes_to_halves<CLEAN>(x, scale), codes_to_halves<CLEAN>(x >> 16, scale),
-                           codes_to_halves<CLEAN>(y, scale), codes_to_halves<CLEAN>(y >> 16, scale));
-                    sts_u4(group + (((left + 1u - odd) ^ swizzle) << 4), codes_to_halves<CLEAN>(z, scale), codes_to_halves<CLEAN>(z >> 16, scale),
-                           codes_to_halves<CLEAN>(w, scale), codes_to_halves<CLEAN>(w >> 16, scale));
+#pragma unroll 1
+                for (int first = thread; first < PA_KEYS * PIECES; first += BATCH * 32 * Shape::VALUE_WARPS) {
+                    uint4 codes[BATCH];
+                    uint32_t scale_bits[BATCH];
+#pragma unroll
+                    for (int n = 0; n < BATCH; ++n) {          // all loads first: each of the stores would hold the next load back
+                        const uint32_t i = first + n * 32 * Shape::VALUE_WARPS, key = i / PIECES, piece = i % PIECES;
+                        codes[n] = lds_u4(v_smem + ring.slot * Shape::KV_BYTES + (piece >> 3) * Shape::KV_ATOM_BYTES + key * 128u + (((piece & 7u) ^ (key & 7u)) << 4));
+                        scale_bits[n] = value_scales[key];
+                    }
+#pragma unroll
+                    for (int n = 0; n < BATCH; ++n) {
+                        const uint32_t i = first + n * 32 * Shape::VALUE_WARPS, key = i / PIECES, piece = i % PIECES, swizzle = key & 7u;
+                        const __half2 scale = *reinterpret_cast<const __half2*>(&scale_bits[n]);
+                        const uint32_t group = values_smem + c * Shape::VALUE_BYTES + (piece >> 2) * Shape::KV_ATOM_BYTES + key * 128u;
+                        const uint32_t odd = (piece >> 2) & 1u, left = (piece & 3u) * 2u;
+                        const uint32_t x = odd ? codes[n].z : codes[n].x, y = odd ? codes[n].w : codes[n].y;
+                        const uint32_t z = odd ? codes[n].x : codes[n].z, w = odd ? codes[n].y : codes[n].w;
+                        sts_u4(group + (((left + odd) ^ swizzle) << 4), codes_to_halves<CLEAN>(x, scale), codes_to_halves<CLEAN>(x >> 16, scale),
+                               codes_to_halves<CLEAN>(y, scale), codes_to_halves<CLEAN>(y >> 16, scale));
+                        sts_u4(group + (((left + 1u - odd) ^ swizzle) << 4), codes_to_halves<CLEAN>(z, scale), codes_to_halves<CLEAN>(z >> 16, scale),
+                               codes_to_halves<CLEAN>(w, scale), codes_to_halves<CLEAN>(w >> 16, scale));
+                    }
                 }
             };
             if (clean) convert(std::true_type{});
