@@ -38,8 +38,10 @@
 //   would spare the conversion of V, have no room for a long tail of weights 2^-15 below the largest).
 //   A scale that is not finite zeroes its row of values and marks the key: rows that see it get NaN from their sum.
 //
-// Few CTAs: the key tiles of a row tile are cut across `splits` CTAs, which leave O, M and L in fp32 in the workspace; a second
-// launch joins them in split order (no atomics: the result does not depend on timing).
+// Row tiles that do not fill the device -- all of a small call's, or those of the last, partial wave -- have their key tiles cut across
+// several CTAs, which leave O, M and L in fp32 in the workspace; a second launch joins them in their order (no atomics: the result does
+// not depend on timing).  The host bounds the row tiles and sizes the launch; how many there are, and so the cut, each CTA works out
+// from the groups' bounds on the device.
 #include "gemm_epilogue.cuh"
 
 #include <cuda.h>
@@ -106,18 +108,20 @@ struct PaArgs {
     const int32_t* members;           // [groups + 1] or nullptr: batch / groups each
     const int32_t* prefix_lengths;    // or nullptr: the capacity
     const int32_t* own_lengths;
-    float* partial;                   // splits > 1: O [work][splits][128][D], then (M, L) [work][splits][128][2]
-    int64_t* row_offsets;             // splits > 1: element offset of each row's output, -1 for rows that do not exist [work][128]
+    float* partial;                   // O [slots][128][D], then (M, L) [slots][128][2]
+    int64_t* row_offsets;             // of the row tiles that are cut: element offset of each row's output, -1 for rows that do not exist [slots / 2][128]
+    int32_t* cut;                     // [2], 8-byte aligned: how many row tiles are cut, and into how many parts each
     unsigned int* status;
     int64_t q_stride[3];
     float scale_log2;
     int batch, groups, heads, kv_heads, queries, prefix_capacity, own_capacity;
-    int rows_per_member, tiles, splits, causal;
+    int rows_per_member, sms, slots, max_splits, causal;      // slots: CTAs that may leave partial rows; 0 = nothing is cut
 };
 
 // What a CTA works on, in shared memory: written by warp 0 before the block barrier.
 struct PaWork {
-    int group, first_member, member_count, row0, rows, segments, first_segment_member, key_tiles;
+    int group, first_member, row0, rows, segments, first_segment_member, key_tiles;
+    int kv_head, split, splits, place;      // place: among the row tiles that are cut, and in all of their parts (split * row tiles + it)
 };
 
 __device__ __forceinline__ int clamp_length(int value, int capacity) { return value < 0 ? 0 : (value > capacity ? capacity : value); }
@@ -321,10 +325,6 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
     unsigned long long* const bad_keys = reinterpret_cast<unsigned long long*>(generic + Shape::OFF_BARS + 640);      // bf16: [STAGES]
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    // row tile fastest: CTAs that run together share the key tiles of their group in the L2
-    const int tile = int(blockIdx.x) % args.tiles;
-    const int kv_head = (int(blockIdx.x) / args.tiles) % args.kv_heads;
-    const int split = int(blockIdx.x) / (args.tiles * args.kv_heads);
 
     if (warp == 0) {          // one lane per barrier (8 bytes each, in the order above); unused places of the arrays are barriers too
         for (int i = lane; i < 74; i += 32) {
@@ -352,23 +352,52 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
     if (warp == PA_LOAD_WARP) {
         // ---- which rows, which keys
         int group = -1, first = 0, count = 0, group_tile = 0;
+        auto group_members = [&](int g, int& a) {
+            a = clamp_length(__ldg(args.members + g), args.batch);
+            const int n = clamp_length(__ldg(args.members + g + 1), args.batch) - a;
+            return n < 0 ? 0 : n;
+        };
+        auto row_tiles = [&](int n) { return (n * args.rows_per_member + PA_ROWS - 1) / PA_ROWS; };
+        constexpr int MANY = 1 << 29;          // bounds that run backwards may add up to anything: enough for every CTA
+        int total_tiles = 0;
         if (args.members == nullptr) {
+            total_tiles = args.groups * row_tiles(args.batch / args.groups);
+        } else {
+            for (int g0 = 0; g0 < args.groups && total_tiles < MANY; g0 += 32) {
+                int a;
+                total_tiles += __reduce_add_sync(0xffffffffu, g0 + lane < args.groups ? row_tiles(group_members(g0 + lane, a)) : 0);
+            }
+        }
+        // ---- which row tile and head, and which part of its keys: whole waves of them uncut, the rest cut into equal parts
+        const int ctas = int(gridDim.x), block = int(blockIdx.x);
+        const int items = int(min(int64_t(total_tiles) * args.kv_heads, int64_t(ctas)));
+        const int uncut = items > args.sms ? items / args.sms * args.sms : 0, rest = items - uncut;
+        int splits = 1, split = 0, place = 0, item = block;
+        if (rest > 0) splits = max(1, min(args.max_splits, min(args.slots, ctas - uncut) / rest));
+        if (block >= uncut) {
+            place = block - uncut;
+            split = rest > 0 ? place / rest : splits;
+            item = uncut + place - split * rest;
+        }
+        if (block == 0 && lane == 0 && args.slots > 0) {
+            args.cut[0] = splits > 1 ? rest : 0;
+            args.cut[1] = splits;
+        }
+        // row tile fastest: CTAs that run together share the key tiles of their group in the L2
+        const int kv_head = total_tiles > 0 ? item / total_tiles : 0, tile = item - kv_head * total_tiles;
+        if (split >= splits) {
+            group = -1;          // nothing left for this one
+        } else if (args.members == nullptr) {
             count = args.batch / args.groups;
-            const int per_group = (count * args.rows_per_member + PA_ROWS - 1) / PA_ROWS;
-            group = tile / per_group;
-            group_tile = tile - group * per_group;
+            group = tile / row_tiles(count);
+            group_tile = tile - group * row_tiles(count);
             first = group * count;
         } else {
             int before = 0;
-            for (int g0 = 0; g0 < args.groups && group < 0; g0 += 32) {
+            for (int g0 = 0; g0 < args.groups && group < 0 && before < MANY; g0 += 32) {
                 const int g = g0 + lane;
-                int a = 0, n = 0;
-                if (g < args.groups) {
-                    a = clamp_length(__ldg(args.members + g), args.batch);
-                    n = clamp_length(__ldg(args.members + g + 1), args.batch) - a;
-                    n = n < 0 ? 0 : n;
-                }
-                const int mine = (n * args.rows_per_member + PA_ROWS - 1) / PA_ROWS;
+                int a = 0;
+                const int n = g < args.groups ? group_members(g, a) : 0, mine = row_tiles(n);
                 int sum = mine;
 #pragma unroll
                 for (int step = 1; step < 32; step <<= 1) {
@@ -390,7 +419,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
         int rows = group < 0 ? 0 : count * args.rows_per_member - row0;
         rows = rows < 0 ? 0 : (rows > PA_ROWS ? PA_ROWS : rows);
         const int first_own = row0 / args.rows_per_member;                      // first member with rows in this tile
-        if (lane == 0) *work = PaWork{group, first, count, row0, rows, 0, first_own, 0};
+        if (lane == 0) *work = PaWork{group, first, row0, rows, 0, first_own, 0, kv_head, split, rows > 0 && block >= uncut ? splits : 1, place};
         named_barrier<3, 288>();          // the softmax warps fetch the queries while the lengths come
         const int segments = rows == 0 ? 1 : (row0 + rows - 1) / args.rows_per_member - first_own + 2;
         int total = 0;
@@ -437,7 +466,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
         if (exists) {
             const int member = (found.row0 + row) / args.rows_per_member, inside = found.row0 + row - member * args.rows_per_member;
             const int head_in_group = inside / args.queries, query = inside - head_in_group * args.queries;
-            const int head = kv_head * (args.heads / args.kv_heads) + head_in_group;
+            const int head = found.kv_head * (args.heads / args.kv_heads) + head_in_group;
             my_segment = member - found.first_segment_member + 1;
             hidden = args.causal ? args.queries - 1 - query : 0;
             out_offset = ((int64_t(found.first_member + member) * args.heads + head) * args.queries + query) * D;
@@ -463,8 +492,8 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
     uint32_t tmem_base;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem_base) : "r"(tmem_slot) : "memory");
     const PaWork w = *work;
-    const int start_tile = int(int64_t(w.key_tiles) * split / args.splits);
-    const int num_tiles = int(int64_t(w.key_tiles) * (split + 1) / args.splits) - start_tile;
+    const int kv_head = w.kv_head, start_tile = int(int64_t(w.key_tiles) * w.split / w.splits);
+    const int num_tiles = int(int64_t(w.key_tiles) * (w.split + 1) / w.splits) - start_tile;
 
     uint32_t patience = PA_PATIENCE;
     if (warp < 8) {
@@ -739,14 +768,12 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
                 for (int i = 0; i < 32; ++i) o[0][i] = __float_as_uint(__uint_as_float(o[0][i]) * weight[0]);
             }
         };
-        const int work_index = kv_head * args.tiles + tile;
         const int first_column = parity_group * (D / 2);          // each group stores half of the columns
-        const bool stored = args.splits == 1;
-        const int64_t first_partial = (int64_t(work_index) * args.splits + split) * PA_ROWS;
+        const bool stored = w.splits == 1;
+        const int64_t first_partial = int64_t(w.place) * PA_ROWS;
         if (!stored && parity_group == 0) {
-            const int64_t total_rows = int64_t(args.tiles) * args.kv_heads * args.splits * PA_ROWS;
-            if (split == 0) args.row_offsets[int64_t(work_index) * PA_ROWS + row] = row_output[row];
-            if (exists) *reinterpret_cast<float2*>(args.partial + total_rows * D + (first_partial + row) * 2) = make_float2(reference, running_sum);
+            if (w.split == 0) args.row_offsets[first_partial + row] = row_output[row];
+            if (exists) *reinterpret_cast<float2*>(args.partial + int64_t(args.slots) * PA_ROWS * D + (first_partial + row) * 2) = make_float2(reference, running_sum);
         }
         // Rows go out through shared memory (the rings are empty now), a bulk copy for each: a thread has a row of the accumulator, and its
         // own stores would touch a sector at a time.  16 bytes between rows spread them over the banks.
@@ -1076,45 +1103,84 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
     }
 }
 
-// out = sum_s 2^(M_s - M) O_s / sum_s 2^(M_s - M) L_s in split order; one row per D / 8 lanes.
+// out = sum_s 2^(M_s - M) O_s / sum_s 2^(M_s - M) L_s; D / 8 lanes per row, each with 8 columns.  The time is latency: everything that does
+// not need another load's result is on its way before that result is waited for.
 template <int D>
-__global__ void __launch_bounds__(256) prefix_attention_join_kernel(const float* __restrict__ partial, const int64_t* __restrict__ row_offsets,
-                                                                    __nv_bfloat16* __restrict__ out, int64_t rows, int splits) {
+__global__ void __launch_bounds__(256) prefix_attention_join_kernel(const __grid_constant__ PaArgs args) {
     pdl_launch_dependents();
-    pdl_wait();
-    constexpr int LANES = D / 8;
+    constexpr int LANES = D / 8, PER_LANE = 64 / LANES, BATCH = 8;
     const int64_t index = (int64_t(blockIdx.x) * 256 + threadIdx.x) / LANES;
     const int lane = threadIdx.x % LANES;
-    if (index >= rows) return;
-    const int64_t offset = row_offsets[index];
-    if (offset < 0) return;
-    const int64_t work = index / PA_ROWS, row = index - work * PA_ROWS;
-    const float* statistics = partial + rows * splits * D;
-    float top = -INFINITY;
-    for (int s = 0; s < splits; ++s) top = fmaxf(top, statistics[((work * splits + s) * PA_ROWS + row) * 2]);
-    const float reference = top == -INFINITY ? 0.0f : top;
-    float total = 0.0f, sum[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-    for (int s = 0; s < splits; ++s) {
-        const int64_t at = (work * splits + s) * PA_ROWS + row;
-        const float2 entry = *reinterpret_cast<const float2*>(statistics + at * 2);
-        const float weight = pa_exp2(entry.x - reference);
-        if (entry.y == 0.0f) continue;      // no visible key in this split: O may not even have been written
-        total = __fmaf_rn(weight, entry.y, total);
-        const float4 a = *reinterpret_cast<const float4*>(partial + at * D + lane * 8), b = *reinterpret_cast<const float4*>(partial + at * D + lane * 8 + 4);
-        const float values[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    pdl_wait();
+    const int2 cut = *reinterpret_cast<const int2*>(args.cut);
+    const int64_t offset = args.row_offsets[index];          // inside the table, whatever the cut
+    const int64_t rows = int64_t(cut.x) * PA_ROWS;
+    const int splits = cut.y;
+    if (rows == 0) return;
+    const bool there = index < rows && offset >= 0;          // lanes without a row stay for the shuffles, on a row that is there
+    const int64_t row = index < rows ? index : 0;
+    const float2* statistics = reinterpret_cast<const float2*>(args.partial + int64_t(args.slots) * PA_ROWS * D) + row;
+    const float* partial = args.partial + row * D + lane * 8;
+    float2 entry[PER_LANE];          // of parts lane, lane + LANES, ..
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum[i] = __fmaf_rn(weight, values[i], sum[i]);
+    for (int i = 0; i < PER_LANE; ++i) {
+        const int s = lane + i * LANES;
+        entry[i] = there && s < splits ? statistics[s * rows] : make_float2(-INFINITY, 0.0f);
     }
+    float4 a[BATCH], b[BATCH];
+    auto load = [&](int first) {
+#pragma unroll
+        for (int n = 0; n < BATCH; ++n) {
+            a[n] = b[n] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (there && first + n < splits) {
+                a[n] = *reinterpret_cast<const float4*>(partial + (first + n) * rows * D);
+                b[n] = *reinterpret_cast<const float4*>(partial + (first + n) * rows * D + 4);
+            }
+        }
+    };
+    load(0);
+    float top = entry[0].x, total = 0.0f;
+#pragma unroll
+    for (int i = 1; i < PER_LANE; ++i) top = fmaxf(top, entry[i].x);
+#pragma unroll
+    for (int step = LANES / 2; step > 0; step >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, step));
+    const float reference = top == -INFINITY ? 0.0f : top;
+    float weight[PER_LANE];
+#pragma unroll
+    for (int i = 0; i < PER_LANE; ++i) {
+        weight[i] = entry[i].y == 0.0f ? 0.0f : pa_exp2(entry[i].x - reference);      // sum 0: no visible key in this part, O is 0
+        total = __fmaf_rn(weight[i], entry[i].y, total);
+    }
+#pragma unroll
+    for (int step = LANES / 2; step > 0; step >>= 1) total += __shfl_xor_sync(0xffffffffu, total, step);
+    float sum[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+    for (int first = 0; first < splits; first += BATCH) {
+        if (first > 0) load(first);
+#pragma unroll
+        for (int n = 0; n < BATCH; ++n) {
+            const int s = first + n;
+            float mine = weight[0];
+#pragma unroll
+            for (int i = 1; i < PER_LANE; ++i) mine = s / LANES == i ? weight[i] : mine;
+            const float w = __shfl_sync(0xffffffffu, mine, s % LANES, LANES);
+            const float values[8] = {a[n].x, a[n].y, a[n].z, a[n].w, b[n].x, b[n].y, b[n].z, b[n].w};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum[i] = __fmaf_rn(w, values[i], sum[i]);
+        }
+    }
+    if (!there) return;
     const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
-    *reinterpret_cast<uint4*>(out + offset + lane * 8) =
+    *reinterpret_cast<uint4*>(args.out + offset + lane * 8) =
         make_uint4(float2_to_bf16x2(make_float2(sum[0] * inverse, sum[1] * inverse)), float2_to_bf16x2(make_float2(sum[2] * inverse, sum[3] * inverse)),
                    float2_to_bf16x2(make_float2(sum[4] * inverse, sum[5] * inverse)), float2_to_bf16x2(make_float2(sum[6] * inverse, sum[7] * inverse)));
 }
 
 struct PaPlan {
-    int tiles = 0, splits = 1;
-    int64_t bytes = 0;          // of workspace
+    int64_t items = 0;          // row tiles times key/value heads, at most
+    int64_t ctas = 0;
+    int slots = 0, max_splits = 1;
+    int64_t bytes = 0;          // of workspace: the cut, row offsets, partial rows and their statistics
 };
 
 PaPlan pa_plan(const b2_prefix_attention_desc* d) {
@@ -1125,25 +1191,33 @@ PaPlan pa_plan(const b2_prefix_attention_desc* d) {
     const int64_t filled = d->groups < d->batch ? d->groups : d->batch;
     const int64_t tiles = d->members == nullptr ? d->groups * ((per_group * per_member + PA_ROWS - 1) / PA_ROWS)
                                                 : filled + (d->batch * per_member - filled) / PA_ROWS;
-    plan.tiles = int(tiles);
     // key tiles of a row tile: the prefix, and the own keys of the members that 128 rows can belong to
     int64_t sharing = (PA_ROWS + per_member - 2) / per_member + 1;
     if (d->members == nullptr && sharing > per_group) sharing = per_group;
     if (sharing > d->batch) sharing = d->batch;
     const int64_t key_tiles = (int64_t(d->prefix_capacity) + PA_KEYS - 1) / PA_KEYS + sharing * ((int64_t(d->own_capacity) + PA_KEYS - 1) / PA_KEYS);
-    const int64_t work = tiles * d->kv_heads;
-    const int64_t sms = sm_count();
-    int64_t best = 0;
-    for (int64_t splits = 1; splits <= 64 && splits <= key_tiles; ++splits) {
-        // In units of a key tile's time: waves of CTAs times (set-up + tiles), and the join's second launch and traffic.
-        const int64_t waves = (work * splits + sms - 1) / sms;
-        const int64_t cost = waves * (4 + (key_tiles + splits - 1) / splits) * 64 + (splits > 1 ? 5 * 64 + work * splits * 64 / 100 : 0);
+    plan.items = tiles * d->kv_heads;
+    const int64_t sms = sm_count(), uncut = plan.items > sms ? plan.items / sms * sms : 0, rest = plan.items - uncut;
+    // The cut of what is behind the last whole wave, in 1/32 of a key tile's time (0.6 to 0.9 us): waves of CTAs times (set-up + tiles) --
+    // looking up the work, fetching the queries and leaving the output take as long as 12 tiles -- and the join's launch and traffic.
+    int64_t best = 0, splits = 1;
+    for (int64_t s = 1; rest > 0 && s <= 64 && s <= key_tiles; ++s) {
+        const int64_t waves = (rest * s + sms - 1) / sms;
+        const int64_t cost = waves * (12 + (key_tiles + s - 1) / s) * 32 + (s > 1 ? 5 * 32 + rest * s : 0);
         if (best == 0 || cost < best) {
             best = cost;
-            plan.splits = int(splits);
+            splits = s;
         }
     }
-    if (plan.splits > 1) plan.bytes = work * PA_ROWS * (int64_t(plan.splits) * (d->head_dim + 2) * 4 + 8);
+    plan.ctas = plan.items;
+    if (splits > 1) {
+        // fewer row tiles than the bound are cut finer, to two key tiles at least
+        plan.slots = int(rest * splits);
+        plan.max_splits = int(splits > key_tiles / 2 ? splits : key_tiles / 2);
+        if (plan.max_splits > 64) plan.max_splits = 64;
+        plan.ctas = uncut + plan.slots;
+        plan.bytes = 32 + int64_t(plan.slots) * PA_ROWS * (4 + (d->head_dim + 2) * 4);
+    }
     return plan;
 }
 
@@ -1176,13 +1250,11 @@ int pa_launch(const b2_prefix_attention_desc* d, const PaPlan& plan, PaArgs& arg
         return B2_E_DRIVER;
     if (!has_prefix) prefix_k = own_k, prefix_v = own_v;
     if (!has_own) own_k = prefix_k, own_v = prefix_v;
-    const int64_t work = int64_t(plan.tiles) * d->kv_heads;
-    const int status = launch_kernel(prefix_attention_kernel<D, FP8>, dim3(unsigned(work * plan.splits)), dim3(Shape::THREADS),
-                                     size_t(Shape::SHARED_BYTES), stream, prefix_k, prefix_v, own_k, own_v, args);
-    if (status != B2_OK || plan.splits == 1) return status;
-    const int64_t rows = work * PA_ROWS;
-    return launch_kernel(prefix_attention_join_kernel<D>, dim3(unsigned((rows * (D / 8) + 255) / 256)), dim3(256), size_t(0), stream,
-                         static_cast<const float*>(args.partial), static_cast<const int64_t*>(args.row_offsets), args.out, rows, plan.splits);
+    const int status = launch_kernel(prefix_attention_kernel<D, FP8>, dim3(unsigned(plan.ctas)), dim3(Shape::THREADS), size_t(Shape::SHARED_BYTES), stream,
+                                     prefix_k, prefix_v, own_k, own_v, args);
+    if (status != B2_OK || plan.slots == 0) return status;
+    const int64_t rows = (plan.items < plan.slots / 2 ? plan.items : plan.slots / 2) * PA_ROWS;          // a row tile that is cut has two parts at least
+    return launch_kernel(prefix_attention_join_kernel<D>, dim3(unsigned((rows * (D / 8) + 255) / 256)), dim3(256), size_t(0), stream, args);
 }
 
 }  // namespace
@@ -1191,8 +1263,11 @@ int64_t prefix_attention_workspace(const b2_prefix_attention_desc* desc) { retur
 
 int launch_prefix_attention(const b2_prefix_attention_desc* desc, cudaStream_t stream) {
     PaPlan plan = pa_plan(desc);
-    if (plan.bytes > 0 && (desc->workspace == nullptr || desc->workspace_bytes < plan.bytes)) plan.splits = 1;
-    if (int64_t(plan.tiles) * desc->kv_heads * plan.splits * PA_ROWS >= (int64_t(1) << 31)) return B2_E_TOO_LARGE;
+    if (plan.bytes > 0 && (desc->workspace == nullptr || desc->workspace_bytes < plan.bytes)) {
+        plan.slots = 0;          // nothing is cut
+        plan.ctas = plan.items;
+    }
+    if (plan.ctas * PA_ROWS >= (int64_t(1) << 31)) return B2_E_TOO_LARGE;
     PaArgs args{};
     args.q = static_cast<const __nv_bfloat16*>(desc->q);
     args.out = static_cast<__nv_bfloat16*>(desc->out);
@@ -1203,10 +1278,11 @@ int launch_prefix_attention(const b2_prefix_attention_desc* desc, cudaStream_t s
     args.members = static_cast<const int32_t*>(desc->members);
     args.prefix_lengths = static_cast<const int32_t*>(desc->prefix_lengths);
     args.own_lengths = static_cast<const int32_t*>(desc->own_lengths);
-    if (plan.splits > 1) {
-        const int64_t rows = int64_t(plan.tiles) * desc->kv_heads * PA_ROWS;
-        args.row_offsets = static_cast<int64_t*>(desc->workspace);
-        args.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(desc->workspace) + rows * 8);
+    if (plan.slots > 0) {
+        uint8_t* const workspace = static_cast<uint8_t*>(desc->workspace);
+        args.cut = reinterpret_cast<int32_t*>(workspace);
+        args.row_offsets = reinterpret_cast<int64_t*>(workspace + 32);
+        args.partial = reinterpret_cast<float*>(workspace + 32 + int64_t(plan.slots) * PA_ROWS * 4);
     }
     args.status = static_cast<unsigned int*>(desc->status);
     for (int i = 0; i < 3; ++i) args.q_stride[i] = desc->q_stride[i];
@@ -1219,8 +1295,9 @@ int launch_prefix_attention(const b2_prefix_attention_desc* desc, cudaStream_t s
     args.prefix_capacity = desc->prefix_capacity;
     args.own_capacity = desc->own_capacity;
     args.rows_per_member = desc->heads / desc->kv_heads * desc->queries;
-    args.tiles = plan.tiles;
-    args.splits = plan.splits;
+    args.sms = sm_count();
+    args.slots = plan.slots;
+    args.max_splits = plan.slots > 0 ? plan.max_splits : 1;
     args.causal = (desc->flags & B2_ATTENTION_CAUSAL) != 0;
     if (desc->head_dim == 256)
         return desc->cache_bits == 8 ? pa_launch<256, true>(desc, plan, args, stream) : pa_launch<256, false>(desc, plan, args, stream);

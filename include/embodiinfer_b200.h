@@ -308,9 +308,9 @@ int b2_kv_cache_read(const b2_kv_cache_desc* desc, void* stream);
  * do such own values (a whole output row) and quantised values; bf16 prefix values that are not finite follow IEEE arithmetic.
  * Scores, softmax statistics and outputs are held in fp32; probabilities enter the second product as bf16 (bf16 cache) or f16
  * (quantised cache; there q enters the first as two e4m3 halves that hold its 8 bits).  head_dim 128 or 256.
- * `workspace`: NULL, or 32-byte aligned device scratch; with b2_prefix_attention_workspace_bytes(desc) bytes a launch of few row
- * tiles cuts their keys across the SMs and joins the parts in a fixed order.  It needs no zeroing and holds nothing between
- * calls, but two calls that may run at the same time need one each.  `status` as in b2_linear_desc.
+ * `workspace`: NULL, or 32-byte aligned device scratch; with b2_prefix_attention_workspace_bytes(desc) bytes the 128-row tiles that
+ * do not fill the device (a small call's, or those of the last partial wave) have their keys cut across the SMs and the parts joined
+ * in a fixed order.  It needs no zeroing and holds nothing between calls, but two calls that may run at the same time need one each.  `status` as in b2_linear_desc.
  * Widens b2_attention (one copy of the keys per batch element, head_dim 256, one key/value head, no lengths); the reference
  * attends per sample (embodiinfer/backend/torch/attention.py:97-106). */
 #define B2_ATTENTION_CAUSAL 1

@@ -163,6 +163,19 @@ def test_cut_and_uncut_launches_agree(device, monkeypatch, dim, quantised):
     assert not torch.equal(cut, uncut)          # another order of the sums: both within their bounds
 
 
+@pytest.mark.parametrize("quantised", [False, True])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 1, 256), (16, 2, 128)])
+def test_the_last_wave_is_cut(device, monkeypatch, heads, kv_heads, dim, quantised):
+    """Some more row tiles than SMs, fewer than the bound that the launch is sized by: the ones behind the first wave are cut."""
+    counts = [12 if g % 2 else 4 for g in range(32 // kv_heads)]
+    bounds = [sum(counts[:g]) for g in range(len(counts) + 1)]
+    lengths = [2000 - (137 * g) % 900 for g in range(len(counts))], [10 - b % 9 for b in range(bounds[-1])]
+    cut = run_case(device, bounds, heads, kv_heads, 10, dim, 2000, 10, False, quantised, *lengths)
+    monkeypatch.setattr(N.load(), "b2_prefix_attention_workspace_bytes", lambda desc: 0)
+    uncut = run_case(device, bounds, heads, kv_heads, 10, dim, 2000, 10, False, quantised, *lengths)
+    assert (cut == uncut).flatten(1).all(1).sum() >= bounds[-1] // 2 and not torch.equal(cut, uncut)          # most are in the whole wave
+
+
 def test_without_a_prefix(device):
     generator = torch.Generator(device=device).manual_seed(5)
     q = torch.randn((3, 8, 4, 128), device=device, generator=generator).to(torch.bfloat16)

@@ -82,10 +82,10 @@ def test_prefix_attention_refuses(changes, code):
 def test_prefix_attention_workspace():
     size = N.load().b2_prefix_attention_workspace_bytes
     assert size(None) == 0 and size(ctypes.byref(_attention_desc(head_dim=64))) == 0
-    few = size(ctypes.byref(_attention_desc(prefix_capacity=32768)))            # two row tiles, 512 key tiles
-    rows = 2 * 128                                                              # two groups of 2 x 80 rows: four row tiles of 128
-    assert few > 0 and few % (2 * rows) == 0
-    assert size(ctypes.byref(_attention_desc(batch=4096, groups=2))) == 0       # row tiles for every SM: nothing to cut
+    few = size(ctypes.byref(_attention_desc(prefix_capacity=32768)))            # two groups of 2 x 80 rows, four row tiles; 512 key tiles
+    part = 128 * (256 * 4 + 2 * 4 + 4)                                          # of one CTA: fp32 rows, their statistics, half of the row offsets
+    assert few >= 32 + 8 * part and (few - 32) % part == 0
+    assert size(ctypes.byref(_attention_desc(batch=4096, groups=2))) == 0       # row tiles for many waves: nothing to cut
 
 
 @pytest.mark.parametrize("arguments,code", [
