@@ -561,9 +561,10 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
                     load(chunk, words);
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
-                        // of the 8 significant bits hi takes the upper 4 and lo the lower: both exact above e4m3's smallest step
+                        // of the 8 significant bits hi takes the upper 4 and lo the lower; below 2^-6, where e4m3 has fewer, lo takes all
                         const __nv_bfloat162 x = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&words[i]), up2);
-                        const uint32_t upper = *reinterpret_cast<const uint32_t*>(&x) & 0xfff0fff0u;
+                        const uint32_t small = __hlt2_mask(__habs2(x), __float2bfloat162_rn(0.015625f));
+                        const uint32_t upper = *reinterpret_cast<const uint32_t*>(&x) & 0xfff0fff0u & ~small;
                         const __nv_bfloat162 rest = __hsub2(x, *reinterpret_cast<const __nv_bfloat162*>(&upper));
                         const uint32_t h = __nv_cvt_float2_to_fp8x2(bf16x2_to_float2(upper), __NV_SATFINITE, __NV_E4M3);
                         const uint32_t l = __nv_cvt_float2_to_fp8x2(bf16x2_to_float2(*reinterpret_cast<const uint32_t*>(&rest)), __NV_SATFINITE, __NV_E4M3);

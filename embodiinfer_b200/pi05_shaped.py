@@ -32,6 +32,7 @@ from .backend.norm_quant import B200NormQuant
 from .backend.projection import B200Projection
 from .backend.quantization import B200Quantizer
 from .bundles import pack_quantized_linears, quantize_linear
+from .kv_cache import QuantizedKVCache
 from .layers.linear import FP8Config, NVFP4Config, parse_quantization_config
 
 
@@ -352,22 +353,29 @@ class GemmaBlock(nn.Module):
             self.mlp_ranges[1] = max(self.mlp_ranges[1], float(hidden.abs().max()))
         return x, (self.down(hidden), gate)
 
-    def forward(self, x, rope, kv_buffers=None, modulations=None, pending=None):
+    def forward(self, x, rope, kv_buffers=None, modulations=None, pending=None, shared=None):
         """``kv_buffers`` (action expert): per-layer [B, 1, prefix + T, D] key/value buffers whose first
         ``prefix`` rows hold the prefix tower's keys/values; this block writes its own rows behind them.
         Adaptive blocks take ``modulations`` = (input norm's, post-attention norm's) fp32 [B, 3 width] and ``pending`` =
-        (MLP output, gate) of the block before, and return (residual stream, own keys/values, pending)."""
+        (MLP output, gate) of the block before, and return (residual stream, own keys/values, pending).
+        ``shared`` (action samples behind one prefix) = (prefix, own) caches, each a bf16 pair or a ``QuantizedKVCache``: the
+        prefix holds one entry for every B / G batch elements, and this block's rows go into ``own``."""
         shape = self.shape
         batch, tokens, _ = x.shape
         attention_gate = None
         q = torch.empty((batch, shape.heads, tokens, shape.head_dim), device=x.device, dtype=x.dtype)
-        if kv_buffers is None:
+        quantised = shared is not None and isinstance(shared[1], QuantizedKVCache)
+        if quantised:
+            k = v = None
+        elif shared is not None:
+            k, v = shared[1]
+        elif kv_buffers is None:
             k = torch.empty((batch, shape.kv_heads, tokens, shape.head_dim), device=x.device, dtype=x.dtype)
             v = torch.empty_like(k)
         else:
             k, v = kv_buffers
         preparation = dict(sine=rope[0], cosine=rope[1], q_out=q, k_out=k, v_out=v, batch=batch, tokens=tokens, heads=shape.heads,
-                           kv_heads=shape.kv_heads, head_dim=shape.head_dim, kv_offset=k.shape[2] - tokens)
+                           kv_heads=shape.kv_heads, head_dim=shape.head_dim, kv_offset=0 if quantised else k.shape[2] - tokens)
         qkv = None
         if self.adaptive:
             if self.qkv.norm is not None and self.fused_norm:
@@ -375,7 +383,7 @@ class GemmaBlock(nn.Module):
                 # A packed FP8 QKV projection of a handful of rows: the attention preparation is the launch's epilogue
                 # (b2_linear_desc.rope) -- measured faster than projection + b2_rope_split up to ~96 rows.
                 if (self.rope_in_projection and self.qkv.plan.precision == "fp8" and self.qkv.dense_bias is None
-                        and shape.head_dim == 256 and batch * tokens <= 96):
+                        and shape.head_dim == 256 and batch * tokens <= 96 and not quantised):
                     self.qkv.plan.apply(x.reshape(-1, x.shape[-1]), encoded, rope=preparation)
                 else:
                     qkv = self.qkv.plan.apply(x.reshape(-1, x.shape[-1]), encoded, bias=self.qkv.dense_bias).reshape(batch, tokens, -1)
@@ -388,7 +396,12 @@ class GemmaBlock(nn.Module):
         else:
             qkv = self.qkv(_rms_norm(x, self.input_scale))
         q_dim = shape.heads * shape.head_dim
-        if qkv is not None:
+        if quantised:
+            # one launch: split, rotate q and k, [B, heads, T, D] queries, keys / values quantised into the cache
+            rows = qkv.view(batch, tokens, -1, shape.head_dim).transpose(1, 2)
+            first, last = shape.heads, shape.heads + shape.kv_heads
+            K.kv_cache_write(rows[:, first:last], rows[:, last:], shared[1], q=rows[:, :first], q_out=q, sine=rope[0], cosine=rope[1])
+        elif qkv is not None:
             # one launch: split, rotate q and k, [B, heads, T, D] queries, keys / values written into the buffers
             K.rope_split(qkv.reshape(batch * tokens, -1), **preparation)
         own_kv = (k, v)
@@ -403,7 +416,9 @@ class GemmaBlock(nn.Module):
         # b2_attention_nvfp4): one launch less.  The NVFP4 encoding is some 150 instructions per 16 values on the four
         # epilogue warps of a CTA, which only pays on the latency chain of a small launch (B = 1 / 8: 7.27 -> 7.16 and
         # 9.45 -> 9.28 ms per chunk); the 560-token prefix (2.20 -> 2.40 ms per stack) and B = 64 keep the encoder launch.
-        if native and output_encoder is not None and self.encode_in_attention and (output_encoder.bits == 8 or batch * tokens <= 128):
+        if shared is not None:
+            attended = K.prefix_attention(q, *shared)          # each prefix once for all its samples
+        elif native and output_encoder is not None and self.encode_in_attention and (output_encoder.bits == 8 or batch * tokens <= 128):
             encoded, attended = output_encoder.plan_for(q), None
             if output_encoder.bits == 8:
                 K.attention(q, k, v, codes=encoded.output, multiplier=output_encoder.scale_value)
@@ -598,15 +613,44 @@ class Pi05ShapedPolicy(nn.Module):
             pad = keys.new_zeros((*keys.shape[:2], ACTION_HORIZON, keys.shape[-1]))
             buffers.append((torch.cat((keys, pad), dim=2), torch.cat((values, pad), dim=2)))
         for step in range(DENOISE_STEPS):
-            modulations = schedule[step]
-            x = F.linear(actions.to(torch.bfloat16), self.action_in)
-            pending = None
-            for index, (block, kv) in enumerate(zip(self.expert, buffers)):
-                x, _, pending = block(x, rope, kv_buffers=kv, modulations=modulations[2 * index: 2 * index + 2], pending=pending)
-            final, _ = _ada_rms_norm(_gated_residual(x, pending), modulations[-1])
-            velocity = F.linear(final, self.action_out).float()
-            actions = actions + dt * velocity              # Euler step of the flow (flow.py:21-23)
+            actions = actions + dt * self._velocity(actions, rope, schedule[step], [dict(kv_buffers=kv) for kv in buffers])
         return actions
+
+    def _velocity(self, actions: torch.Tensor, rope, modulations, caches: list[dict]) -> torch.Tensor:
+        """The expert's flow velocity at ``actions`` [B, 10, 32]; ``caches`` is each block's ``kv_buffers`` or ``shared``."""
+        x = F.linear(actions.to(torch.bfloat16), self.action_in)
+        pending = None
+        for index, (block, cache) in enumerate(zip(self.expert, caches)):
+            x, _, pending = block(x, rope, modulations=modulations[2 * index: 2 * index + 2], pending=pending, **cache)
+        final, _ = _ada_rms_norm(_gated_residual(x, pending), modulations[-1])
+        return F.linear(final, self.action_out).float()
+
+    def denoise_samples(self, cache, prefix_length: int, noise: torch.Tensor, *, quantised_cache: bool = False) -> torch.Tensor:
+        """Several action chunks of every observation: ``noise`` [B, N, 10, 32] fp32, one starting point per sample, to
+        [B, N, 10, 32].  ``cache`` is ``encode_prefix``'s for the B observations: the N samples of an observation read its one
+        prefix (``b2_prefix_attention``), where ``denoise`` would need it N times.  ``quantised_cache`` holds the prefixes'
+        and the samples' keys and values as e4m3 codes with a scale for each row (``b2_kv_cache_write``)."""
+        batch, samples = noise.shape[:2]
+        count, device, head_dim = batch * samples, self.device_, GEMMA_300M.head_dim
+        actions = noise.reshape(count, ACTION_HORIZON, ACTION_DIM)
+        if count == 0:
+            return noise.clone()
+        positions = prefix_length + torch.arange(ACTION_HORIZON, device=device)
+        rope = K.rope_axes(positions[None], (head_dim // 2,))
+        schedule = self.modulation_schedule(count)
+        caches = []
+        for keys, values in cache[: len(self.expert)]:
+            own_shape = (count, GEMMA_300M.kv_heads, ACTION_HORIZON, head_dim)
+            if quantised_cache:
+                prefix = QuantizedKVCache.allocate(*keys.shape, device)
+                K.kv_cache_write(keys, values, prefix)
+                own = QuantizedKVCache.allocate(*own_shape, device)
+            else:
+                prefix, own = (keys, values), tuple(keys.new_empty(own_shape) for _ in range(2))
+            caches.append(dict(shared=(prefix, own)))
+        for step in range(DENOISE_STEPS):
+            actions = actions - self._velocity(actions, rope, schedule[step], caches) / DENOISE_STEPS
+        return actions.view(noise.shape)
 
     def noise(self, batch: int) -> torch.Tensor:
         generator = torch.Generator(device=self.device_).manual_seed(self.noise_seed)
@@ -617,6 +661,16 @@ class Pi05ShapedPolicy(nn.Module):
         images, tokens = observations["images"], observations["tokens"]
         cache, prefix_length = self.encode_prefix(images, tokens)
         return self.denoise(cache, prefix_length, self.noise(images.shape[0]) if noise is None else noise)
+
+    @torch.no_grad()
+    def sample(self, observations: dict, samples: int, noise: torch.Tensor | None = None, *, quantised_cache: bool = False) -> torch.Tensor:
+        """``samples`` action chunks [B, samples, 10, 32] of every observation, for a caller that chooses among them: the vision
+        and prefix towers run once per observation, and the samples share the prefix's keys and values."""
+        images, tokens = observations["images"], observations["tokens"]
+        cache, prefix_length = self.encode_prefix(images, tokens)
+        if noise is None:
+            noise = self.noise(images.shape[0] * samples).view(images.shape[0], samples, ACTION_HORIZON, ACTION_DIM)
+        return self.denoise_samples(cache, prefix_length, noise, quantised_cache=quantised_cache)
 
     @torch.no_grad()
     def calibrate_fused_mlp(self, observations: dict, margin: float = 1.0) -> None:

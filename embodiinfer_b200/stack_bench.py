@@ -5,7 +5,8 @@
 * prefix stack: 18 Gemma-2B-shaped layers over 560 prefix tokens (one observation), random-init weights,
   input ~N(0, 1) bf16;
 * action-expert denoise: 18 Gemma-300M-shaped layers over a 10-token action chunk, 10 Euler steps,
-  batch B, attending to random prefix keys/values [B, 1, 560, 256] per layer.
+  batch B, attending to random prefix keys/values [B, 1, 560, 256] per layer;
+* the same denoise for several samples of each observation, over one copy of the prefix per observation.
 
 Each measurement is one CUDA graph replayed 20 times between CUDA events (after 3 warm-up replays); the
 MLPs run as the calibrated fused plan unless ``--registry-route`` is given.  One JSON line per case.
@@ -70,6 +71,21 @@ def measure_denoise(policy: Pi05ShapedPolicy, batches=(1, 8, 64), seed: int = 10
 
 
 @torch.no_grad()
+def measure_samples(policy: Pi05ShapedPolicy, observations: int = 8, samples: int = 8, seed: int = 1006) -> dict[str, float]:
+    """Milliseconds of the 10-step denoise of ``samples`` action chunks for each of ``observations`` prefixes of 560 tokens: over
+    one copy of the prefix per observation (bf16 and quantised caches), and over one copy per sample."""
+    device = policy.device_
+    generator = torch.Generator(device=device).manual_seed(seed)
+    cache = [tuple(torch.randn((observations, 1, PREFIX_TOKENS, GEMMA_300M.head_dim), device=device, generator=generator).to(torch.bfloat16)
+                   for _ in range(2)) for _ in policy.expert]
+    noise = torch.randn((observations, samples, ACTION_HORIZON, ACTION_DIM), device=device, generator=generator)
+    repeated = [tuple(part.repeat_interleave(samples, 0) for part in pair) for pair in cache]
+    return {"shared": graph_milliseconds(lambda: policy.denoise_samples(cache, PREFIX_TOKENS, noise)),
+            "shared_quantised": graph_milliseconds(lambda: policy.denoise_samples(cache, PREFIX_TOKENS, noise, quantised_cache=True)),
+            "a_copy_per_sample": graph_milliseconds(lambda: policy.denoise(repeated, PREFIX_TOKENS, noise.flatten(0, 1)))}
+
+
+@torch.no_grad()
 def main() -> None:
     parser = argparse.ArgumentParser()
     parser.add_argument("--quantization", default="fp8")
@@ -109,6 +125,11 @@ def main() -> None:
         print(json.dumps({"case": f"expert_denoise_10_steps_B{batch}", "ms": round(milliseconds, 4),
                           "ms_per_step": round(milliseconds / 10, 4),
                           "quantised_linear_tflops": round(flops / milliseconds / 1e9, 2), **common}), flush=True)
+
+    for observations, samples in ((1, 8), (8, 8)):
+        found = measure_samples(policy, observations, samples)
+        print(json.dumps({"case": f"expert_denoise_10_steps_{samples}_samples_of_{observations}",
+                          **{f"ms_{key}": round(value, 4) for key, value in found.items()}, **common}), flush=True)
 
 
 if __name__ == "__main__":
