@@ -358,12 +358,28 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
             return n < 0 ? 0 : n;
         };
         auto row_tiles = [&](int n) { return (n * args.rows_per_member + PA_ROWS - 1) / PA_ROWS; };
+        auto inclusive_sum = [&](int sum) {
+#pragma unroll
+            for (int step = 1; step < 32; step <<= 1) {
+                const int other = __shfl_up_sync(0xffffffffu, sum, step);
+                if (lane >= step) sum += other;
+            }
+            return sum;
+        };
         constexpr int MANY = 1 << 29;          // bounds that run backwards may add up to anything: enough for every CTA
         int total_tiles = 0;
+        int batch_first = 0, batch_count = 0, batch_sum = 0;          // of 32 groups, one per lane: the first 32, until they have to be passed
+        auto load_groups = [&](int g0) {
+            batch_first = batch_count = 0;
+            if (g0 + lane < args.groups) batch_count = group_members(g0 + lane, batch_first);
+            batch_sum = inclusive_sum(row_tiles(batch_count));
+        };
         if (args.members == nullptr) {
             total_tiles = args.groups * row_tiles(args.batch / args.groups);
         } else {
-            for (int g0 = 0; g0 < args.groups && total_tiles < MANY; g0 += 32) {
+            load_groups(0);
+            total_tiles = __shfl_sync(0xffffffffu, batch_sum, 31);
+            for (int g0 = 32; g0 < args.groups && total_tiles < MANY; g0 += 32) {
                 int a;
                 total_tiles += __reduce_add_sync(0xffffffffu, g0 + lane < args.groups ? row_tiles(group_members(g0 + lane, a)) : 0);
             }
@@ -395,24 +411,17 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
         } else {
             int before = 0;
             for (int g0 = 0; g0 < args.groups && group < 0 && before < MANY; g0 += 32) {
-                const int g = g0 + lane;
-                int a = 0;
-                const int n = g < args.groups ? group_members(g, a) : 0, mine = row_tiles(n);
-                int sum = mine;
-#pragma unroll
-                for (int step = 1; step < 32; step <<= 1) {
-                    const int other = __shfl_up_sync(0xffffffffu, sum, step);
-                    if (lane >= step) sum += other;
-                }
-                const unsigned hit = __ballot_sync(0xffffffffu, mine > 0 && tile >= before + sum - mine && tile < before + sum);
+                if (g0 > 0) load_groups(g0);
+                const int mine = row_tiles(batch_count), start = before + batch_sum - mine;
+                const unsigned hit = __ballot_sync(0xffffffffu, mine > 0 && tile >= start && tile < start + mine);
                 if (hit != 0u) {
                     const int source = __ffs(int(hit)) - 1;
                     group = g0 + source;
-                    first = __shfl_sync(0xffffffffu, a, source);
-                    count = __shfl_sync(0xffffffffu, n, source);
-                    group_tile = tile - before - __shfl_sync(0xffffffffu, sum - mine, source);
+                    first = __shfl_sync(0xffffffffu, batch_first, source);
+                    count = __shfl_sync(0xffffffffu, batch_count, source);
+                    group_tile = tile - __shfl_sync(0xffffffffu, start, source);
                 }
-                before += __shfl_sync(0xffffffffu, sum, 31);
+                before += __shfl_sync(0xffffffffu, batch_sum, 31);
             }
         }
         const int row0 = group_tile * PA_ROWS;
@@ -1204,7 +1213,7 @@ PaPlan pa_plan(const b2_prefix_attention_desc* d) {
     int64_t best = 0, splits = 1;
     for (int64_t s = 1; rest > 0 && s <= 64 && s <= key_tiles; ++s) {
         const int64_t waves = (rest * s + sms - 1) / sms;
-        const int64_t cost = waves * (12 + (key_tiles + s - 1) / s) * 32 + (s > 1 ? 5 * 32 + rest * s : 0);
+        const int64_t cost = waves * (12 + (key_tiles + s - 1) / s) * 32 + (s > 1 ? 5 * 32 + 3 * rest * s : 0);
         if (best == 0 || cost < best) {
             best = cost;
             splits = s;
