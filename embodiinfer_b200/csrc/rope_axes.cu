@@ -132,7 +132,7 @@ int launch_rope_axes(const void* positions, int position_bytes, const int32_t* s
     const int columns_per_row = columns < AXES_THREADS ? columns : AXES_THREADS;
     const int rows_per_block = AXES_THREADS / columns_per_row;
     const unsigned planes = unsigned((columns + columns_per_row - 1) / columns_per_row);
-    const int64_t wanted = (tokens + rows_per_block - 1) / rows_per_block, cap = int64_t(sm_count()) * 8;
+    const int64_t wanted = (tokens + rows_per_block - 1) / rows_per_block, cap = int64_t(sm_count()) * 5;      // what the registers let run at once
     const int64_t blocks = wanted < cap ? wanted : cap;
     const dim3 grid(unsigned(blocks), planes), block(AXES_THREADS);
     const int64_t step = blocks * rows_per_block;
