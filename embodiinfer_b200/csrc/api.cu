@@ -246,6 +246,9 @@ int b2_kv_cache_read(const b2_kv_cache_desc* desc, void* stream) {
     const int status = check_kv_cache(desc);
     if (status != B2_OK) return status;
     if (desc->q != nullptr || desc->q_out != nullptr || desc->sine != nullptr || desc->cosine != nullptr) return B2_E_INVALID;
+    const int32_t extents[3] = {desc->batch, desc->kv_heads, desc->tokens};
+    for (int i = 0; i < 3; ++i)          // rows that lie on one another cannot be written
+        if (extents[i] > 1 && (desc->k_stride[i] < desc->head_dim || desc->v_stride[i] < desc->head_dim)) return B2_E_INVALID;
     return b2::launch_kv_cache_read(desc, static_cast<cudaStream_t>(stream));
 }
 

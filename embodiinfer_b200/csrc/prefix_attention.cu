@@ -8,17 +8,27 @@
 // a CTA takes 128 of them and walks the prefix in tiles of 64 keys -- every key tile is loaded once for all 128 rows -- and then
 // the own keys of the members its rows belong to, where the rows of the other members are masked.  The own part so spends tensor
 // instructions on masked rows; it stays below the time of loading those keys, which nobody else needs.
-//   warp 0        TMA producer: key and value tiles through rings
-//   warp 1        tensor-memory owner and MMA issuer: S = Q K^T (128 x 64) and O += P V (128 x D), fp32 accumulators in tensor memory
-//   warps 2-9     two softmax groups of 128 threads, one thread per row, for the even and the odd key tiles: scores, reference and
-//                 sum, probabilities, output
-//   warps 10..    what the value tile still needs before the tensor core may read it (see below)
-// What bounds such a loop is shared memory: 128 bytes per cycle have to take the tiles from TMA and give them to the tensor core,
-// and with Q and P there as well (128 rows of 32 bytes again for every 64 keys) they cost more than K and V themselves.  So Q lives
-// in tensor memory as the first product's "A" operand, and P as the second one's:
-// S of the even and odd tiles 2 x 64 columns, O D columns, Q and P the rest (D = 256: a quarter of Q stays in shared memory).
-// The two softmax groups work a tile apart and pass one float per row: the running reference, which a group needs from the
-// other only after it has the maximum of its own tile.  Every wait is bounded and reports through the status word.
+//   warps 0-7     two softmax groups of 128 threads, one thread per row, for the even and the odd key tiles: queries into tensor memory,
+//                 scores, reference and sum, probabilities, output
+//   warp 8        which rows and keys; TMA producer: key and value tiles through rings
+//   warps 9, 10   issuers of S = Q K^T (128 x 64) and of O += P V (128 x D), fp32 accumulators in tensor memory
+//   warp 11       the scales of a quantised cache
+//   warps 12-15   what the value tile still needs before the tensor core may read it (see below)
+// Shared memory has 128 bytes per cycle to take the tiles from TMA and give them to the tensor core; with Q and P there as well (128
+// rows of 32 bytes again for every 64 keys) they would cost more than K and V themselves.  So Q lives in tensor memory as the first
+// product's "A" operand, and P as the second one's.  D = 128: S of the even and odd tiles 2 x 64 columns, an accumulator for each
+// group 2 x 128, Q 64, P 2 x 32: the groups meet at the end only.  D = 256: S 2 x 64, one accumulator 256, three quarters of Q 96 (the
+// last one in shared memory), one P 32: the groups work a tile apart and pass one float per row, the running reference, which a group
+// needs from the other only after it has the maximum of its own tile.  Every wait is bounded and reports through the status word.
+//
+// Measured (B200; a tile is 64 keys for 128 rows, whose products alone are 500 cycles at D = 128 and 1000 at D = 256):
+//   fifty-query chunks of 64 members over 4 x 8192 bf16 keys, D = 256: 187 us (1150 TFLOP/s), 1430 cycles per tile
+//   64 members, one query, 32768 quantised keys, D = 128: 81 us, 1400 cycles per tile; without its exponentials 74, without its
+//   products 78, without the conversion of values 74: the chain of a softmax group -- scores out, maximum, exponentials, P in, each with
+//   its latency and two warps per scheduler to hide it -- and not one unit is what bounds the loop
+//   256 ten-query chunks over 32 x 712 quantised keys, D = 256: 45 us: 176 row tiles of 12 key tiles on 148 SMs, 21 k of a CTA's 41 k
+//   cycles before and behind the loop (4.9 k look-up, 3.6 k splitting Q, 5 k output)
+//   four ten-query chunks over 560 bf16 keys, D = 256: 14.0 us, 9 in this kernel for one tile per CTA, the rest the join
 //
 // bf16 cache.  K and V are read as they lie in memory.  What the tensor core must not see is taken out of the value tile in
 // shared memory, because a probability of zero times an infinity or a NaN is not zero: rows behind the end of a segment are set to
@@ -28,14 +38,15 @@
 // Quantised cache (e4m3 codes, one fp32 scale per row: ks for keys, vs for values).
 //   Scores.  The codes go to the tensor core as they are (kind::f8f6f4).  Q is split into two e4m3 operands, q 2^e = hi + lo with
 //   2^e bringing the row's largest value into [128, 256): a bf16 value has 8 significant bits, hi takes 4 and lo the rest,
-//   exactly, down to 2^-18 of the row's largest value.  Two products at twice the bf16 rate cost what one bf16 product
+//   exactly, down to 2^-17 of the row's largest value.  Two products at twice the bf16 rate cost what one bf16 product
 //   would, and no key is ever converted.  ks multiplies the score.
-//   Output.  The four value warps turn the codes into f16, exactly, and multiply by vs 2^-E: one rounding of 2^-11 for the scale and one for the product, beside the 2^-9 of the result.  2^E is the unit
-//   of the accumulator, the same for all rows: it follows the largest vs of a key tile when that leaves [2^-10, 2^6) units, and
-//   the accumulator is rescaled then as it is for a new reference.  A value keeps its precision as long as its scale is within
-//   2^-20 of the largest in its tile of 64 keys, whatever the scales of other tiles are.  P is f16 as well: with its 11 bits the
-//   result is as exact as its own rounding allows (bf16 probabilities would add as much error again; two e4m3 halves, which
-//   would spare the conversion of V, have no room for a long tail of weights 2^-15 below the largest).
+//   Output.  The four value warps turn the codes into f16, exactly, and multiply by vs 2^-E: one rounding of 2^-11 for the scale and
+//   one for the product, beside the 2^-8 of the result.  2^E is the unit of the accumulator, the same for all rows: it follows the
+//   largest vs of a key tile when that leaves [2^-3, 2^6) units, and the accumulator is rescaled then as it is for a new reference.
+//   A value is so off by at most 2^-10 of itself and, f16 ending at 2^-24 units, 2^-22 of the largest in its tile of 64 keys, whatever
+//   other tiles hold.  P is f16 as well: with its 11 bits the result is as exact as its own rounding allows (bf16 probabilities would
+//   add as much error again; two e4m3 halves, which would spare the conversion of V, have no room for a long tail of weights 2^-15
+//   below the largest).
 //   A scale that is not finite zeroes its row of values and marks the key: rows that see it get NaN from their sum.
 //
 // Row tiles that do not fill the device -- all of a small call's, or those of the last, partial wave -- have their key tiles cut across
@@ -56,8 +67,8 @@ namespace {
 constexpr int PA_ROWS = 128;                     // query rows per CTA
 constexpr int PA_KEYS = 64;                      // keys per tile
 constexpr int PA_LOAD_WARP = 8, PA_SCORES_WARP = 9, PA_OUTPUT_WARP = 10, PA_SCALE_WARP = 11, PA_VALUE_WARP = 12, PA_WARPS = 16;      // 0-7: softmax
-// Registers per thread: 128 at launch (512 threads); the softmax warpgroups take what the others give up.
-constexpr int PA_SOFTMAX_REGISTERS = 168, PA_OTHER_REGISTERS = 88;
+// Registers per thread: 128 at launch (512 threads); the softmax warpgroups take what the others give up (168 / 88: 84 us for the 32768 keys).
+constexpr int PA_SOFTMAX_REGISTERS = 184, PA_OTHER_REGISTERS = 72;
 static_assert(256 * PA_SOFTMAX_REGISTERS + (PA_WARPS * 32 - 256) * PA_OTHER_REGISTERS <= PA_WARPS * 32 * 128, "registers of the launch");
 constexpr uint32_t PA_PATIENCE = 1400000000u;     // cycles of a wait
 constexpr int PA_SCALE_STAGES = 4, PA_RAW_STAGES = 8;      // of the quantised cache's scales: as the softmax reads them; as they come
@@ -1070,10 +1081,10 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
                     else largest = max(largest, bits);
                 }
                 largest = __reduce_max_sync(0xffffffffu, largest);
-                // the unit 2^E: kept unless the tile's largest scale is outside [2^-10, 2^6) of it (a tile of zeros fits any)
+                // the unit 2^E: kept unless the tile's largest scale is outside [2^-3, 2^6) of it (a tile of zeros fits any)
                 const int exponent = int(largest >> 23) - 127, relative = exponent - unit_exponent;
                 int change = 0;
-                if (largest != 0u && (j == 0 || relative > 5 || relative < -10)) {
+                if (largest != 0u && (j == 0 || relative > 5 || relative < -3)) {
                     int next = exponent < -60 ? -60 : (exponent > 60 ? 60 : exponent);
                     if (j > 0) {
                         next = next < unit_exponent - 60 ? unit_exponent - 60 : next;          // the accumulator grows by the step

@@ -421,7 +421,8 @@ def prefix_attention(q: torch.Tensor, prefix, own=None, *, members: torch.Tensor
     or a :class:`QuantizedKVCache`, both of one kind.  ``members`` int32 [G + 1]: group g is the batch elements
     [members[g], members[g + 1]); default B / G each.  ``prefix_lengths`` int32 [G], ``own_lengths`` int32 [B]: default the
     capacities.  ``causal``: query t sees all but the last T - 1 - t own keys.  ``scale`` defaults to 1 / sqrt(D).  Returns bf16
-    [B, H, T, D]; rows that see no key are zero.  See ``b2_prefix_attention``."""
+    [B, H, T, D]; rows that see no key are zero, batch elements outside every group are left as ``out`` had them.  See
+    ``b2_prefix_attention``."""
     if prefix is None:
         raise ValueError("prefix_attention requires a prefix cache (its capacity may be 0)")
     device = _require_cuda(q, *prefix, *(own or ()), members, prefix_lengths, own_lengths, out, status)

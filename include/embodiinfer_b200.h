@@ -269,8 +269,8 @@ int b2_rope_axes(const void* positions, int32_t position_bytes, const int32_t* s
  * scale and codes are 0 when max|x| < 2^-50, and the scale is NaN (the whole row reads back as NaN) when max|x| >= 2^40 or a value
  * is not finite.
  * Two tokens of one call that fall on one position (only possible by overlapping sequences' memory) are not ordered.
- * b2_kv_cache_read: writes bf16(code * scale) of position offsets[b] + t to row t of `k`, `v` (any strides).  q, q_out, sine and
- * cosine must be NULL.
+ * b2_kv_cache_read: writes bf16(code * scale) of position offsets[b] + t to row t of `k`, `v` (any strides of at least head_dim, where
+ * there is more than one row along them).  q, q_out, sine and cosine must be NULL.
  * All pointers 16-byte aligned (scales, offsets and lengths: 4), strides multiples of 8 elements and not negative, and
  * batch * tokens * (heads + 2 kv_heads) < 2^31.  The reference has no quantised cache. */
 typedef struct b2_kv_cache_desc {
@@ -307,7 +307,8 @@ int b2_kv_cache_read(const b2_kv_cache_desc* desc, void* stream);
  * behind a length is never used.  A key row that holds a NaN or an infinity gives NaN to the rows that see it, and to no other; so
  * do such own values (a whole output row) and quantised values; bf16 prefix values that are not finite follow IEEE arithmetic.
  * Scores, softmax statistics and outputs are held in fp32; probabilities enter the second product as bf16 (bf16 cache) or f16
- * (quantised cache; there q enters the first as two e4m3 halves that hold its 8 bits).  head_dim 128 or 256.
+ * (quantised cache; there q enters the first as two e4m3 halves that hold its 8 bits, and a value is off by at most 2^-10 of itself
+ * and 2^-22 of the largest in its 64 keys).  head_dim 128 or 256.
  * `workspace`: NULL, or 32-byte aligned device scratch; with b2_prefix_attention_workspace_bytes(desc) bytes the 128-row tiles that
  * do not fill the device (a small call's, or those of the last partial wave) have their keys cut across the SMs and the parts joined
  * in a fixed order.  It needs no zeroing and holds nothing between calls, but two calls that may run at the same time need one each.  `status` as in b2_linear_desc.

@@ -294,6 +294,32 @@ def test_capture_replay_streams_and_repetition(device):
     del graphs
 
 
+@pytest.mark.parametrize("quantised", [False, True])
+def test_a_replay_follows_the_device_data(device, quantised):
+    """Bounds and lengths are read when the launch runs: a captured call of few row tiles, and so its cut, follows them."""
+    generator = torch.Generator(device=device).manual_seed(12)
+    batch, groups, prefix, own = 9, 3, 900, 70
+    q = (1.5 * torch.randn((batch, 8, 3, 128), device=device, generator=generator)).to(torch.bfloat16)
+    shared, mine = make_cache(generator, groups, 2, prefix, 128, quantised, device), make_cache(generator, batch, 2, own, 128, quantised, device)
+    bounds, prefix_lengths, own_lengths = whole([0, 3, 6, 9], device), whole([prefix] * groups, device), whole([own] * batch, device)
+    run = lambda: K.prefix_attention(q, shared, mine, members=bounds, prefix_lengths=prefix_lengths, own_lengths=own_lengths, causal=True)
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    for new in (([0, 3, 6, 9], [900, 900, 900], [70] * 9), ([0, 9, 9, 9], [5, 900, 0], [1, 70, 0, 3, 64, 65, 2, 69, 7]),
+                ([0, 0, 1, 9], [900, 63, 640], [0] * 9), ([0, 1, 8, 9], [0, 1, 128], [0, 9, 9, 9, 0, 0, 1, 2, 0])):
+        for tensor, values in zip((bounds, prefix_lengths, own_lengths), new):
+            tensor.copy_(whole(values, device))
+        got.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        K.check_status(device)
+        check(got, *reference(q, shared, mine, *new, True, 128 ** -0.5))
+    del graph
+
+
 def test_keys_behind_four_gigabytes(device):
     """The last group's rows start beyond 2^32 bytes; only what the lengths cover is ever written or read."""
     if torch.cuda.mem_get_info(device)[0] < 40 << 30:

@@ -56,7 +56,8 @@ def test_cache_write_refuses_half_given_operands():
                     dict(q=FAKE, q_out=FAKE, heads=8, q_stride=(8, 8, 1)), dict(sine=FAKE, cosine=FAKE, factor_batch_stride=2),
                     dict(sine=FAKE, cosine=FAKE + 4)):
         assert library.b2_kv_cache_write(ctypes.byref(_cache_desc(**changes)), None) == N.E_INVALID, changes
-    for changes in (dict(q=FAKE, q_out=FAKE, heads=8), dict(sine=FAKE, cosine=FAKE)):
+    for changes in (dict(q=FAKE, q_out=FAKE, heads=8), dict(sine=FAKE, cosine=FAKE), dict(batch=2, k_stride=(0, 2048, 256)),
+                    dict(tokens=2, v_stride=(4096, 2048, 64))):          # rows written over one another
         assert library.b2_kv_cache_read(ctypes.byref(_cache_desc(**changes)), None) == N.E_INVALID, changes
 
 
