@@ -12,7 +12,9 @@
 // once on the packed fp32 pipe.  Frequencies are formed in fp64, to a few 2^-53 of themselves.
 //
 // Each thread keeps the frequencies of VECTOR neighbouring columns and walks down the tokens: one 16-byte store per table
-// and token, bound by those stores.
+// and token.  Measured (B200): 8 x 16384 positions, head dimension 128, 16.0 us (70 MB, 4.4 TB/s), bound by the 30 instructions of an
+// angle and the latency of the positions; as many blocks as fit at once, for the frequencies are formed once per block (three waves of
+// them 17.5 us; 40 registers 18.1, 32 registers 27.5; angles in fp64 and the library's sincospif 24).
 #include "common.cuh"
 
 namespace b2 {
