@@ -12,9 +12,10 @@
 // once on the packed fp32 pipe.  Frequencies are formed in fp64, to a few 2^-53 of themselves.
 //
 // Each thread keeps the frequencies of VECTOR neighbouring columns and walks down the tokens: one 16-byte store per table
-// and token.  Measured (B200): 8 x 16384 positions, head dimension 128, 16.0 us (70 MB, 4.4 TB/s), bound by the 30 instructions of an
-// angle and the latency of the positions; as many blocks as fit at once, for the frequencies are formed once per block (three waves of
-// them 17.5 us; 40 registers 18.1, 32 registers 27.5; angles in fp64 and the library's sincospif 24).
+// and token.  Measured (B200): 8 x 16384 positions, head dimension 128, 14.9 us (70 MB, 4.7 TB/s), bound by the stores: without the
+// series it takes no less.  Stores that leave the L2 first (kept there 16.0 us); as many blocks as fit at once, for the frequencies are
+// formed once per block (two waves of them 17.5 us); 40 registers 18.1, eight columns per thread 25; angles in fp64 and the library's
+// sincospif 24.
 #include "common.cuh"
 
 namespace b2 {
@@ -101,8 +102,8 @@ __global__ void __launch_bounds__(AXES_THREADS) rope_axes_kernel(const __grid_co
 #pragma unroll
         for (int v = 0; v < VECTOR; ++v) sincos_turns(angle[v], s[v], c[v]);
         if (VECTOR == 4) {
-            *reinterpret_cast<float4*>(args.sine + out) = make_float4(s[0], s[1 % VECTOR], s[2 % VECTOR], s[3 % VECTOR]);
-            *reinterpret_cast<float4*>(args.cosine + out) = make_float4(c[0], c[1 % VECTOR], c[2 % VECTOR], c[3 % VECTOR]);
+            __stcs(reinterpret_cast<float4*>(args.sine + out), make_float4(s[0], s[1 % VECTOR], s[2 % VECTOR], s[3 % VECTOR]));
+            __stcs(reinterpret_cast<float4*>(args.cosine + out), make_float4(c[0], c[1 % VECTOR], c[2 % VECTOR], c[3 % VECTOR]));
         } else {
             args.sine[out] = s[0];
             args.cosine[out] = c[0];
