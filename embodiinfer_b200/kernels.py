@@ -10,7 +10,6 @@ from __future__ import annotations
 
 import ctypes
 import struct
-from contextlib import nullcontext
 
 import torch
 
@@ -38,9 +37,13 @@ def _require_cuda(*tensors: torch.Tensor | None) -> torch.device:
             return tensor.device
 
 
-def _on(device: torch.device):
-    """The device's context, or none when it is already current (entering one costs more than the launch)."""
-    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def _launch(function, device: torch.device, *arguments) -> int:
+    """``function(*arguments, stream)`` with ``device`` current; its context is entered only where it is not (that costs more than
+    the launch)."""
+    if device.index == torch.cuda.current_device():
+        return function(*arguments, torch._C._cuda_getCurrentRawStream(device.index))
+    with torch.cuda.device(device):
+        return function(*arguments, _stream(device))
 
 
 def gelu_table_range(table: torch.Tensor) -> tuple[int, int]:
@@ -281,7 +284,7 @@ def rope_axes(positions: torch.Tensor, sections: tuple[int, ...], sine: torch.Te
         raise ValueError("rope_axes requires one positive section for each axis")
     shape = (*shape[1:], half)
     if sine is None and cosine is None:
-        sine = torch.empty(shape, device=device, dtype=torch.float32)
+        sine = positions.new_empty(shape, dtype=torch.float32)
         cosine = torch.empty_like(sine)
     else:
         for table in (sine, cosine):
@@ -290,10 +293,8 @@ def rope_axes(positions: torch.Tensor, sections: tuple[int, ...], sine: torch.Te
     tokens = positions.numel() // axes if axes else 0
     if tokens == 0:
         return sine, cosine
-    with _on(device):
-        status = N.load().b2_rope_axes(positions.data_ptr(), positions.element_size(), struct.pack(f"{axes}i", *sections), axes, tokens,
-                                       2 * half, float(theta), N.ROPE_OWN_SPECTRUM if own_spectrum else 0, sine.data_ptr(),
-                                       cosine.data_ptr(), _stream(device))
+    status = _launch(N.load().b2_rope_axes, device, positions.data_ptr(), positions.element_size(), struct.pack(f"{axes}i", *sections), axes,
+                     tokens, 2 * half, float(theta), N.ROPE_OWN_SPECTRUM if own_spectrum else 0, sine.data_ptr(), cosine.data_ptr())
     N.check(status, "b2_rope_axes")
     return sine, cosine
 
@@ -313,7 +314,8 @@ def _check_cache(cache: QuantizedKVCache, what: str) -> tuple[int, int, int, int
     """The (batch, kv_heads, capacity, head_dim) of a quantised cache."""
     k_codes, k_scales, v_codes, v_scales = cache
     shape = k_codes.shape
-    if len(shape) != 4 or v_codes.shape != shape or k_scales.shape != shape[:3] or v_scales.shape != shape[:3]:
+    rows = shape[:3]
+    if len(shape) != 4 or v_codes.shape != shape or k_scales.shape != rows or v_scales.shape != rows:
         raise ValueError(f"{what} requires codes [batch, kv_heads, capacity, head_dim] and scales [batch, kv_heads, capacity]")
     if not (k_codes.element_size() == 1 == v_codes.element_size() and k_scales.dtype is torch.float32 is v_scales.dtype and k_codes.is_contiguous()
             and v_codes.is_contiguous() and k_scales.is_contiguous() and v_scales.is_contiguous()):
@@ -373,9 +375,7 @@ def kv_cache_write(k: torch.Tensor, v: torch.Tensor, cache: QuantizedKVCache, *,
     desc = _CACHE_DESC.pack(_address(q), _address(q_out), k.data_ptr(), v.data_ptr(), _address(sine), _address(cosine), k_codes.data_ptr(),
                             k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(), _address(offsets), _address(lengths), *q_stride,
                             *strides, factor_stride, batch, tokens, heads, kv_heads, head_dim, capacity)
-    with _on(device):
-        status = N.load().b2_kv_cache_write(desc, _stream(device))
-    N.check(status, "b2_kv_cache_write")
+    N.check(_launch(N.load().b2_kv_cache_write, device, desc), "b2_kv_cache_write")
 
 
 def kv_cache_read(cache: QuantizedKVCache, k_out: torch.Tensor, v_out: torch.Tensor, *, offsets: torch.Tensor | None = None,
@@ -389,9 +389,7 @@ def kv_cache_read(cache: QuantizedKVCache, k_out: torch.Tensor, v_out: torch.Ten
         desc = _CACHE_DESC.pack(0, 0, k_out.data_ptr(), v_out.data_ptr(), 0, 0, k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
                                 v_scales.data_ptr(), _address(offsets), _address(lengths), 0, 0, 0, *strides, 0, batch, tokens, 0, kv_heads,
                                 head_dim, capacity)
-        with _on(device):
-            status = N.load().b2_kv_cache_read(desc, _stream(device))
-        N.check(status, "b2_kv_cache_read")
+        N.check(_launch(N.load().b2_kv_cache_read, device, desc), "b2_kv_cache_read")
     return k_out, v_out
 
 
@@ -411,6 +409,15 @@ def _cache_part(part, count: int, width: int, what: str) -> tuple[int, int, int,
     if batch != count and count >= 0 or head_dim != width:
         raise ValueError(f"prefix_attention: the {what} cache does not fit the queries")
     return bits, batch, kv_heads, capacity, pointers if capacity else (0, 0, 0, 0)
+
+
+def _attend(library, q: torch.Tensor, pointers: tuple, sizes: tuple, stream: int) -> int:
+    desc = _ATTENTION_DESC.pack(*pointers, 0, 0, *sizes)
+    size = library.b2_prefix_attention_workspace_bytes(desc)
+    if size:          # scratch of this call alone (also inside a captured graph: it is the graph's own)
+        workspace = q.new_empty(size, dtype=torch.uint8)
+        desc = _ATTENTION_DESC.pack(*pointers, workspace.data_ptr(), size, *sizes)
+    return library.b2_prefix_attention(desc, stream)
 
 
 def prefix_attention(q: torch.Tensor, prefix, own=None, *, members: torch.Tensor | None = None, prefix_lengths: torch.Tensor | None = None,
@@ -442,7 +449,7 @@ def prefix_attention(q: torch.Tensor, prefix, own=None, *, members: torch.Tensor
     if kv_heads == 0 or heads % kv_heads or groups == 0 or (members is None and batch % groups):
         raise ValueError("prefix_attention requires heads divisible by kv_heads, and a batch divisible by the groups unless members is given")
     if out is None:
-        out = torch.empty(shape, device=device, dtype=torch.bfloat16)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != shape or out.dtype is not torch.bfloat16 or not out.is_contiguous():
         raise ValueError("attention output must be a contiguous bf16 tensor of the queries' shape")
     if not (batch and heads and queries and head_dim):
@@ -455,16 +462,7 @@ def prefix_attention(q: torch.Tensor, prefix, own=None, *, members: torch.Tensor
                 _address(own_lengths), status.data_ptr())
     sizes = (*q_stride[:3], head_dim ** -0.5 if scale is None else scale, N.ATTENTION_CAUSAL if causal else 0, batch, groups, heads,
              kv_heads, queries, head_dim, prefix_capacity, own_capacity, bits)
-    desc = _ATTENTION_DESC.pack(*pointers, 0, 0, *sizes)
-    library = N.load()
-    with _on(device):
-        # scratch of this call alone (also inside a captured graph: it is the graph's own)
-        size = library.b2_prefix_attention_workspace_bytes(desc)
-        if size:
-            workspace = torch.empty(size, device=device, dtype=torch.uint8)
-            desc = _ATTENTION_DESC.pack(*pointers, workspace.data_ptr(), size, *sizes)
-        code = library.b2_prefix_attention(desc, _stream(device))
-    N.check(code, "b2_prefix_attention")
+    N.check(_launch(_attend, device, N.load(), q, pointers, sizes), "b2_prefix_attention")
     return out
 
 
