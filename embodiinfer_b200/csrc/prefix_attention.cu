@@ -126,7 +126,7 @@ struct PaArgs {
     int64_t q_stride[3];
     float scale_log2;
     int batch, groups, heads, kv_heads, queries, prefix_capacity, own_capacity;
-    int rows_per_member, sms, slots, max_splits, causal;      // slots: CTAs that may leave partial rows; 0 = nothing is cut
+    int rows_per_member, sms, slots, max_splits, causal, share;      // share: query heads of a key/value head; slots: CTAs that may leave partial rows; 0 = nothing is cut
 };
 
 // What a CTA works on, in shared memory: written by warp 0 before the block barrier.
@@ -134,6 +134,16 @@ struct PaWork {
     int group, first_member, row0, rows, segments, first_segment_member, key_tiles;
     int kv_head, split, splits, place;      // place: among the row tiles that are cut, and in all of their parts (split * row tiles + it)
 };
+
+// a / b for a >= 0, b > 0.  Below 2^21 the fp32 quotient (2 steps of 2^-23 off at most) is within one of it and takes a quarter of an integer
+// division's time; the look-up is a chain of them.
+__device__ __forceinline__ int pa_divide(int a, int b) {
+    if (a >= 1 << 21) return a / b;
+    int q = int(__fdividef(float(a), float(b)));
+    const int r = a - q * b;
+    q += r < 0 ? -1 : r >= b ? 1 : 0;
+    return q;
+}
 
 __device__ __forceinline__ int clamp_length(int value, int capacity) { return value < 0 ? 0 : (value > capacity ? capacity : value); }
 
@@ -398,12 +408,12 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
         // ---- which row tile and head, and which part of its keys: whole waves of them uncut, the rest cut into equal parts
         const int ctas = int(gridDim.x), block = int(blockIdx.x);
         const int items = int(min(int64_t(total_tiles) * args.kv_heads, int64_t(ctas)));
-        const int uncut = items > args.sms ? items / args.sms * args.sms : 0, rest = items - uncut;
+        const int uncut = items > args.sms ? pa_divide(items, args.sms) * args.sms : 0, rest = items - uncut;
         int splits = 1, split = 0, place = 0, item = block;
-        if (rest > 0) splits = max(1, min(args.max_splits, min(args.slots, ctas - uncut) / rest));
+        if (rest > 0 && args.slots > 0) splits = max(1, min(args.max_splits, pa_divide(min(args.slots, ctas - uncut), rest)));
         if (block >= uncut) {
             place = block - uncut;
-            split = rest > 0 ? place / rest : splits;
+            split = rest > 0 ? pa_divide(place, rest) : splits;
             item = uncut + place - split * rest;
         }
         if (block == 0 && lane == 0 && args.slots > 0) {
@@ -411,12 +421,12 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
             args.cut[1] = splits;
         }
         // row tile fastest: CTAs that run together share the key tiles of their group in the L2
-        const int kv_head = total_tiles > 0 ? item / total_tiles : 0, tile = item - kv_head * total_tiles;
+        const int kv_head = total_tiles > 0 ? pa_divide(item, total_tiles) : 0, tile = item - kv_head * total_tiles;
         if (split >= splits) {
             group = -1;          // nothing left for this one
         } else if (args.members == nullptr) {
             count = args.batch / args.groups;
-            group = tile / row_tiles(count);
+            group = pa_divide(tile, row_tiles(count));
             group_tile = tile - group * row_tiles(count);
             first = group * count;
         } else {
@@ -438,10 +448,10 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
         const int row0 = group_tile * PA_ROWS;
         int rows = group < 0 ? 0 : count * args.rows_per_member - row0;
         rows = rows < 0 ? 0 : (rows > PA_ROWS ? PA_ROWS : rows);
-        const int first_own = row0 / args.rows_per_member;                      // first member with rows in this tile
+        const int first_own = pa_divide(row0, args.rows_per_member);                      // first member with rows in this tile
         if (lane == 0) *work = PaWork{group, first, row0, rows, 0, first_own, 0, kv_head, split, rows > 0 && block >= uncut ? splits : 1, place};
         named_barrier<3, 288>();          // the softmax warps fetch the queries while the lengths come
-        const int segments = rows == 0 ? 1 : (row0 + rows - 1) / args.rows_per_member - first_own + 2;
+        const int segments = rows == 0 ? 1 : pa_divide(row0 + rows - 1, args.rows_per_member) - first_own + 2;
         int total = 0;
         for (int s0 = 0; s0 < segments; s0 += 32) {
             const int s = s0 + lane;
@@ -484,9 +494,9 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
         int64_t query_offset = -1, out_offset = -1;
         exists = row < found.rows;
         if (exists) {
-            const int member = (found.row0 + row) / args.rows_per_member, inside = found.row0 + row - member * args.rows_per_member;
-            const int head_in_group = inside / args.queries, query = inside - head_in_group * args.queries;
-            const int head = found.kv_head * (args.heads / args.kv_heads) + head_in_group;
+            const int member = pa_divide(found.row0 + row, args.rows_per_member), inside = found.row0 + row - member * args.rows_per_member;
+            const int head_in_group = pa_divide(inside, args.queries), query = inside - head_in_group * args.queries;
+            const int head = found.kv_head * args.share + head_in_group;
             my_segment = member - found.first_segment_member + 1;
             hidden = args.causal ? args.queries - 1 - query : 0;
             out_offset = ((int64_t(found.first_member + member) * args.heads + head) * args.queries + query) * D;
@@ -497,13 +507,19 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
             row_output[row] = out_offset;
         }
         named_barrier<1, 256>();
-#pragma unroll 4
-        for (int i = int(threadIdx.x); i < PA_ROWS * PIECES; i += 256) {
-            const int r = i / PIECES, piece = i % PIECES;
-            const int64_t from = row_query[r];
-            const uint32_t to = staging_smem + uint32_t(r * D * 2 + ((piece ^ (r & 7)) << 4));
-            const __nv_bfloat16* source = args.q + (from < 0 ? 0 : from) + piece * 8;
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(source), "r"(from < 0 ? 0 : 16) : "memory");
+        constexpr int BATCH = 8;          // the copies would hold the next offset's load back
+#pragma unroll 1
+        for (int first = int(threadIdx.x); first < PA_ROWS * PIECES; first += BATCH * 256) {
+            int64_t from[BATCH];
+#pragma unroll
+            for (int n = 0; n < BATCH; ++n) from[n] = row_query[(first + n * 256) / PIECES];
+#pragma unroll
+            for (int n = 0; n < BATCH; ++n) {
+                const int i = first + n * 256, r = i / PIECES, piece = i % PIECES;
+                const uint32_t to = staging_smem + uint32_t(r * D * 2 + ((piece ^ (r & 7)) << 4));
+                const __nv_bfloat16* source = args.q + (from[n] < 0 ? 0 : from[n]) + piece * 8;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(source), "r"(from[n] < 0 ? 0 : 16) : "memory");
+            }
         }
     }
     tc_fence_before_sync();
@@ -1315,7 +1331,8 @@ int launch_prefix_attention(const b2_prefix_attention_desc* desc, cudaStream_t s
     args.queries = desc->queries;
     args.prefix_capacity = desc->prefix_capacity;
     args.own_capacity = desc->own_capacity;
-    args.rows_per_member = desc->heads / desc->kv_heads * desc->queries;
+    args.share = desc->heads / desc->kv_heads;
+    args.rows_per_member = args.share * desc->queries;
     args.sms = sm_count();
     args.slots = plan.slots;
     args.max_splits = plan.slots > 0 ? plan.max_splits : 1;
