@@ -389,10 +389,27 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
         };
         constexpr int MANY = 1 << 29;          // bounds that run backwards may add up to anything: enough for every CTA
         int total_tiles = 0;
+        // More row tiles than SMs: the longest prefixes first, so that the last wave is made of short ones (as far as a warp sees all groups).
+        const bool sorted = args.prefix_lengths != nullptr && args.groups <= 32 && int(gridDim.x) > args.sms;
+        int group_at = lane;          // sorted: the group at this place
+        if (sorted) {
+            const int length = lane < args.groups ? clamp_length(__ldg(args.prefix_lengths + lane), args.prefix_capacity) : -1;
+            int rank = 0;
+#pragma unroll 8
+            for (int other = 0; other < 32; ++other) {
+                const int its = __shfl_sync(0xffffffffu, length, other);
+                rank += its > length || (its == length && other < lane);
+            }
+            segment_first[rank] = lane;
+            __syncwarp();
+            group_at = segment_first[lane];
+            __syncwarp();
+        }
         int batch_first = 0, batch_count = 0, batch_sum = 0;          // of 32 groups, one per lane: the first 32, until they have to be passed
         auto load_groups = [&](int g0) {
+            const int g = g0 + group_at;
             batch_first = batch_count = 0;
-            if (g0 + lane < args.groups) batch_count = group_members(g0 + lane, batch_first);
+            if (g < args.groups) batch_count = group_members(g, batch_first);
             batch_sum = inclusive_sum(row_tiles(batch_count));
         };
         if (args.members == nullptr) {
@@ -420,14 +437,16 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
             args.cut[0] = splits > 1 ? rest : 0;
             args.cut[1] = splits;
         }
-        // row tile fastest: CTAs that run together share the key tiles of their group in the L2
-        const int kv_head = total_tiles > 0 ? pa_divide(item, total_tiles) : 0, tile = item - kv_head * total_tiles;
+        // row tile fastest: CTAs that run together share the key tiles of their group in the L2; sorted: all heads of a row tile in its turn
+        const int slow = pa_divide(item, sorted ? args.kv_heads : max(total_tiles, 1)), fast = item - slow * (sorted ? args.kv_heads : max(total_tiles, 1));
+        const int kv_head = sorted ? fast : slow, tile = sorted ? slow : fast;
         if (split >= splits) {
             group = -1;          // nothing left for this one
         } else if (args.members == nullptr) {
             count = args.batch / args.groups;
             group = pa_divide(tile, row_tiles(count));
             group_tile = tile - group * row_tiles(count);
+            if (sorted) group = __shfl_sync(0xffffffffu, group_at, group);
             first = group * count;
         } else {
             int before = 0;
@@ -437,7 +456,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
                 const unsigned hit = __ballot_sync(0xffffffffu, mine > 0 && tile >= start && tile < start + mine);
                 if (hit != 0u) {
                     const int source = __ffs(int(hit)) - 1;
-                    group = g0 + source;
+                    group = g0 + __shfl_sync(0xffffffffu, group_at, source);
                     first = __shfl_sync(0xffffffffu, batch_first, source);
                     count = __shfl_sync(0xffffffffu, batch_count, source);
                     group_tile = tile - __shfl_sync(0xffffffffu, start, source);
@@ -845,11 +864,13 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
                 }
             }
         }
+        // each thread sends what it has written: the other group's half of the row does not have to be waited for
         fence_async_shared();
-        named_barrier<1, 256>();
-        if (exists && parity_group == 0) {
-            const void* destination = stored ? static_cast<const void*>(args.out + row_output[row]) : static_cast<const void*>(args.partial + (first_partial + row) * D);
-            asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(destination), "r"(out_row), "r"(row_bytes) : "memory");
+        if (exists) {
+            const uint32_t half_bytes = row_bytes / 2, from = out_row + uint32_t(parity_group) * half_bytes;
+            const void* destination = stored ? static_cast<const void*>(args.out + row_output[row] + first_column)
+                                             : static_cast<const void*>(args.partial + (first_partial + row) * D + first_column);
+            asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(destination), "r"(from), "r"(half_bytes) : "memory");
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
             asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");          // the rows have been taken: the CTA may leave
         }

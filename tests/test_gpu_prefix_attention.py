@@ -176,6 +176,12 @@ def test_the_last_wave_is_cut(device, monkeypatch, heads, kv_heads, dim, quantis
     assert (cut == uncut).flatten(1).all(1).sum() >= bounds[-1] // 2 and not torch.equal(cut, uncut)          # most are in the whole wave
 
 
+def test_uniform_groups_in_several_waves(device):
+    """No bounds given, more row tiles than SMs: the row tiles are taken in the order of their prefixes' lengths."""
+    bounds = [10 * g for g in range(25)]
+    run_case(device, bounds, 8, 1, 10, 256, 130, 10, True, True, [(59 * g) % 131 for g in range(24)], [b % 11 for b in range(240)], uniform=True)
+
+
 def test_without_a_prefix(device):
     generator = torch.Generator(device=device).manual_seed(5)
     q = torch.randn((3, 8, 4, 128), device=device, generator=generator).to(torch.bfloat16)
