@@ -88,7 +88,7 @@ struct PaShape {
     static constexpr int FREE_V_STAGES = FP8 ? STAGES : STAGES - int(PA_ROWS * D * 2 / KV_BYTES);      // of V: not under the queries as they come in
     static constexpr int VALUE_STAGES = FP8 ? 2 : 0;                        // converted value tiles
     static constexpr uint32_t VALUE_BYTES = PA_KEYS * D * 2;
-    static constexpr int VALUE_WARPS = 4;
+    static constexpr int VALUE_WARPS = 4, VALUE_TEAM = FP8 ? 2 : 4;         // warps that prepare a value tile: quantised, two teams a tile apart
     static constexpr int THREADS = PA_WARPS * 32;
     // With D = 128 each softmax group has an accumulator of its own and never meets the other before the end; with D = 256 there is
     // room for one accumulator and one P, and for three of Q's four atoms (32 columns: 64 bf16 or 128 e4m3 values of a row): the last one
@@ -350,10 +350,10 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
     if (warp == 0) {          // one lane per barrier (8 bytes each, in the order above); unused places of the arrays are barriers too
         for (int i = lane; i < 74; i += 32) {
             int count = 1;
-            if (i >= 24 && i < 32 && FP8) count = Shape::VALUE_WARPS;                 // v_empty
-            else if (i >= 32 && i < 40) count = Shape::VALUE_WARPS;                   // value_full
+            if (i >= 24 && i < 32 && FP8) count = Shape::VALUE_TEAM;                  // v_empty
+            else if (i >= 32 && i < 40) count = Shape::VALUE_TEAM;                    // value_full
             else if (i >= 50 && i < 54) count = 4;                                    // s_free, p_ready
-            else if (i >= 60 && i < 64) count = 4 + Shape::VALUE_WARPS;               // scale_empty
+            else if (i >= 60 && i < 64) count = 4 + Shape::VALUE_TEAM;                // scale_empty
             else if (i == 73) count = 8;                                              // q_ready
             mbar_init(bars + 8 * i, count);
         }
@@ -1019,35 +1019,34 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
         // becomes two 16-byte chunks of the 64-column group they belong to.  Odd groups store their two chunks in the other order: the
         // eight lanes of a store then meet all banks.
         constexpr int PIECES = D / 16, BATCH = 4;
-        static_assert(PA_KEYS * PIECES % (BATCH * 32 * Shape::VALUE_WARPS) == 0, "whole batches");
-        const int thread = (warp - PA_VALUE_WARP) * 32 + lane;
-        PaRing<STAGES> ring;
-        PaCursor cursor(segment_first, segment_length, num_tiles > 0 ? start_tile : -1);
+        static_assert(PA_KEYS * PIECES % (BATCH * 32 * Shape::VALUE_TEAM) == 0, "whole batches");
+        const int team = (warp - PA_VALUE_WARP) / Shape::VALUE_TEAM, thread = ((warp - PA_VALUE_WARP) % Shape::VALUE_TEAM) * 32 + lane;
+        PaCursor cursor(segment_first, segment_length, team < num_tiles ? start_tile + team : -1);
         if (num_tiles > 0) pa_wait(q_ready, 0u, patience);          // the queries came through this place
-        for (int j = 0; j < num_tiles; ++j) {
-            const int c = j & 1, stage = j % PA_SCALE_STAGES;
+        for (int j = team; j < num_tiles; j += 2) {
+            const int c = team, stage = j % PA_SCALE_STAGES, slot = j % STAGES;
             const uint32_t* value_scales = reinterpret_cast<const uint32_t*>(generic + Shape::OFF_SCALES) + stage * PA_SCALE_FLOATS + PA_KEYS;
             cursor.seek(start_tile + j);
             // prefix keys are seen by every row: what is not finite among them may reach all
             const bool clean = cursor.segment > 0 || cursor.keys(start_tile + j) < PA_KEYS;
             pa_wait(scale_full + 8 * stage, uint32_t(j / PA_SCALE_STAGES) & 1u, patience);
-            pa_wait(v_full + 8 * ring.slot, ring.parity, patience);
+            pa_wait(v_full + 8 * slot, uint32_t(j / STAGES) & 1u, patience);
             pa_wait(value_empty + 8 * c, (uint32_t(j >> 1) & 1u) ^ 1u, patience);
             auto convert = [&](auto tag) {
                 constexpr bool CLEAN = decltype(tag)::value;
 #pragma unroll 1
-                for (int first = thread; first < PA_KEYS * PIECES; first += BATCH * 32 * Shape::VALUE_WARPS) {
+                for (int first = thread; first < PA_KEYS * PIECES; first += BATCH * 32 * Shape::VALUE_TEAM) {
                     uint4 codes[BATCH];
                     uint32_t scale_bits[BATCH];
 #pragma unroll
                     for (int n = 0; n < BATCH; ++n) {          // all loads first: each of the stores would hold the next load back
-                        const uint32_t i = first + n * 32 * Shape::VALUE_WARPS, key = i / PIECES, piece = i % PIECES;
-                        codes[n] = lds_u4(v_smem + ring.slot * Shape::KV_BYTES + (piece >> 3) * Shape::KV_ATOM_BYTES + key * 128u + (((piece & 7u) ^ (key & 7u)) << 4));
+                        const uint32_t i = first + n * 32 * Shape::VALUE_TEAM, key = i / PIECES, piece = i % PIECES;
+                        codes[n] = lds_u4(v_smem + slot * Shape::KV_BYTES + (piece >> 3) * Shape::KV_ATOM_BYTES + key * 128u + (((piece & 7u) ^ (key & 7u)) << 4));
                         scale_bits[n] = value_scales[key];
                     }
 #pragma unroll
                     for (int n = 0; n < BATCH; ++n) {
-                        const uint32_t i = first + n * 32 * Shape::VALUE_WARPS, key = i / PIECES, piece = i % PIECES, swizzle = key & 7u;
+                        const uint32_t i = first + n * 32 * Shape::VALUE_TEAM, key = i / PIECES, piece = i % PIECES, swizzle = key & 7u;
                         const __half2 scale = *reinterpret_cast<const __half2*>(&scale_bits[n]);
                         const uint32_t group = values_smem + c * Shape::VALUE_BYTES + (piece >> 2) * Shape::KV_ATOM_BYTES + key * 128u;
                         const uint32_t odd = (piece >> 2) & 1u, left = (piece & 3u) * 2u;
@@ -1065,11 +1064,10 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
             fence_async_shared();
             __syncwarp();
             if (lane == 0) {
-                mbar_arrive(v_empty + 8 * ring.slot);
+                mbar_arrive(v_empty + 8 * slot);
                 mbar_arrive(value_full + 8 * c);
                 mbar_arrive(scale_empty + 8 * stage);
             }
-            ring.next();
         }
     } else if (FP8 && warp == PA_SCALE_WARP) {
         // ------------------------------------------------------------- scales of the key tiles
