@@ -26,9 +26,9 @@
 //   64 members, one query, 32768 quantised keys, D = 128: 81 us, 1400 cycles per tile; without its exponentials 74, without its
 //   products 78, without the conversion of values 74: the chain of a softmax group -- scores out, maximum, exponentials, P in, each with
 //   its latency and two warps per scheduler to hide it -- and not one unit is what bounds the loop
-//   256 ten-query chunks over 32 x 712 quantised keys, D = 256: 45 us: 176 row tiles of 12 key tiles on 148 SMs, 21 k of a CTA's 41 k
-//   cycles before and behind the loop (4.9 k look-up, 3.6 k splitting Q, 5 k output)
-//   four ten-query chunks over 560 bf16 keys, D = 256: 14.0 us, 9 in this kernel for one tile per CTA, the rest the join
+//   256 ten-query chunks over 32 x 712 quantised keys, D = 256: 41 us (in the groups' order 44): 176 row tiles of 12 key tiles on 148
+//   SMs, 21 k of a CTA's 41 k cycles before and behind the loop (4.8 k look-up, 3.6 k splitting Q, 5 k output)
+//   four ten-query chunks over 560 bf16 keys, D = 256: 13.6 us, 9 in this kernel for two tiles per CTA, the rest the join
 //
 // bf16 cache.  K and V are read as they lie in memory.  What the tensor core must not see is taken out of the value tile in
 // shared memory, because a probability of zero times an infinity or a NaN is not zero: rows behind the end of a segment are set to
@@ -40,7 +40,7 @@
 //   2^e bringing the row's largest value into [128, 256): a bf16 value has 8 significant bits, hi takes 4 and lo the rest,
 //   exactly, down to 2^-17 of the row's largest value.  Two products at twice the bf16 rate cost what one bf16 product
 //   would, and no key is ever converted.  ks multiplies the score.
-//   Output.  The four value warps turn the codes into f16, exactly, and multiply by vs 2^-E: one rounding of 2^-11 for the scale and
+//   Output.  The four value warps, two teams a tile apart, turn the codes into f16, exactly, and multiply by vs 2^-E: one rounding of 2^-11 for the scale and
 //   one for the product, beside the 2^-8 of the result.  2^E is the unit of the accumulator, the same for all rows: it follows the
 //   largest vs of a key tile when that leaves [2^-3, 2^6) units, and the accumulator is rescaled then as it is for a new reference.
 //   A value is so off by at most 2^-10 of itself and, f16 ending at 2^-24 units, 2^-22 of the largest in its tile of 64 keys, whatever

@@ -625,16 +625,25 @@ class Pi05ShapedPolicy(nn.Module):
         final, _ = _ada_rms_norm(_gated_residual(x, pending), modulations[-1])
         return F.linear(final, self.action_out).float()
 
-    def denoise_samples(self, cache, prefix_length: int, noise: torch.Tensor, *, quantised_cache: bool = False) -> torch.Tensor:
+    def denoise_samples(self, cache, prefix_length: int, noise: torch.Tensor, *, quantised_cache: bool = False,
+                        shared_prefix: bool | None = None) -> torch.Tensor:
         """Several action chunks of every observation: ``noise`` [B, N, 10, 32] fp32, one starting point per sample, to
         [B, N, 10, 32].  ``cache`` is ``encode_prefix``'s for the B observations: the N samples of an observation read its one
-        prefix (``b2_prefix_attention``), where ``denoise`` would need it N times.  ``quantised_cache`` holds the prefixes'
-        and the samples' keys and values as e4m3 codes with a scale for each row (``b2_kv_cache_write``)."""
+        prefix (``b2_prefix_attention``).  ``shared_prefix=False`` gives every sample a copy (``denoise``); by default calls of
+        at most 64 chunks do, whose attention is a chain of short launches that ``b2_attention`` has less of (ten steps over 560
+        tokens: 8 / 64 / 128 / 256 chunks take 8.1 / 13.4 / 17.5 / 27.0 ms with copies, 9.6 / 13.6 / 15.5 / 24.3 without).
+        ``quantised_cache`` holds the prefixes' and the samples' keys and values as e4m3 codes with a scale for each row
+        (``b2_kv_cache_write``), half the memory of the one bf16 copy, always shared."""
         batch, samples = noise.shape[:2]
         count, device, head_dim = batch * samples, self.device_, GEMMA_300M.head_dim
         actions = noise.reshape(count, ACTION_HORIZON, ACTION_DIM)
         if count == 0:
             return noise.clone()
+        if shared_prefix is None:
+            shared_prefix = count > 64
+        if not (shared_prefix or quantised_cache):
+            copies = [tuple(part.repeat_interleave(samples, 0) for part in pair) for pair in cache[: len(self.expert)]]
+            return self.denoise(copies, prefix_length, actions).view(noise.shape)
         positions = prefix_length + torch.arange(ACTION_HORIZON, device=device)
         rope = K.rope_axes(positions[None], (head_dim // 2,))
         schedule = self.modulation_schedule(count)
@@ -663,14 +672,15 @@ class Pi05ShapedPolicy(nn.Module):
         return self.denoise(cache, prefix_length, self.noise(images.shape[0]) if noise is None else noise)
 
     @torch.no_grad()
-    def sample(self, observations: dict, samples: int, noise: torch.Tensor | None = None, *, quantised_cache: bool = False) -> torch.Tensor:
+    def sample(self, observations: dict, samples: int, noise: torch.Tensor | None = None, *, quantised_cache: bool = False,
+               shared_prefix: bool | None = None) -> torch.Tensor:
         """``samples`` action chunks [B, samples, 10, 32] of every observation, for a caller that chooses among them: the vision
-        and prefix towers run once per observation, and the samples share the prefix's keys and values."""
+        and prefix towers run once per observation (see ``denoise_samples`` for what the samples share)."""
         images, tokens = observations["images"], observations["tokens"]
         cache, prefix_length = self.encode_prefix(images, tokens)
         if noise is None:
             noise = self.noise(images.shape[0] * samples).view(images.shape[0], samples, ACTION_HORIZON, ACTION_DIM)
-        return self.denoise_samples(cache, prefix_length, noise, quantised_cache=quantised_cache)
+        return self.denoise_samples(cache, prefix_length, noise, quantised_cache=quantised_cache, shared_prefix=shared_prefix)
 
     @torch.no_grad()
     def calibrate_fused_mlp(self, observations: dict, margin: float = 1.0) -> None:

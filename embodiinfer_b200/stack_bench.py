@@ -80,7 +80,7 @@ def measure_samples(policy: Pi05ShapedPolicy, observations: int = 8, samples: in
                    for _ in range(2)) for _ in policy.expert]
     noise = torch.randn((observations, samples, ACTION_HORIZON, ACTION_DIM), device=device, generator=generator)
     repeated = [tuple(part.repeat_interleave(samples, 0) for part in pair) for pair in cache]
-    return {"shared": graph_milliseconds(lambda: policy.denoise_samples(cache, PREFIX_TOKENS, noise)),
+    return {"shared": graph_milliseconds(lambda: policy.denoise_samples(cache, PREFIX_TOKENS, noise, shared_prefix=True)),
             "shared_quantised": graph_milliseconds(lambda: policy.denoise_samples(cache, PREFIX_TOKENS, noise, quantised_cache=True)),
             "a_copy_per_sample": graph_milliseconds(lambda: policy.denoise(repeated, PREFIX_TOKENS, noise.flatten(0, 1)))}
 
@@ -126,7 +126,7 @@ def main() -> None:
                           "ms_per_step": round(milliseconds / 10, 4),
                           "quantised_linear_tflops": round(flops / milliseconds / 1e9, 2), **common}), flush=True)
 
-    for observations, samples in ((1, 8), (8, 8)):
+    for observations, samples in ((1, 8), (8, 8), (32, 8)):
         found = measure_samples(policy, observations, samples)
         print(json.dumps({"case": f"expert_denoise_10_steps_{samples}_samples_of_{observations}",
                           **{f"ms_{key}": round(value, 4) for key, value in found.items()}, **common}), flush=True)

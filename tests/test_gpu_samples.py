@@ -73,20 +73,23 @@ def test_samples_share_the_prefix(device):
     for calibrated in (False, True):
         if calibrated:
             policy.calibrate_fused_mlp(observations)
-        actions = policy.sample(observations, 4)
+        actions = policy.sample(observations, 4, shared_prefix=True)
         assert actions.shape == (3, 4, ACTION_HORIZON, ACTION_DIM) and torch.isfinite(actions).all()
-        assert torch.equal(actions, policy.sample(observations, 4)), "sampling must be deterministic"
+        assert torch.equal(actions, policy.sample(observations, 4, shared_prefix=True)), "sampling must be deterministic"
         cache, length = policy.encode_prefix(observations["images"], observations["tokens"])
         repeated = [tuple(part.repeat_interleave(4, 0) for part in pair) for pair in cache]
         noise = policy.noise(12)
         with torch.no_grad():
             expected = policy.denoise(repeated, length, noise).view(actions.shape)
+        assert torch.equal(policy.sample(observations, 4), expected)          # few chunks: a copy each
         assert float((actions - expected).norm() / expected.norm()) < 2e-2
         # the quantised cache rounds keys and values to 2^-4 of themselves
         quantised = policy.sample(observations, 4, quantised_cache=True)
         error = float((quantised - actions).norm() / actions.norm())
         assert 0.0 < error < 2.0 ** -4
         assert not torch.equal(actions[:, 0], actions[:, 1])
+    many = policy.sample(observations, 24)
+    assert torch.equal(many, policy.sample(observations, 24, shared_prefix=True)) and not torch.equal(many, policy.sample(observations, 24, shared_prefix=False))
     assert policy.sample(observations, 0).shape == (3, 0, ACTION_HORIZON, ACTION_DIM)
     K.check_status(device)
 
@@ -98,8 +101,8 @@ def test_samples_in_a_graph(device):
     with torch.no_grad():
         cache, length = policy.encode_prefix(observations["images"], observations["tokens"])
         noise = policy.noise(6).view(2, 3, ACTION_HORIZON, ACTION_DIM)
-        for quantised in (False, True):
-            run = lambda: policy.denoise_samples(cache, length, noise, quantised_cache=quantised)
+        for options in (dict(), dict(shared_prefix=True), dict(quantised_cache=True)):
+            run = lambda: policy.denoise_samples(cache, length, noise, **options)
             eager = run()
             stream = torch.cuda.Stream()
             stream.wait_stream(torch.cuda.current_stream())
