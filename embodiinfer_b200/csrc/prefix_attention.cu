@@ -1255,9 +1255,10 @@ PaPlan pa_plan(const b2_prefix_attention_desc* d) {
     plan.items = tiles * d->kv_heads;
     const int64_t sms = sm_count(), uncut = plan.items > sms ? plan.items / sms * sms : 0, rest = plan.items - uncut;
     // The cut of what is behind the last whole wave, in 1/32 of a key tile's time (0.6 to 0.9 us): waves of CTAs times (set-up + tiles) --
-    // looking up the work, fetching the queries and leaving the output take as long as 12 tiles -- and the join's launch and traffic.
+    // looking up the work, fetching the queries and leaving the output take as long as 12 tiles -- and the join's launch and traffic.  At most
+    // four waves of parts: their fp32 rows are 64 or 128 KB each.
     int64_t best = 0, splits = 1;
-    for (int64_t s = 1; rest > 0 && s <= 64 && s <= key_tiles; ++s) {
+    for (int64_t s = 1; rest > 0 && s <= 64 && s <= key_tiles && (s == 1 || rest * s <= 4 * sms); ++s) {
         const int64_t waves = (rest * s + sms - 1) / sms;
         const int64_t cost = waves * (12 + (key_tiles + s - 1) / s) * 32 + (s > 1 ? 5 * 32 + 3 * rest * s : 0);
         if (best == 0 || cost < best) {
