@@ -218,6 +218,20 @@ __device__ __forceinline__ void pa_tmem_store16(uint32_t address, const uint32_t
 
 __device__ __forceinline__ void pa_tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Nothing that uses `v` is moved ahead of this place.
+__device__ __forceinline__ void pa_tie(uint32_t (&v)[32]) {
+    asm volatile(""
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]),
+                   "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]),
+                   "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31]));
+}
+
+// The loads issued so far have arrived, `v`'s among them.
+__device__ __forceinline__ void pa_tmem_load_wait(uint32_t (&v)[32]) {
+    tmem_load_wait();
+    pa_tie(v);
+}
+
 __device__ __forceinline__ float pa_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -665,21 +679,15 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
             pa_wait(s_full + 8 * parity_group, phase, patience);
             tc_fence_after_sync();
             uint32_t raw[2][32];
-            if (!none) {
-                tmem_load_32x32(s_tmem, raw[0]);
-                tmem_load_32x32(s_tmem + 32, raw[1]);
-                tmem_load_wait();
-            }
-            tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(s_free + 8 * parity_group);
             float tile_max = -INFINITY;
-            if (!none) {
+            // D = 128: one half of the scores is scaled while the other one is on its way (80 us for the 32768 keys, both first 81.5; D = 256, where
+            // the scores' place is waited for: 188.5 and 187 us for the fifty-query chunks)
+            auto scaled = [&](int half) {
                 if (FP8) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
+                    for (int i = 8 * half; i < 8 * half + 8; ++i) {
                         const float4 ks = tile_scales[i];
-                        uint32_t* r = &raw[i >> 3][(i & 7) * 4];
+                        uint32_t* r = &raw[half][(i & 7) * 4];
                         const float2 a = __fmul2_rn(make_float2(__uint_as_float(r[0]), __uint_as_float(r[1])), make_float2(ks.x, ks.y));
                         const float2 c = __fmul2_rn(make_float2(__uint_as_float(r[2]), __uint_as_float(r[3])), make_float2(ks.z, ks.w));
                         r[0] = __float_as_uint(a.x); r[1] = __float_as_uint(a.y); r[2] = __float_as_uint(c.x); r[3] = __float_as_uint(c.y);
@@ -687,14 +695,32 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
                 }
                 if (!whole) {
 #pragma unroll
-                    for (int i = 0; i < 64; ++i)
-                        if (i >= valid) raw[i >> 5][i & 31] = __float_as_uint(-INFINITY);
+                    for (int i = 32 * half; i < 32 * half + 32; ++i)
+                        if (i >= valid) raw[half][i & 31] = __float_as_uint(-INFINITY);
                 }
                 float partial_max[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    partial_max[i & 3] = fmaxf(fmaxf(partial_max[i & 3], __uint_as_float(raw[0][i])), __uint_as_float(raw[1][i]));
-                tile_max = fmaxf(fmaxf(partial_max[0], partial_max[1]), fmaxf(partial_max[2], partial_max[3])) * factor;
+                for (int i = 0; i < 32; ++i) partial_max[i & 3] = fmaxf(partial_max[i & 3], __uint_as_float(raw[half][i]));
+                return fmaxf(fmaxf(partial_max[0], partial_max[1]), fmaxf(partial_max[2], partial_max[3]));
+            };
+            if (!none) {
+                tmem_load_32x32(s_tmem, raw[0]);
+                if (Shape::SHARED) tmem_load_32x32(s_tmem + 32, raw[1]);
+                pa_tmem_load_wait(raw[0]);
+                if (Shape::SHARED) {
+                    pa_tie(raw[1]);
+                } else {
+                    tmem_load_32x32(s_tmem + 32, raw[1]);
+                    tile_max = scaled(0);
+                    pa_tmem_load_wait(raw[1]);
+                }
+            }
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(s_free + 8 * parity_group);
+            if (!none) {
+                if (Shape::SHARED) tile_max = scaled(0);
+                tile_max = fmaxf(tile_max, scaled(1)) * factor;
             }
             // The reference follows the maximum lazily: it moves only when the maximum has grown by more than 2^8 since it was set, so
             // weights stay below 2^8 and the accumulator is rescaled a few times per row.  A row that has seen no key yet has none; 0
@@ -769,7 +795,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
                     for (int chunk = 0; chunk < D / 32; ++chunk) {
                         uint32_t o[32];
                         tmem_load_32x32(o_tmem + chunk * 32, o);
-                        tmem_load_wait();
+                        pa_tmem_load_wait(o);
 #pragma unroll
                         for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * correction);
                         pa_tmem_store(o_tmem + chunk * 32, o);
@@ -809,17 +835,19 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
             tmem_load_32x32(lane_address + Shape::TMEM_O + column, o[0]);
             if constexpr (Shape::SHARED) {
                 tmem_load_32x32(lane_address + Shape::TMEM_O + column + 32, o[1]);
-                tmem_load_wait();
+                pa_tmem_load_wait(o[0]);
+                pa_tie(o[1]);
 #pragma unroll
                 for (int i = 0; i < 64; ++i) o[i / 32][i % 32] = __float_as_uint(__uint_as_float(o[i / 32][i % 32]) * weight[0]);
             } else if (num_tiles > 1) {
                 uint32_t other[32];
                 tmem_load_32x32(lane_address + Shape::TMEM_O + D + column, other);
-                tmem_load_wait();
+                pa_tmem_load_wait(o[0]);
+                pa_tie(other);
 #pragma unroll
                 for (int i = 0; i < 32; ++i) o[0][i] = __float_as_uint(__uint_as_float(o[0][i]) * weight[0] + __uint_as_float(other[i]) * weight[1]);
             } else {
-                tmem_load_wait();
+                pa_tmem_load_wait(o[0]);
 #pragma unroll
                 for (int i = 0; i < 32; ++i) o[0][i] = __float_as_uint(__uint_as_float(o[0][i]) * weight[0]);
             }
