@@ -23,8 +23,8 @@
 //
 // Measured (B200; a tile is 64 keys for 128 rows, whose products alone are 500 cycles at D = 128 and 1000 at D = 256):
 //   fifty-query chunks of 64 members over 4 x 8192 bf16 keys, D = 256: 187 us (1150 TFLOP/s), 1430 cycles per tile
-//   64 members, one query, 32768 quantised keys, D = 128: 81 us, 1400 cycles per tile; without its exponentials 74, without its
-//   products 78, without the conversion of values 74: the chain of a softmax group -- scores out, maximum, exponentials, P in, each with
+//   64 members, one query, 32768 quantised keys, D = 128: 80 us, 1370 cycles per tile; of an earlier 83 without its exponentials 74,
+//   without its products 78, without the conversion of values 74: the chain of a softmax group -- scores out, maximum, exponentials, P in, each with
 //   its latency and two warps per scheduler to hide it -- and not one unit is what bounds the loop
 //   256 ten-query chunks over 32 x 712 quantised keys, D = 256: 41 us (in the groups' order 44): 176 row tiles of 12 key tiles on 148
 //   SMs, 21 k of a CTA's 41 k cycles before and behind the loop (4.8 k look-up, 3.6 k splitting Q, 5 k output)

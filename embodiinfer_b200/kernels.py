@@ -276,7 +276,7 @@ def rope_axes(positions: torch.Tensor, sections: tuple[int, ...], sine: torch.Te
     shape = positions.shape
     axes, half = shape[0], 0
     for section in sections:
-        if type(section) is not int or section <= 0:
+        if type(section) is not int or not 0 < section < 1 << 30:
             axes = -1
             break
         half += section
