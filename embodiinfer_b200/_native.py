@@ -149,6 +149,8 @@ _library: ctypes.CDLL | None = None
 def load() -> ctypes.CDLL:
     """Load the shared object once and declare every entry point's signature."""
     global _library
+    if _library is not None:
+        return _library
     with _lock:
         if _library is None:
             if not LIBRARY_PATH.exists():
