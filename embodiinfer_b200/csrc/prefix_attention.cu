@@ -344,7 +344,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
     int64_t* const row_output = row_query + PA_ROWS;                                                  // [128]: of its output
     float* const row_reference = reinterpret_cast<float*>(generic + Shape::OFF_ROWS);           // [2][128]: of the latest even and odd tile
     float* const row_exchange = row_reference + 2 * PA_ROWS;                                    // [2][128]: row maxima of Q, then the sums
-    int* const group_unit = reinterpret_cast<int*>(generic + Shape::OFF_BARS + 720);          // [2]: last units of the accumulators, as exponents
+    int* const group_unit = reinterpret_cast<int*>(generic + Shape::OFF_BARS + 728);          // [2]: last units of the accumulators, as exponents
     int* const segment_first = reinterpret_cast<int*>(generic + Shape::OFF_SEGMENTS);
     int* const segment_length = segment_first + PA_MAX_SEGMENTS + 3;
     const uint32_t bars = base + Shape::OFF_BARS;
@@ -357,7 +357,8 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
     const uint32_t reference_ready = bars + 512;                           // [4 quarters][2]
     const uint32_t all_done = bars + 576, q_ready = bars + 584, tmem_slot = bars + 592;
     PaWork* const work = reinterpret_cast<PaWork*>(generic + Shape::OFF_BARS + 608);
-    unsigned long long* const bad_keys = reinterpret_cast<unsigned long long*>(generic + Shape::OFF_BARS + 640);      // bf16: [STAGES]
+    unsigned long long* const bad_keys = reinterpret_cast<unsigned long long*>(generic + Shape::OFF_BARS + 664);      // bf16: [STAGES]
+    static_assert(sizeof(PaWork) <= 664 - 608 && 664 + STAGES * 8 <= 728, "places behind the barriers");
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
