@@ -42,7 +42,8 @@
 //   would, and no key is ever converted.  ks multiplies the score.
 //   Output.  The four value warps, two teams a tile apart, turn the codes into f16, exactly, and multiply by vs 2^-E: one rounding of 2^-11 for the scale and
 //   one for the product, beside the 2^-8 of the result.  2^E is the unit of the accumulator, the same for all rows: it follows the
-//   largest vs of a key tile when that leaves [2^-3, 2^6) units, and the accumulator is rescaled then as it is for a new reference.
+//   largest vs of a key tile when that leaves [2^-3, 2^6) units (2^-48 is the smallest), and the accumulator is rescaled then as it is for a
+//   new reference.
 //   A value is so off by at most 2^-10 of itself and, f16 ending at 2^-24 units, 2^-22 of the largest in its tile of 64 keys, whatever
 //   other tiles hold.  P is f16 as well: with its 11 bits the result is as exact as its own rounding allows (bf16 probabilities would
 //   add as much error again; two e4m3 halves, which would spare the conversion of V, have no room for a long tail of weights 2^-15
@@ -75,6 +76,7 @@ constexpr int PA_SCALE_STAGES = 4, PA_RAW_STAGES = 8;      // of the quantised c
 // A key tile's scales as the roles read them: ks, vs in units as pairs of halves, then bits of keys whose vs is not finite (2 words), the
 // unit, and the unit of the tile before less this one (exponents).
 constexpr int PA_SCALE_FLOATS = 2 * PA_KEYS + 4;
+constexpr int PA_UNIT_LEAST = -48;               // the smallest unit of the values, as an exponent
 constexpr int PA_MAX_SEGMENTS = PA_ROWS + 1;     // the prefix and at most one member per row
 
 template <int D, bool FP8>
@@ -1145,15 +1147,15 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
                     else largest = max(largest, bits);
                 }
                 largest = __reduce_max_sync(0xffffffffu, largest);
-                // the unit 2^E: kept unless the tile's largest scale is outside [2^-3, 2^6) of it (a tile of zeros fits any)
+                // the unit 2^E: kept unless the tile's largest scale is outside [2^-3, 2^6) of it (a tile of zeros fits any).  It may fall by any
+                // step: the limit below is what keeps the accumulator, which grows by the step, in fp32's range -- values below 2^40 with weights
+                // of at most 2^8 are below 2^96 of the smallest unit, times the number of keys.  Scales from 2^-59 on are still 2^-11 of
+                // it, normal numbers of f16.
                 const int exponent = int(largest >> 23) - 127, relative = exponent - unit_exponent;
                 int change = 0;
                 if (largest != 0u && (j == 0 || relative > 5 || relative < -3)) {
-                    int next = exponent < -60 ? -60 : (exponent > 60 ? 60 : exponent);
-                    if (j > 0) {
-                        next = next < unit_exponent - 60 ? unit_exponent - 60 : next;          // the accumulator grows by the step
-                        change = unit_exponent - next;
-                    }
+                    const int next = exponent < PA_UNIT_LEAST ? PA_UNIT_LEAST : (exponent > 60 ? 60 : exponent);
+                    if (j > 0) change = unit_exponent - next;
                     unit_exponent = next;
                 }
                 const float up = __uint_as_float(uint32_t(127 - unit_exponent) << 23);          // 2^-E
