@@ -38,7 +38,7 @@
 // Quantised cache (e4m3 codes, one fp32 scale per row: ks for keys, vs for values).
 //   Scores.  The codes go to the tensor core as they are (kind::f8f6f4).  Q is split into two e4m3 operands, q 2^e = hi + lo with
 //   2^e bringing the row's largest value into [128, 256): a bf16 value has 8 significant bits, hi takes 4 and lo the rest,
-//   exactly, down to 2^-17 of the row's largest value.  Two products at twice the bf16 rate cost what one bf16 product
+//   exactly, down to 2^-17 of the row's largest value (of 2^-119 in a row of smaller ones).  Two products at twice the bf16 rate cost what one bf16 product
 //   would, and no key is ever converted.  ks multiplies the score.
 //   Output.  The four value warps, two teams a tile apart, turn the codes into f16, exactly, and multiply by vs 2^-E: one rounding of 2^-11 for the scale and
 //   one for the product, beside the 2^-8 of the result.  2^E is the unit of the accumulator, the same for all rows: it follows the
@@ -617,9 +617,10 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
                 row_exchange[parity_group * PA_ROWS + row] = __uint_as_float(largest);
                 named_barrier<1, 256>();
                 largest = max(largest, __float_as_uint(row_exchange[(parity_group ^ 1) * PA_ROWS + row]));
-                // 2^e that brings the largest magnitude into [128, 256), kept a normal number
+                // 2^e that brings the largest magnitude into [128, 256); it and its reciprocal are normal numbers for every finite row from
+                // 2^-119 on
                 int exponent = int(largest >> 7) - 127;
-                exponent = exponent < -110 ? -110 : (exponent > 120 ? 120 : exponent);
+                exponent = exponent < -119 ? -119 : (exponent > 127 ? 127 : exponent);
                 const float up = largest == 0u ? 1.0f : __uint_as_float(uint32_t(127 + 7 - exponent) << 23);
                 const float down = largest == 0u ? 1.0f : __uint_as_float(uint32_t(127 - 7 + exponent) << 23);
                 // a row with an infinity or a NaN: every score is NaN

@@ -62,3 +62,23 @@ def test_small_values_behind_large_ones_of_no_weight(device, dim, exponents):
     want = (cache.v_codes.float().double() * cache.v_scales.double()[..., None])[0, 0, seen: seen + 64].mean(0)
     # all weights are 1: the result's rounding, the scale's and the product's to f16; sums of 64 positive fp32 numbers
     assert ((got.double() - want).abs() <= (2.0 ** -8 + 2 * 2.0 ** -11 + 2.0 ** -15) * want).all()
+
+
+@pytest.mark.parametrize("dim", [128, 256])
+@pytest.mark.parametrize("query,key,scale", [(126, -48, -78), (-124, 39, 85)])
+def test_queries_from_both_ends_of_the_range(device, dim, query, key, scale):
+    """Query rows whose largest values are at 2^query, behind quantised keys that bring the scores back to order 1.  The query is held
+    down to 2^-17 of its row's largest value, or of 2^-119 (2^-12 of 2^-124): the reference's bound with that in place of 2^-17."""
+    generator = torch.Generator(device=device).manual_seed(23)
+    draw = lambda *shape: 2.0 * torch.rand(shape, device=device, generator=generator) - 1.0
+    q = (draw(2, 8, 3, dim) * 2.0 ** (query + 1)).to(torch.bfloat16)
+    q[..., 0] = 1.5 * 2.0 ** query
+    cache = written(draw(1, 1, 100, dim) * 2.0 ** key, draw(1, 1, 100, dim))
+    factor = 0.25 * 2.0 ** scale
+    got = K.prefix_attention(q, cache, scale=factor)
+    want, bound = reference(q, cache, None, [0, 2], [100], [0, 0], False, factor)
+    if query < -119:
+        keys, values = (codes.float().double() * scales.double()[..., None] for codes, scales in ((cache.k_codes, cache.k_scales), (cache.v_codes, cache.v_scales)))
+        lost = 2.0 ** -12 * factor * float(q.double().abs().amax() * keys.abs().sum(-1).amax())
+        bound = bound + 2 * lost * float(values.abs().amax())
+    check(got, want, bound)
