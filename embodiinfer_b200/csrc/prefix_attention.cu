@@ -48,7 +48,8 @@
 //   other tiles hold.  P is f16 as well: with its 11 bits the result is as exact as its own rounding allows (bf16 probabilities would
 //   add as much error again; two e4m3 halves, which would spare the conversion of V, have no room for a long tail of weights 2^-15
 //   below the largest).
-//   A scale that is not finite zeroes its row of values and marks the key: rows that see it get NaN from their sum.
+//   A scale that is not finite zeroes its row of values and marks the key: rows that see it get NaN from their sum.  So do rows that see an
+//   own key with a NaN among its codes: those codes are zeroed as they are converted, and the first such key of each member is kept to the end.
 //
 // Row tiles that do not fill the device -- all of a small call's, or those of the last, partial wave -- have their key tiles cut across
 // several CTAs, which leave O, M and L in fp32 in the workspace; a second launch joins them in their order (no atomics: the result does
@@ -59,6 +60,7 @@
 #include <cuda.h>
 #include <cuda_fp16.h>
 
+#include <climits>
 #include <type_traits>
 
 namespace b2 {
@@ -109,7 +111,7 @@ struct PaShape {
     static constexpr uint32_t OFF_ROWS = OFF_RAW_SCALES + (FP8 ? PA_RAW_STAGES * 2 * PA_KEYS * 4 : 0);      // float [2][128], twice
     static constexpr uint32_t OFF_ROW_OFFSETS = OFF_ROWS + 4 * PA_ROWS * 4;          // int64 [2][128]
     static constexpr uint32_t OFF_SEGMENTS = OFF_ROW_OFFSETS + 2 * PA_ROWS * 8;
-    static constexpr uint32_t OFF_BARS = OFF_SEGMENTS + (PA_MAX_SEGMENTS + 3) * 8;
+    static constexpr uint32_t OFF_BARS = OFF_SEGMENTS + (PA_MAX_SEGMENTS + 3) * (FP8 ? 12 : 8);
     static constexpr int SHARED_BYTES = 1024 + int(OFF_BARS) + 768;
 };
 
@@ -263,15 +265,14 @@ __device__ __forceinline__ uint32_t float2_to_half2_bits(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&pair);
 }
 
-// Two e4m3 codes in the low half of `codes` -> two f16 of the values times `scale`.  CLEAN: codes that are NaN become 448, for tiles
-// with rows that some queries pass over with probability zero.
-template <bool CLEAN>
+// Two e4m3 codes in the low half of `codes` -> two f16 of the values times `scale`.
 __device__ __forceinline__ uint32_t codes_to_halves(uint32_t codes, __half2 scale) {
-    __half2 value(__nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(codes), __NV_E4M3));
-    if (CLEAN) value = __hmin2(value, __float2half2_rn(448.0f));
-    value = __hmul2(value, scale);
+    const __half2 value = __hmul2(__half2(__nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(codes), __NV_E4M3)), scale);
     return *reinterpret_cast<const uint32_t*>(&value);
 }
+
+// The bytes of `codes` that are e4m3 NaN (all magnitude bits set), as their top bits.
+__device__ __forceinline__ uint32_t codes_not_a_number(uint32_t codes) { return ((codes & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
 // Whether one of the two bf16 values of a word is an infinity or a NaN.
 __device__ __forceinline__ bool has_not_finite(uint32_t word) {
@@ -349,6 +350,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
     int* const group_unit = reinterpret_cast<int*>(generic + Shape::OFF_BARS + 728);          // [2]: last units of the accumulators, as exponents
     int* const segment_first = reinterpret_cast<int*>(generic + Shape::OFF_SEGMENTS);
     int* const segment_length = segment_first + PA_MAX_SEGMENTS + 3;
+    int* const segment_nan = segment_length + PA_MAX_SEGMENTS + 3;          // quantised: first of its own keys here whose value has a code that is NaN
     const uint32_t bars = base + Shape::OFF_BARS;
     constexpr int STAGES = Shape::STAGES;
     static_assert(STAGES <= 8, "barrier arrays");
@@ -510,6 +512,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
             if (s < segments) {
                 segment_first[s] = total + sum - mine;
                 segment_length[s] = length;
+                if (FP8) segment_nan[s] = INT_MAX;
             }
             total += __shfl_sync(0xffffffffu, sum, 31);
         }
@@ -818,6 +821,10 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
             __syncwarp();
             tc_fence_after_sync();
         }
+        if (FP8) {          // what the value warps have found: their last arrivals
+            for (int j = num_tiles > 2 ? num_tiles - 2 : 0; j < num_tiles; ++j) pa_wait(value_full + 8 * (j & 1), uint32_t(j >> 1) & 1u, patience);
+            if (my_segment > 0 && num_tiles > 0 && segment_nan[my_segment] < segment_length[my_segment] - hidden) running_sum = __uint_as_float(0x7fc00000u);
+        }
         row_reference[parity_group * PA_ROWS + row] = reference;      // what its last tile left there, or -inf
         row_exchange[parity_group * PA_ROWS + row] = running_sum;
         if (!Shape::SHARED && row == 0) group_unit[parity_group] = unit;
@@ -1059,13 +1066,17 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
             const int c = team, stage = j % PA_SCALE_STAGES, slot = j % STAGES;
             const uint32_t* value_scales = reinterpret_cast<const uint32_t*>(generic + Shape::OFF_SCALES) + stage * PA_SCALE_FLOATS + PA_KEYS;
             cursor.seek(start_tile + j);
-            // prefix keys are seen by every row: what is not finite among them may reach all
-            const bool clean = cursor.segment > 0 || cursor.keys(start_tile + j) < PA_KEYS;
+            // Prefix keys are seen by every row: a NaN among their codes may reach all.  A row with a NaN among own keys' codes is zero here,
+            // because the tile's other members' rows, and earlier queries, pass over it with probability zero; where it lies is kept for the
+            // rows that do see it.
+            const bool own = cursor.segment > 0;
+            const int valid = cursor.keys(start_tile + j), first_key = cursor.first_key(start_tile + j);
+            const bool plain = !own && valid == PA_KEYS;
             pa_wait(scale_full + 8 * stage, uint32_t(j / PA_SCALE_STAGES) & 1u, patience);
             pa_wait(v_full + 8 * slot, uint32_t(j / STAGES) & 1u, patience);
             pa_wait(value_empty + 8 * c, (uint32_t(j >> 1) & 1u) ^ 1u, patience);
             auto convert = [&](auto tag) {
-                constexpr bool CLEAN = decltype(tag)::value;
+                constexpr bool PLAIN = decltype(tag)::value;
 #pragma unroll 1
                 for (int first = thread; first < PA_KEYS * PIECES; first += BATCH * 32 * Shape::VALUE_TEAM) {
                     uint4 codes[BATCH];
@@ -1075,6 +1086,12 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
                         const uint32_t i = first + n * 32 * Shape::VALUE_TEAM, key = i / PIECES, piece = i % PIECES;
                         codes[n] = lds_u4(v_smem + slot * Shape::KV_BYTES + (piece >> 3) * Shape::KV_ATOM_BYTES + key * 128u + (((piece & 7u) ^ (key & 7u)) << 4));
                         scale_bits[n] = value_scales[key];
+                        if (!PLAIN) {
+                            const uint32_t nan = codes_not_a_number(codes[n].x) | codes_not_a_number(codes[n].y) | codes_not_a_number(codes[n].z) | codes_not_a_number(codes[n].w);
+                            const bool there = int(key) < valid, marked = there && own && nan != 0u;
+                            if (marked) atomicMin(segment_nan + cursor.segment, first_key + int(key));
+                            if (!there || marked) codes[n] = make_uint4(0u, 0u, 0u, 0u);
+                        }
                     }
 #pragma unroll
                     for (int n = 0; n < BATCH; ++n) {
@@ -1084,14 +1101,14 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
                         const uint32_t odd = (piece >> 2) & 1u, left = (piece & 3u) * 2u;
                         const uint32_t x = odd ? codes[n].z : codes[n].x, y = odd ? codes[n].w : codes[n].y;
                         const uint32_t z = odd ? codes[n].x : codes[n].z, w = odd ? codes[n].y : codes[n].w;
-                        sts_u4(group + (((left + odd) ^ swizzle) << 4), codes_to_halves<CLEAN>(x, scale), codes_to_halves<CLEAN>(x >> 16, scale),
-                               codes_to_halves<CLEAN>(y, scale), codes_to_halves<CLEAN>(y >> 16, scale));
-                        sts_u4(group + (((left + 1u - odd) ^ swizzle) << 4), codes_to_halves<CLEAN>(z, scale), codes_to_halves<CLEAN>(z >> 16, scale),
-                               codes_to_halves<CLEAN>(w, scale), codes_to_halves<CLEAN>(w >> 16, scale));
+                        sts_u4(group + (((left + odd) ^ swizzle) << 4), codes_to_halves(x, scale), codes_to_halves(x >> 16, scale),
+                               codes_to_halves(y, scale), codes_to_halves(y >> 16, scale));
+                        sts_u4(group + (((left + 1u - odd) ^ swizzle) << 4), codes_to_halves(z, scale), codes_to_halves(z >> 16, scale),
+                               codes_to_halves(w, scale), codes_to_halves(w >> 16, scale));
                     }
                 }
             };
-            if (clean) convert(std::true_type{});
+            if (plain) convert(std::true_type{});
             else convert(std::false_type{});
             fence_async_shared();
             __syncwarp();

@@ -305,7 +305,8 @@ int b2_kv_cache_read(const b2_kv_cache_desc* desc, void* stream);
  * members [members[g], members[g + 1]) of the batch (device int32[groups + 1], not decreasing, from 0 to batch; members that no
  * group holds get no output), or batch / groups each when `members` is NULL.  Lengths are clamped to their capacity.  What lies
  * behind a length is never used.  A key row that holds a NaN or an infinity gives NaN to the rows that see it, and to no other; so
- * do such own values (a whole output row) and quantised values; bf16 prefix values that are not finite follow IEEE arithmetic.
+ * do (a whole output row) own values that are not finite, an e4m3 NaN among them, and values whose scale is not finite; other
+ * prefix values that are not finite, bf16 or e4m3, follow IEEE arithmetic.
  * Scores, softmax statistics and outputs are held in fp32; probabilities enter the second product as bf16 (bf16 cache) or f16
  * (quantised cache; there q enters the first as two e4m3 halves that hold its 8 bits, and a value is off by at most 2^-10 of itself
  * and 2^-22 of the largest in its 64 keys).  head_dim 128 or 256.

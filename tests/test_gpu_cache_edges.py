@@ -7,7 +7,7 @@ import torch
 
 from embodiinfer_b200 import kernels as K
 from embodiinfer_b200.kv_cache import QuantizedKVCache
-from tests.test_gpu_prefix_attention import check, reference
+from tests.test_gpu_prefix_attention import check, make_cache, reference, whole
 
 pytestmark = pytest.mark.gpu
 
@@ -82,3 +82,56 @@ def test_queries_from_both_ends_of_the_range(device, dim, query, key, scale):
         lost = 2.0 ** -12 * factor * float(q.double().abs().amax() * keys.abs().sum(-1).amax())
         bound = bound + 2 * lost * float(values.abs().amax())
     check(got, want, bound)
+
+
+# ---- attention: values that are not finite ----------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dim", [128, 256])
+@pytest.mark.parametrize("which", ["k_codes", "v_codes"])
+@pytest.mark.parametrize("code", [0x7f, 0xff])
+def test_codes_that_are_nan_under_a_finite_scale(device, dim, which, code):
+    """An own key's reach the rows that see it, a prefix key's all rows (a value's: its column, in whole and partial key tiles alike);
+    those behind a length reach none."""
+    generator = torch.Generator(device=device).manual_seed(22)
+    q = torch.randn((3, 8, 4, dim), device=device, generator=generator).to(torch.bfloat16)
+    own = make_cache(generator, 3, 1, 20, dim, True, device)
+
+    def with_code(cache, b, position):
+        changed = cache._replace(**{which: getattr(cache, which).clone()})
+        getattr(changed, which).view(torch.uint8)[b, 0, position, 17] = code
+        return changed
+
+    for length in (30, 64, 100):
+        shared = make_cache(generator, 1, 1, 128, dim, True, device, [length])
+        shared.k_scales.nan_to_num_(1.0), shared.v_scales.nan_to_num_(1.0)          # behind the length: NaN codes, finite scales
+        run = lambda prefix, mine: K.prefix_attention(q, prefix, mine, causal=True, prefix_lengths=whole([length], device))
+        want = run(shared, own)
+        assert not want.isnan().any()
+        for position in (5, 19):
+            got = run(shared, with_code(own, 1, position))
+            touched = torch.zeros((3, 8, 4), device=device, dtype=torch.bool)
+            touched[1, :, max(0, position - 16):] = True          # causal: query t sees 17 + t own keys
+            assert got[touched].isnan().all() and torch.equal(got[~touched], want[~touched])
+        for position in (3, length - 1):
+            got = run(with_code(shared, 0, position), own)
+            if which == "k_codes":
+                assert got.isnan().all()
+            else:
+                others = torch.arange(dim, device=device) != 17
+                assert got[..., 17].isnan().all() and torch.equal(got[..., others], want[..., others])
+
+
+def test_codes_that_are_nan_in_cut_launches_and_many_members(device):
+    """One row tile of 128 members, and keys cut across SMs: only the rows of the member with the NaN are touched."""
+    generator = torch.Generator(device=device).manual_seed(25)
+    for members, heads, own_keys, position in ((128, 1, 70, 69), (3, 8, 3000, 2500)):
+        q = torch.randn((members, heads, 1, 128), device=device, generator=generator).to(torch.bfloat16)
+        own = make_cache(generator, members, 1, own_keys, 128, True, device)
+        want = K.prefix_attention(q, no_keys(own), own)
+        changed = own._replace(v_codes=own.v_codes.clone())
+        changed.v_codes.view(torch.uint8)[1, 0, position, 100] = 0x7f
+        got = K.prefix_attention(q, no_keys(own), changed)
+        assert got[1].isnan().all() and torch.equal(got[[0, *range(2, members)]], want[[0, *range(2, members)]])
+        seen = K.prefix_attention(q, no_keys(own), changed, own_lengths=whole([position] * members, device))
+        assert torch.equal(seen, K.prefix_attention(q, no_keys(own), own, own_lengths=whole([position] * members, device)))
