@@ -45,9 +45,9 @@
 //   largest vs of a key tile when that leaves [2^-3, 2^6) units (2^-48 is the smallest), and the accumulator is rescaled then as it is for a
 //   new reference.
 //   A value is so off by at most 2^-10 of itself and, f16 ending at 2^-24 units, 2^-22 of the largest in its tile of 64 keys, whatever
-//   other tiles hold.  P is f16 as well: with its 11 bits the result is as exact as its own rounding allows (bf16 probabilities would
-//   add as much error again; two e4m3 halves, which would spare the conversion of V, have no room for a long tail of weights 2^-15
-//   below the largest).
+//   other tiles hold.  P is f16 as well, down to 2^-31 of the reference's weight: with its 11 bits the result is as exact as its own rounding
+//   allows (bf16 probabilities would add as much error again; two e4m3 halves, which would spare the conversion of V, have no room for a long
+//   tail of weights 2^-15 below the largest).
 //   A scale that is not finite zeroes its row of values and marks the key: rows that see it get NaN from their sum.  So do rows that see an
 //   own key with a NaN among its codes: those codes are zeroed as they are converted, and the first such key of each member is kept to the end.
 //
@@ -78,6 +78,10 @@ constexpr int PA_SCALE_STAGES = 4, PA_RAW_STAGES = 8;      // of the quantised c
 // A key tile's scales as the roles read them: ks, vs in units as pairs of halves, then bits of keys whose vs is not finite (2 words), the
 // unit, and the unit of the tile before less this one (exponents).
 constexpr int PA_SCALE_FLOATS = 2 * PA_KEYS + 4;
+// Weights and their sums are held 2^7 times as large where P is f16 (they stay below 2^15): its smallest number, 2^-24, is then 2^-31 of the
+// reference's weight, and a tail of 2^19 keys with weights of 2^-25 each, a hundredth of the sum, is there.  bf16 has fp32's range.
+template <bool FP8>
+constexpr float PA_WEIGHT_BITS = FP8 ? 7.0f : 0.0f;
 constexpr int PA_UNIT_LEAST = -48;               // the smallest unit of the values, as an exponent
 constexpr int PA_MAX_SEGMENTS = PA_ROWS + 1;     // the prefix and at most one member per row
 
@@ -730,7 +734,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
                 tile_max = fmaxf(tile_max, scaled(1)) * factor;
             }
             // The reference follows the maximum lazily: it moves only when the maximum has grown by more than 2^8 since it was set, so
-            // weights stay below 2^8 and the accumulator is rescaled a few times per row.  A row that has seen no key yet has none; 0
+            // weights stay within 2^8 of its and the accumulator is rescaled a few times per row.  A row that has seen no key yet has none; 0
             // stands in, its weights are 0.  With one accumulator the reference of the tile before comes from the other group.
             float previous = reference;
             if (Shape::SHARED && j > 0) {
@@ -767,7 +771,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
 #pragma unroll
                 for (int i = 0; i < 32; ++i) packed[i] = 0u;
             } else {
-                const float shift = now == -INFINITY ? 0.0f : -now;
+                const float shift = now == -INFINITY ? 0.0f : PA_WEIGHT_BITS<FP8> - now;
                 const float2 shift2 = make_float2(shift, shift), factor2 = make_float2(factor, factor);
                 float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
@@ -1167,7 +1171,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
                 largest = __reduce_max_sync(0xffffffffu, largest);
                 // the unit 2^E: kept unless the tile's largest scale is outside [2^-3, 2^6) of it (a tile of zeros fits any).  It may fall by any
                 // step: the limit below is what keeps the accumulator, which grows by the step, in fp32's range -- values below 2^40 with weights
-                // of at most 2^8 are below 2^96 of the smallest unit, times the number of keys.  Scales from 2^-59 on are still 2^-11 of
+                // of at most 2^15 are below 2^103 of the smallest unit, times the number of keys (2^24 of them, all at both ends).  Scales from 2^-59 on are still 2^-11 of
                 // it, normal numbers of f16.
                 const int exponent = int(largest >> 23) - 127, relative = exponent - unit_exponent;
                 int change = 0;

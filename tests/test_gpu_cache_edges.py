@@ -84,6 +84,26 @@ def test_queries_from_both_ends_of_the_range(device, dim, query, key, scale):
     check(got, want, bound)
 
 
+@pytest.mark.parametrize("dim", [128, 256])
+def test_a_long_tail_of_small_weights(device, dim):
+    """One key of value 0 and weight 1, 2^19 of value 1 and weight e^-8 to e^-20, a part of the result from 0.99 to 0.001.  Beside the result's
+    rounding: weights in f16 off by 2^-11 of themselves and 2^-32 of the largest, the exponential by 2^-22 (20 + 1), the
+    weights' sum in fp32 over 2^13 tiles by 2^-24 of itself each, and the accumulator, which takes 16 keys at a time: 2^15 additions, each off
+    by at most a step (the tensor core's rounding is not specified), 2^-23 of a sum that grows evenly, half of the last one on average:
+    2^15 2^-23 / 2.  Rows for every SM, so that one CTA walks all keys."""
+    count, rows = 1 << 19, 128 * torch.cuda.get_device_properties(device).multi_processor_count
+    codes = lambda: torch.zeros((1, 1, count, dim), device=device, dtype=torch.uint8)
+    k, v, scales = codes(), codes(), torch.ones((1, 1, count), device=device)
+    k[0, 0, 1:, 0], v[0, 0, 1:] = 0xb8, 0x38          # -1 and 1
+    q = torch.zeros((1, rows, 1, dim), device=device, dtype=torch.bfloat16)
+    q[..., 0] = torch.linspace(8.0, 20.0, rows, device=device).to(torch.bfloat16)[:, None]
+    got = K.prefix_attention(q, QuantizedKVCache(k, scales, v, scales), scale=1.0)
+    tail = (count - 1) * torch.exp(-q[..., :1].double())
+    want = (tail / (1.0 + tail)).expand_as(got)
+    bound = (2.0 ** -8 + 2.0 ** -11 + 2.0 ** -22 * 21 + 2.0 ** 13 * 2.0 ** -24 + 2.0 ** 15 * 2.0 ** -23 / 2) * want + count * 2.0 ** -32 / (1.0 + tail)
+    check(got, want, bound)
+
+
 # ---- attention: values that are not finite ----------------------------------------------------------------
 
 
