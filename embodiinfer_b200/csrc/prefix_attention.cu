@@ -828,6 +828,8 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
         if (FP8) {          // what the value warps have found: their last arrivals
             for (int j = num_tiles > 2 ? num_tiles - 2 : 0; j < num_tiles; ++j) pa_wait(value_full + 8 * (j & 1), uint32_t(j >> 1) & 1u, patience);
             if (my_segment > 0 && num_tiles > 0 && segment_nan[my_segment] < segment_length[my_segment] - hidden) running_sum = __uint_as_float(0x7fc00000u);
+            // a query that is not finite makes NaN of masked scores too: a row that sees no key is zero all the same
+            if (segment_length[0] == 0 && (my_segment < 0 || segment_length[my_segment] <= hidden)) running_sum = 0.0f;
         }
         row_reference[parity_group * PA_ROWS + row] = reference;      // what its last tile left there, or -inf
         row_exchange[parity_group * PA_ROWS + row] = running_sum;

@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -155,3 +157,21 @@ def test_codes_that_are_nan_in_cut_launches_and_many_members(device):
         assert got[1].isnan().all() and torch.equal(got[[0, *range(2, members)]], want[[0, *range(2, members)]])
         seen = K.prefix_attention(q, no_keys(own), changed, own_lengths=whole([position] * members, device))
         assert torch.equal(seen, K.prefix_attention(q, no_keys(own), own, own_lengths=whole([position] * members, device)))
+
+
+@pytest.mark.parametrize("quantised", [False, True])
+@pytest.mark.parametrize("dim", [128, 256])
+@pytest.mark.parametrize("own_keys", [9, 2000])          # 2000: cut across SMs
+def test_a_query_that_is_not_finite_and_sees_no_key(device, dim, quantised, own_keys):
+    """Members of one row tile: the one without keys is zero, whatever its queries hold."""
+    generator = torch.Generator(device=device).manual_seed(24)
+    q = torch.randn((3, 8, 2, dim), device=device, generator=generator).to(torch.bfloat16)
+    want_q = q.clone()
+    q[1, 3, 0, 7], q[1, 4, 1, 7] = math.nan, math.inf
+    own = make_cache(generator, 3, 1, own_keys, dim, quantised, device)
+    lengths = whole([own_keys, 0, 3], device)
+    got, want = (K.prefix_attention(queries, no_keys(own), own, own_lengths=lengths) for queries in (q, want_q))
+    assert not got[1].any() and not got.isnan().any() and torch.equal(got, want)
+    causal = K.prefix_attention(q, no_keys(own), own, own_lengths=whole([own_keys, 1, 3], device), causal=True)          # query 0 sees nothing
+    assert not causal[1, :, 0].any() and not causal[[0, 2]].isnan().any()
+    assert causal[1, 4, 1].isnan().all() or not quantised          # bf16: its one score is an infinity of either sign
