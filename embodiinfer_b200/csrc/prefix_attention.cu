@@ -128,7 +128,8 @@ struct PaArgs {
     const int32_t* prefix_lengths;    // or nullptr: the capacity
     const int32_t* own_lengths;
     float* partial;                   // O [slots][128][D], then (M, L) [slots][128][2]
-    int64_t* row_offsets;             // of the row tiles that are cut: element offset of each row's output, -1 for rows that do not exist [slots / 2][128]
+    int64_t* row_offsets;             // of the row tiles that are cut: element offset of each row's output, + 1 if it sees a key; -1 for rows that do not
+                                      // exist [slots / 2][128]
     int32_t* cut;                     // [2], 8-byte aligned: how many row tiles are cut, and into how many parts each
     unsigned int* status;
     int64_t q_stride[3];
@@ -825,11 +826,12 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
             __syncwarp();
             tc_fence_after_sync();
         }
+        const bool sees = segment_length[0] > 0 || (my_segment > 0 && segment_length[my_segment] > hidden);          // a key, anywhere
         if (FP8) {          // what the value warps have found: their last arrivals
             for (int j = num_tiles > 2 ? num_tiles - 2 : 0; j < num_tiles; ++j) pa_wait(value_full + 8 * (j & 1), uint32_t(j >> 1) & 1u, patience);
             if (my_segment > 0 && num_tiles > 0 && segment_nan[my_segment] < segment_length[my_segment] - hidden) running_sum = __uint_as_float(0x7fc00000u);
             // a query that is not finite makes NaN of masked scores too: a row that sees no key is zero all the same
-            if (segment_length[0] == 0 && (my_segment < 0 || segment_length[my_segment] <= hidden)) running_sum = 0.0f;
+            if (!sees) running_sum = 0.0f;
         }
         row_reference[parity_group * PA_ROWS + row] = reference;      // what its last tile left there, or -inf
         row_exchange[parity_group * PA_ROWS + row] = running_sum;
@@ -873,12 +875,14 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
         const bool stored = w.splits == 1;
         const int64_t first_partial = int64_t(w.place) * PA_ROWS;
         if (!stored && parity_group == 0) {
-            if (w.split == 0) args.row_offsets[first_partial + row] = row_output[row];
+            if (w.split == 0) args.row_offsets[first_partial + row] = exists ? row_output[row] | int64_t(sees) : -1;
             if (exists) *reinterpret_cast<float2*>(args.partial + int64_t(args.slots) * PA_ROWS * D + (first_partial + row) * 2) = make_float2(reference, running_sum);
         }
         // Rows go out through shared memory (the rings are empty now), a bulk copy for each: a thread has a row of the accumulator, and its
         // own stores would touch a sector at a time.  16 bytes between rows spread them over the banks.
-        const float inverse = stored ? (running_sum == 0.0f ? 0.0f : 1.0f / running_sum) : 1.0f;          // sum 0: the row sees no key
+        // sum 0: the row sees no key, or (IEEE arithmetic: NaN) none whose score is above -inf
+        if (stored && sees && running_sum == 0.0f) running_sum = __uint_as_float(0x7fc00000u);
+        const float inverse = stored ? (running_sum == 0.0f ? 0.0f : 1.0f / running_sum) : 1.0f;
         const uint32_t row_bytes = stored ? D * 2 : D * 4, out_row = base + uint32_t(row) * (row_bytes + 16);
         constexpr int BATCH = Shape::SHARED ? 2 : 1;          // of 32 columns
 #pragma unroll 1
@@ -1224,11 +1228,11 @@ __global__ void __launch_bounds__(256) prefix_attention_join_kernel(const __grid
     const int lane = threadIdx.x % LANES;
     pdl_wait();
     const int2 cut = *reinterpret_cast<const int2*>(args.cut);
-    const int64_t offset = args.row_offsets[index];          // inside the table, whatever the cut
+    const int64_t offset_and_sees = args.row_offsets[index], offset = offset_and_sees & ~int64_t(1);          // inside the table, whatever the cut
     const int64_t rows = int64_t(cut.x) * PA_ROWS;
     const int splits = cut.y;
     if (rows == 0) return;
-    const bool there = index < rows && offset >= 0;          // lanes without a row stay for the shuffles, on a row that is there
+    const bool there = index < rows && offset_and_sees >= 0;          // lanes without a row stay for the shuffles, on a row that is there
     const int64_t row = index < rows ? index : 0;
     const float2* statistics = reinterpret_cast<const float2*>(args.partial + int64_t(args.slots) * PA_ROWS * D) + row;
     const float* partial = args.partial + row * D + lane * 8;
@@ -1281,7 +1285,7 @@ __global__ void __launch_bounds__(256) prefix_attention_join_kernel(const __grid
         }
     }
     if (!there) return;
-    const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+    const float inverse = total == 0.0f ? ((offset_and_sees & 1) != 0 ? __uint_as_float(0x7fc00000u) : 0.0f) : 1.0f / total;
     *reinterpret_cast<uint4*>(args.out + offset + lane * 8) =
         make_uint4(float2_to_bf16x2(make_float2(sum[0] * inverse, sum[1] * inverse)), float2_to_bf16x2(make_float2(sum[2] * inverse, sum[3] * inverse)),
                    float2_to_bf16x2(make_float2(sum[4] * inverse, sum[5] * inverse)), float2_to_bf16x2(make_float2(sum[6] * inverse, sum[7] * inverse)));

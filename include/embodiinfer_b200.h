@@ -304,9 +304,11 @@ int b2_kv_cache_read(const b2_kv_cache_desc* desc, void* stream);
  * [batch, kv_heads, own_capacity, head_dim], contiguous; one of the capacities may be 0 (its pointers NULL).  Group g has the
  * members [members[g], members[g + 1]) of the batch (device int32[groups + 1], not decreasing, from 0 to batch; members that no
  * group holds get no output), or batch / groups each when `members` is NULL.  Lengths are clamped to their capacity.  What lies
- * behind a length is never used.  A key row that holds a NaN or an infinity gives NaN to the rows that see it, and to no other; so
- * do (a whole output row) own values that are not finite, an e4m3 NaN among them, and values whose scale is not finite; other
- * prefix values that are not finite, bf16 or e4m3, follow IEEE arithmetic.
+ * behind a length is never used.  Scores that are not finite follow IEEE arithmetic: a key whose score is NaN or +infinity gives NaN to
+ * the rows that see it, and to no other; one whose score is -infinity has no weight, and a row that sees only such keys is NaN.  (A
+ * query row with a NaN or an infinity has NaN scores over a quantised cache.)  Own values that are not finite, an e4m3 NaN among
+ * them, and values whose scale is not finite give NaN to the whole output rows that see them; other prefix values that are not
+ * finite, bf16 or e4m3, follow IEEE arithmetic.
  * Scores, softmax statistics and outputs are held in fp32; probabilities enter the second product as bf16 (bf16 cache) or f16
  * (quantised cache; there q enters the first as two e4m3 halves that hold its 8 bits, and a value is off by at most 2^-10 of itself
  * and 2^-22 of the largest in its 64 keys).  head_dim 128 or 256.

@@ -175,3 +175,27 @@ def test_a_query_that_is_not_finite_and_sees_no_key(device, dim, quantised, own_
     causal = K.prefix_attention(q, no_keys(own), own, own_lengths=whole([own_keys, 1, 3], device), causal=True)          # query 0 sees nothing
     assert not causal[1, :, 0].any() and not causal[[0, 2]].isnan().any()
     assert causal[1, 4, 1].isnan().all() or not quantised          # bf16: its one score is an infinity of either sign
+
+
+@pytest.mark.parametrize("quantised", [False, True])
+@pytest.mark.parametrize("dim", [128, 256])
+@pytest.mark.parametrize("own_keys", [20, 2500])          # 2500: cut across SMs
+def test_scores_of_minus_infinity(device, dim, quantised, own_keys):
+    """A key whose score is -inf has no weight; a row that sees no other is NaN, one that sees no key at all zero."""
+    generator = torch.Generator(device=device).manual_seed(26)
+    q = torch.rand((4, 8, 2, dim), device=device, generator=generator).add(0.5).to(torch.bfloat16)
+    own = make_cache(generator, 4, 1, own_keys, dim, quantised, device)
+    def sink(b, keys):          # all channels negative and one, or the scale, infinite: -inf for these queries
+        if quantised:
+            own.k_codes.view(torch.uint8)[b, 0, keys] = 0xb8
+            own.k_scales[b, 0, keys] = math.inf
+        else:
+            own[0][b, 0, keys] = -1.0
+            own[0][b, 0, keys, 5] = -math.inf
+    sink(0, own_keys - 1), sink(1, slice(None)), sink(2, slice(None))
+    run = lambda *lengths: K.prefix_attention(q, no_keys(own), own, own_lengths=whole(lengths, device))
+    got = run(own_keys, own_keys, 0, own_keys)
+    assert torch.equal(got[[0, 3]], run(own_keys - 1, own_keys, 0, own_keys)[[0, 3]])          # (the same key tiles)
+    assert not got[[0, 3]].isnan().any()
+    assert got[1].isnan().all() and not got[2].any()
+    assert run(own_keys, 1, 1, own_keys)[1:3].isnan().all()
