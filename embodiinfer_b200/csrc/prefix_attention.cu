@@ -83,6 +83,7 @@ constexpr int PA_SCALE_FLOATS = 2 * PA_KEYS + 4;
 template <bool FP8>
 constexpr float PA_WEIGHT_BITS = FP8 ? 7.0f : 0.0f;
 constexpr int PA_UNIT_LEAST = -48;               // the smallest unit of the values, as an exponent
+constexpr uint32_t PA_SCALE_END = 0x4f800000u;   // 2^32: value scales from here on, which no write leaves, count as not finite; f16 could not hold them in any unit
 constexpr int PA_MAX_SEGMENTS = PA_ROWS + 1;     // the prefix and at most one member per row
 
 template <int D, bool FP8>
@@ -1170,8 +1171,8 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
                 for (int i = 0; i < 2; ++i) {
                     vs[i] = raw[PA_KEYS + 32 * i];
                     const uint32_t bits = __float_as_uint(vs[i]) & 0x7fffffffu;
-                    not_finite[i] = __ballot_sync(0xffffffffu, bits >= 0x7f800000u);
-                    if (bits >= 0x7f800000u) vs[i] = 0.0f;
+                    not_finite[i] = __ballot_sync(0xffffffffu, bits >= PA_SCALE_END);
+                    if (bits >= PA_SCALE_END) vs[i] = 0.0f;
                     else largest = max(largest, bits);
                 }
                 largest = __reduce_max_sync(0xffffffffu, largest);
@@ -1182,7 +1183,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
                 const int exponent = int(largest >> 23) - 127, relative = exponent - unit_exponent;
                 int change = 0;
                 if (largest != 0u && (j == 0 || relative > 5 || relative < -3)) {
-                    const int next = exponent < PA_UNIT_LEAST ? PA_UNIT_LEAST : (exponent > 60 ? 60 : exponent);
+                    const int next = exponent < PA_UNIT_LEAST ? PA_UNIT_LEAST : exponent;
                     if (j > 0) change = unit_exponent - next;
                     unit_exponent = next;
                 }

@@ -307,8 +307,8 @@ int b2_kv_cache_read(const b2_kv_cache_desc* desc, void* stream);
  * behind a length is never used.  Scores that are not finite follow IEEE arithmetic: a key whose score is NaN or +infinity gives NaN to
  * the rows that see it, and to no other; one whose score is -infinity has no weight, and a row that sees only such keys is NaN.  (A
  * query row with a NaN or an infinity has NaN scores over a quantised cache.)  Own values that are not finite, an e4m3 NaN among
- * them, and values whose scale is not finite give NaN to the whole output rows that see them; other prefix values that are not
- * finite, bf16 or e4m3, follow IEEE arithmetic.
+ * them, and values whose scale is not finite (or 2^32 and more, which no write leaves) give NaN to the whole output rows that see
+ * them; other prefix values that are not finite, bf16 or e4m3, follow IEEE arithmetic.
  * Scores, softmax statistics and outputs are held in fp32; probabilities enter the second product as bf16 (bf16 cache) or f16
  * (quantised cache; there q enters the first as two e4m3 halves that hold its 8 bits, and a value is off by at most 2^-10 of itself
  * and 2^-22 of the largest in its 64 keys).  head_dim 128 or 256.

@@ -199,3 +199,21 @@ def test_scores_of_minus_infinity(device, dim, quantised, own_keys):
     assert not got[[0, 3]].isnan().any()
     assert got[1].isnan().all() and not got[2].any()
     assert run(own_keys, 1, 1, own_keys)[1:3].isnan().all()
+
+
+@pytest.mark.parametrize("dim", [128, 256])
+def test_value_scales_that_no_write_leaves(device, dim):
+    """2^32 and more count as not finite; 2^31 is a scale like any other."""
+    generator = torch.Generator(device=device).manual_seed(27)
+    q = torch.randn((3, 8, 4, dim), device=device, generator=generator).to(torch.bfloat16)
+    own = make_cache(generator, 3, 1, 20, dim, True, device)
+    own.v_codes.view(torch.uint8)[1, 0, 5, ::2] = 0
+    want = K.prefix_attention(q, no_keys(own), own)
+    for exponent in (31, 32, 70, 127):
+        changed = own._replace(v_scales=own.v_scales.clone())
+        changed.v_scales[1, 0, 5] = 2.0 ** exponent
+        got = K.prefix_attention(q, no_keys(own), changed)
+        if exponent < 32:
+            check(got, *reference(q, no_keys(own), changed, [0, 3], [0], [20] * 3, False, dim ** -0.5))
+        else:
+            assert got[1].isnan().all() and torch.equal(got[[0, 2]], want[[0, 2]])
