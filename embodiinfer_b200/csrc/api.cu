@@ -207,9 +207,11 @@ int b2_rope_axes(const void* positions, int32_t position_bytes, const int32_t* s
                                 cosine, static_cast<cudaStream_t>(stream));
 }
 
-static bool strides_valid(const int64_t (&stride)[3]) {
-    for (const int64_t s : stride)
-        if (s < 0 || (s & 7) != 0 || s > (int64_t(1) << 40)) return false;
+// Strides of 16-byte rows; along an extent of 1 there is no step to take.
+static bool strides_valid(const int64_t (&stride)[3], int32_t batch, int32_t heads, int32_t tokens) {
+    const int32_t extents[3] = {batch, heads, tokens};
+    for (int i = 0; i < 3; ++i)
+        if (stride[i] < 0 || (extents[i] > 1 && ((stride[i] & 7) != 0 || stride[i] > (int64_t(1) << 40)))) return false;
     return true;
 }
 
@@ -226,7 +228,9 @@ static int check_kv_cache(const b2_kv_cache_desc* desc) {
     const void* words[] = {desc->k_scales, desc->v_scales, desc->offsets, desc->lengths};
     for (const void* pointer : words)
         if (!is_aligned(pointer, 4)) return B2_E_INVALID;
-    if (!strides_valid(desc->k_stride) || !strides_valid(desc->v_stride)) return B2_E_INVALID;
+    if (!strides_valid(desc->k_stride, desc->batch, desc->kv_heads, desc->tokens) ||
+        !strides_valid(desc->v_stride, desc->batch, desc->kv_heads, desc->tokens))
+        return B2_E_INVALID;
     const int64_t heads = desc->q == nullptr ? 0 : desc->heads, limit = (int64_t(1) << 31) - 1;
     if (heads > limit / 4 || desc->kv_heads > limit / 4) return B2_E_TOO_LARGE;
     if (int64_t(desc->batch) * desc->tokens > limit / (heads + 2 * int64_t(desc->kv_heads))) return B2_E_TOO_LARGE;
@@ -237,7 +241,7 @@ int b2_kv_cache_write(const b2_kv_cache_desc* desc, void* stream) {
     const int status = check_kv_cache(desc);
     if (status != B2_OK) return status;
     if ((desc->q == nullptr) != (desc->q_out == nullptr) || (desc->sine == nullptr) != (desc->cosine == nullptr)) return B2_E_INVALID;
-    if (desc->q != nullptr && (desc->heads <= 0 || !strides_valid(desc->q_stride))) return B2_E_INVALID;
+    if (desc->q != nullptr && (desc->heads <= 0 || !strides_valid(desc->q_stride, desc->batch, desc->heads, desc->tokens))) return B2_E_INVALID;
     if (desc->factor_batch_stride < 0 || (desc->factor_batch_stride & 3) != 0) return B2_E_INVALID;
     return b2::launch_kv_cache_write(desc, static_cast<cudaStream_t>(stream));
 }
@@ -288,7 +292,7 @@ int b2_prefix_attention(const b2_prefix_attention_desc* desc, void* stream) {
                            desc->prefix_lengths, desc->own_lengths, desc->status};
     for (const void* pointer : words)
         if (!is_aligned(pointer, 4)) return B2_E_INVALID;
-    if (!strides_valid(desc->q_stride) || !is_aligned(desc->workspace, 32)) return B2_E_INVALID;
+    if (!strides_valid(desc->q_stride, desc->batch, desc->heads, desc->queries) || !is_aligned(desc->workspace, 32)) return B2_E_INVALID;
     return b2::launch_prefix_attention(desc, static_cast<cudaStream_t>(stream));
 }
 

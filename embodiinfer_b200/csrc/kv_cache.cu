@@ -261,7 +261,8 @@ int launch_kv_cache_write(const b2_kv_cache_desc* desc, cudaStream_t stream) {
 int launch_kv_cache_read(const b2_kv_cache_desc* desc, cudaStream_t stream) {
     CacheArgs args = cache_args(desc);
     args.wide = ((reinterpret_cast<uintptr_t>(desc->k) | reinterpret_cast<uintptr_t>(desc->v)) & 31u) == 0;
-    for (int i = 0; i < 3; ++i) args.wide = args.wide && (desc->k_stride[i] | desc->v_stride[i]) % 16 == 0;
+    const int32_t extents[3] = {desc->batch, desc->kv_heads, desc->tokens};
+    for (int i = 0; i < 3; ++i) args.wide = args.wide && (extents[i] == 1 || (desc->k_stride[i] | desc->v_stride[i]) % 16 == 0);
     const int64_t rows = int64_t(args.batch) * args.kv_heads * args.tokens;
     const int64_t block_rows = CACHE_THREADS / (desc->head_dim / 16);
     // as in the write: four rows per thread once the launch fills the device with them

@@ -271,7 +271,8 @@ int b2_rope_axes(const void* positions, int32_t position_bytes, const int32_t* s
  * Two tokens of one call that fall on one position (only possible by overlapping sequences' memory) are not ordered.
  * b2_kv_cache_read: writes bf16(code * scale) of position offsets[b] + t to row t of `k`, `v` (any strides of at least head_dim, where
  * there is more than one row along them).  q, q_out, sine and cosine must be NULL.
- * All pointers 16-byte aligned (scales, offsets and lengths: 4), strides multiples of 8 elements and not negative, and
+ * All pointers 16-byte aligned (scales, offsets and lengths: 4), strides not negative and, where there is more than one row along them,
+ * multiples of 8 elements, and
  * batch * tokens * (heads + 2 kv_heads) < 2^31.  The reference has no quantised cache. */
 typedef struct b2_kv_cache_desc {
     const void* q;          /* bf16 or NULL */
@@ -335,7 +336,7 @@ typedef struct b2_prefix_attention_desc {
     void* status;
     void* workspace;
     int64_t workspace_bytes;
-    int64_t q_stride[3];         /* elements between batch entries, heads, queries: multiples of 8, not negative */
+    int64_t q_stride[3];         /* elements between batch entries, heads, queries: not negative, multiples of 8 where there are several */
     float scale;                 /* finite, > 0 */
     int32_t flags;               /* B2_ATTENTION_CAUSAL; any other bit: B2_E_INVALID */
     int32_t batch, groups, heads, kv_heads, queries, head_dim, prefix_capacity, own_capacity, cache_bits;

@@ -1,0 +1,23 @@
+"""Edges of the cache operators' checks, at the C ABI and in the wrappers.  No kernel is launched here."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+
+from embodiinfer_b200 import _native as N
+from tests.test_kv_cache import _cache_desc
+
+MOST = (1 << 31) - 1
+
+
+@pytest.mark.parametrize("changes", [dict(batch=1, tokens=MOST, k_stride=(3, 128, 128), v_stride=(1 << 50, 128, 128)),
+                                     dict(batch=1 << 20, tokens=1 << 11, k_stride=(768, 5, 128)), dict(batch=MOST, tokens=1, v_stride=(256, 128, 1))])
+def test_strides_count_only_where_there_are_steps(changes):
+    """A stride along an extent of 1 is not looked at: these calls are refused for their size alone, which is looked at behind the strides.
+    Along an extent of 2 the same strides are refused."""
+    grown = {**changes, **{name: max(2, changes.get(name, 0)) for name in ("batch", "tokens")}, "kv_heads": 2}
+    for call in (N.load().b2_kv_cache_write, N.load().b2_kv_cache_read):
+        assert call(ctypes.byref(_cache_desc(**changes)), None) == N.E_TOO_LARGE
+        assert call(ctypes.byref(_cache_desc(**grown)), None) == N.E_INVALID

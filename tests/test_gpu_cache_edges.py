@@ -217,3 +217,29 @@ def test_value_scales_that_no_write_leaves(device, dim):
             check(got, *reference(q, no_keys(own), changed, [0, 3], [0], [20] * 3, False, dim ** -0.5))
         else:
             assert got[1].isnan().all() and torch.equal(got[[0, 2]], want[[0, 2]])
+
+
+# ---- layouts ----------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dim", [128, 256])
+def test_any_stride_along_an_extent_of_one(device, dim):
+    """One token per sequence as a view whose token stride is 1, and one sequence whose batch stride is odd."""
+    generator = torch.Generator(device=device).manual_seed(28)
+    draw = lambda *shape: torch.randn(shape, device=device, generator=generator).to(torch.bfloat16)
+    view = lambda x: x.unsqueeze(-1).transpose(2, 3)          # [B, heads, D] -> [B, heads, 1, D]
+    k, v, q = draw(3, 2, dim), draw(3, 2, dim), draw(3, 8, dim)
+    assert view(k).stride(2) == 1
+    got, want = (QuantizedKVCache.allocate(3, 2, 4, dim, device) for _ in range(2))
+    got_q, want_q = (torch.empty((3, 8, 1, dim), device=device, dtype=torch.bfloat16) for _ in range(2))
+    K.kv_cache_write(view(k), view(v), got, q=view(q), q_out=got_q)
+    K.kv_cache_write(k[:, :, None].contiguous(), v[:, :, None].contiguous(), want, q=q[:, :, None].contiguous(), q_out=want_q)
+    assert torch.equal(got_q, want_q) and all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(got, want))
+    assert torch.equal(K.prefix_attention(view(q), got), K.prefix_attention(want_q, got))
+    outs = [view(torch.empty((3, 2, dim), device=device, dtype=torch.bfloat16)) for _ in range(2)]
+    wants = [torch.empty((3, 2, 1, dim), device=device, dtype=torch.bfloat16) for _ in range(2)]
+    for a, b in zip(K.kv_cache_read(got, *outs), K.kv_cache_read(got, *wants)):
+        assert torch.equal(a, b)
+    one = torch.empty(2 * dim, device=device, dtype=torch.bfloat16).as_strided((1, 2, 1, dim), (3, dim, 5, 1))
+    K.kv_cache_read(QuantizedKVCache(*(t[:1].contiguous() for t in got)), one, wants[1][:1])
+    assert torch.equal(one, wants[0][:1])
