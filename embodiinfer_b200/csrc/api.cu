@@ -2,6 +2,7 @@
 // Declarations and per-entry documentation live in include/embodiinfer_b200.h.
 #include "common.cuh"
 
+#include <algorithm>
 #include <cstring>
 
 namespace b2 {
@@ -215,6 +216,20 @@ static bool strides_valid(const int64_t (&stride)[3], int32_t batch, int32_t hea
     return true;
 }
 
+// Whether each stride passes over everything that the shorter ones reach, a row of head_dim elements first.
+static bool rows_apart(const int64_t (&stride)[3], int32_t batch, int32_t heads, int32_t tokens, int32_t head_dim) {
+    const int32_t extents[3] = {batch, heads, tokens};
+    int order[3] = {0, 1, 2};
+    std::sort(order, order + 3, [&](int a, int b) { return stride[a] < stride[b]; });
+    __int128 reach = head_dim;
+    for (const int i : order) {
+        if (extents[i] == 1) continue;
+        if (stride[i] < reach) return false;
+        reach += __int128(extents[i] - 1) * stride[i];
+    }
+    return true;
+}
+
 // What the write and the read of the quantised cache ask of a descriptor alike.
 static int check_kv_cache(const b2_kv_cache_desc* desc) {
     if (desc == nullptr || desc->k == nullptr || desc->v == nullptr || desc->k_codes == nullptr || desc->k_scales == nullptr ||
@@ -250,9 +265,10 @@ int b2_kv_cache_read(const b2_kv_cache_desc* desc, void* stream) {
     const int status = check_kv_cache(desc);
     if (status != B2_OK) return status;
     if (desc->q != nullptr || desc->q_out != nullptr || desc->sine != nullptr || desc->cosine != nullptr) return B2_E_INVALID;
-    const int32_t extents[3] = {desc->batch, desc->kv_heads, desc->tokens};
-    for (int i = 0; i < 3; ++i)          // rows that lie on one another cannot be written
-        if (extents[i] > 1 && (desc->k_stride[i] < desc->head_dim || desc->v_stride[i] < desc->head_dim)) return B2_E_INVALID;
+    // rows that lie on one another cannot be written
+    if (desc->k == desc->v || !rows_apart(desc->k_stride, desc->batch, desc->kv_heads, desc->tokens, desc->head_dim) ||
+        !rows_apart(desc->v_stride, desc->batch, desc->kv_heads, desc->tokens, desc->head_dim))
+        return B2_E_INVALID;
     return b2::launch_kv_cache_read(desc, static_cast<cudaStream_t>(stream));
 }
 

@@ -269,8 +269,8 @@ int b2_rope_axes(const void* positions, int32_t position_bytes, const int32_t* s
  * scale and codes are 0 when max|x| < 2^-50, and the scale is NaN (the whole row reads back as NaN) when max|x| >= 2^40 or a value
  * is not finite.
  * Two tokens of one call that fall on one position (only possible by overlapping sequences' memory) are not ordered.
- * b2_kv_cache_read: writes bf16(code * scale) of position offsets[b] + t to row t of `k`, `v` (any strides of at least head_dim, where
- * there is more than one row along them).  q, q_out, sine and cosine must be NULL.
+ * b2_kv_cache_read: writes bf16(code * scale) of position offsets[b] + t to row t of `k`, `v` (two tensors, any strides that keep
+ * their rows apart: each passes over all that the shorter ones reach).  q, q_out, sine and cosine must be NULL.
  * All pointers 16-byte aligned (scales, offsets and lengths: 4), strides not negative and, where there is more than one row along them,
  * multiples of 8 elements, and
  * batch * tokens * (heads + 2 kv_heads) < 2^31.  The reference has no quantised cache. */

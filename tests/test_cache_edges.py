@@ -7,7 +7,7 @@ import ctypes
 import pytest
 
 from embodiinfer_b200 import _native as N
-from tests.test_kv_cache import _cache_desc
+from tests.test_kv_cache import FAKE, _cache_desc
 
 MOST = (1 << 31) - 1
 
@@ -21,3 +21,16 @@ def test_strides_count_only_where_there_are_steps(changes):
     for call in (N.load().b2_kv_cache_write, N.load().b2_kv_cache_read):
         assert call(ctypes.byref(_cache_desc(**changes)), None) == N.E_TOO_LARGE
         assert call(ctypes.byref(_cache_desc(**grown)), None) == N.E_INVALID
+
+
+@pytest.mark.parametrize("k_stride,v_stride,extents", [
+    ((128, 128, 128), (768, 384, 128), (2, 2, 3)), ((768, 384, 128), (256, 384, 128), (2, 2, 3)),          # steps that fall on other rows
+    ((768, 128, 128), (768, 384, 128), (2, 2, 3)), ((0, 0, 0), (0, 0, 0), (2, 1, 1)), ((384, 256, 128), (384, 256, 128), (1, 2, 3))])
+def test_read_refuses_rows_on_one_another(k_stride, v_stride, extents):
+    batch, kv_heads, tokens = extents
+    fields = dict(batch=batch, kv_heads=kv_heads, tokens=tokens, v=2 * FAKE)
+    assert N.load().b2_kv_cache_read(ctypes.byref(_cache_desc(k_stride=k_stride, v_stride=v_stride, **fields)), None) == N.E_INVALID
+
+
+def test_read_refuses_one_tensor_for_both():
+    assert N.load().b2_kv_cache_read(ctypes.byref(_cache_desc(k_stride=(384, 384, 128), v_stride=(384, 384, 128), v=FAKE)), None) == N.E_INVALID
