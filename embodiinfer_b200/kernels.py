@@ -454,8 +454,11 @@ def prefix_attention(q: torch.Tensor, prefix, own=None, *, members: torch.Tensor
         raise ValueError("attention output must be a contiguous bf16 tensor of the queries' shape")
     if not (batch and heads and queries and head_dim):
         return out
-    if prefix_capacity == 0 and own_capacity == 0:
-        return out.zero_()
+    if prefix_capacity == 0 and own_capacity == 0:          # nothing to see: zeros, for what the groups hold
+        if members is None:
+            return out.zero_()
+        index = torch.arange(batch, device=device)
+        return out.masked_fill_(((index >= members[0]) & (index < members[-1])).view(batch, 1, 1, 1), 0.0)
     if status is None:
         status = status_word(device)
     pointers = (q.data_ptr(), out.data_ptr(), *prefix_pointers, *own_pointers, _address(members), _address(prefix_lengths),

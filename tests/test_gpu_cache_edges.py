@@ -243,3 +243,12 @@ def test_any_stride_along_an_extent_of_one(device, dim):
     one = torch.empty(2 * dim, device=device, dtype=torch.bfloat16).as_strided((1, 2, 1, dim), (3, dim, 5, 1))
     K.kv_cache_read(QuantizedKVCache(*(t[:1].contiguous() for t in got)), one, wants[1][:1])
     assert torch.equal(one, wants[0][:1])
+
+
+def test_no_keys_at_all_and_members_of_no_group(device):
+    q = torch.randn((5, 8, 2, 128), device=device).to(torch.bfloat16)
+    empty = tuple(torch.empty((2, 1, 0, 128), device=device, dtype=torch.bfloat16) for _ in range(2))
+    out = torch.full_like(q, 7.0)
+    assert K.prefix_attention(q, empty, members=whole([1, 2, 4], device), out=out) is out
+    assert not out[1:4].any() and (out[[0, 4]] == 7.0).all()
+    assert not K.prefix_attention(q, tuple(t[:1] for t in empty), out=out).any()
