@@ -635,6 +635,8 @@ class Pi05ShapedPolicy(nn.Module):
         ``quantised_cache`` holds the prefixes' and the samples' keys and values as e4m3 codes with a scale for each row
         (``b2_kv_cache_write``), half the memory of the one bf16 copy, always shared."""
         batch, samples = noise.shape[:2]
+        if noise.shape[2:] != (ACTION_HORIZON, ACTION_DIM) or any(part.shape[0] != batch for pair in cache for part in pair):
+            raise ValueError(f"denoise_samples requires noise [B, N, {ACTION_HORIZON}, {ACTION_DIM}] for the cache's B observations")
         count, device, head_dim = batch * samples, self.device_, GEMMA_300M.head_dim
         actions = noise.reshape(count, ACTION_HORIZON, ACTION_DIM)
         if count == 0:
@@ -677,6 +679,8 @@ class Pi05ShapedPolicy(nn.Module):
         """``samples`` action chunks [B, samples, 10, 32] of every observation, for a caller that chooses among them: the vision
         and prefix towers run once per observation (see ``denoise_samples`` for what the samples share)."""
         images, tokens = observations["images"], observations["tokens"]
+        if noise is not None and noise.shape[:2] != (images.shape[0], samples):
+            raise ValueError("sample requires noise [B, samples, ...] of the observations' B")
         cache, prefix_length = self.encode_prefix(images, tokens)
         if noise is None:
             noise = self.noise(images.shape[0] * samples).view(images.shape[0], samples, ACTION_HORIZON, ACTION_DIM)

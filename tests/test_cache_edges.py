@@ -3,10 +3,13 @@
 from __future__ import annotations
 
 import ctypes
+from types import SimpleNamespace
 
 import pytest
+import torch
 
 from embodiinfer_b200 import _native as N
+from embodiinfer_b200.pi05_shaped import ACTION_DIM, ACTION_HORIZON, Pi05ShapedPolicy
 from tests.test_kv_cache import FAKE, _cache_desc
 
 MOST = (1 << 31) - 1
@@ -34,3 +37,16 @@ def test_read_refuses_rows_on_one_another(k_stride, v_stride, extents):
 
 def test_read_refuses_one_tensor_for_both():
     assert N.load().b2_kv_cache_read(ctypes.byref(_cache_desc(k_stride=(384, 384, 128), v_stride=(384, 384, 128), v=FAKE)), None) == N.E_INVALID
+
+
+@pytest.mark.parametrize("options", [dict(), dict(shared_prefix=True), dict(quantised_cache=True)])
+def test_samples_refuse_noise_of_other_observations(options):
+    """Noise for four observations behind the cache of two would hand every prefix to other observations' samples."""
+    policy = SimpleNamespace(expert=[None], device_=torch.device("cpu"))          # refused before anything of it is used
+    cache = [tuple(torch.zeros((2, 1, 12, 256), dtype=torch.bfloat16) for _ in range(2))]
+    for shape in ((4, 3, ACTION_HORIZON, ACTION_DIM), (1, 3, ACTION_HORIZON, ACTION_DIM), (2, 3, ACTION_DIM, ACTION_HORIZON)):
+        with pytest.raises(ValueError, match="noise"):
+            Pi05ShapedPolicy.denoise_samples(policy, cache, 12, torch.zeros(shape), **options)
+    observations = dict(images=torch.zeros((2, 1)), tokens=torch.zeros((2, 1)))
+    with pytest.raises(ValueError, match="noise"):
+        Pi05ShapedPolicy.sample(policy, observations, 3, torch.zeros((2, 4, ACTION_HORIZON, ACTION_DIM)), **options)
