@@ -600,18 +600,23 @@ class Pi05ShapedPolicy(nn.Module):
             cached = self.schedules[batch] = tuple(rows)
         return cached
 
-    def denoise(self, cache, prefix_length: int, noise: torch.Tensor) -> torch.Tensor:
+    def denoise(self, cache, prefix_length: int, noise: torch.Tensor, samples: int = 1) -> torch.Tensor:
         """``noise`` [B, 10, 32] fp32 ~ N(0, 1): ten Euler steps of the flow from t = 1 to t = 0.  The flow time reaches
-        the expert only through its AdaRMS norms."""
+        the expert only through its AdaRMS norms.  ``samples`` chunks in a row belong to one entry of ``cache`` and get a copy of
+        its keys and values each."""
         actions = noise
         rope = rope_tables(prefix_length + torch.arange(ACTION_HORIZON, device=self.device_), GEMMA_300M.head_dim)
         dt = -1.0 / DENOISE_STEPS
         schedule = self.modulation_schedule(noise.shape[0])
-        # one key/value buffer per layer: the prefix rows are written once, the action rows every step
-        buffers = []
-        for keys, values in cache[: len(self.expert)]:
-            pad = keys.new_zeros((*keys.shape[:2], ACTION_HORIZON, keys.shape[-1]))
-            buffers.append((torch.cat((keys, pad), dim=2), torch.cat((values, pad), dim=2)))
+        # one key/value buffer per layer: the prefix rows are written once (straight to their place: the copies are the call's largest
+        # memory), the action rows every step
+        def buffer(part):
+            rows = part.new_empty((part.shape[0], samples, part.shape[1], part.shape[2] + ACTION_HORIZON, part.shape[3]))
+            rows[..., : part.shape[2], :] = part.unsqueeze(1)
+            rows[..., part.shape[2]:, :] = 0.0
+            return rows.flatten(0, 1)
+
+        buffers = [tuple(buffer(part) for part in pair) for pair in cache[: len(self.expert)]]
         for step in range(DENOISE_STEPS):
             actions = actions + dt * self._velocity(actions, rope, schedule[step], [dict(kv_buffers=kv) for kv in buffers])
         return actions
@@ -644,8 +649,7 @@ class Pi05ShapedPolicy(nn.Module):
         if shared_prefix is None:
             shared_prefix = count > 64
         if not (shared_prefix or quantised_cache):
-            copies = [tuple(part.repeat_interleave(samples, 0) for part in pair) for pair in cache[: len(self.expert)]]
-            return self.denoise(copies, prefix_length, actions).view(noise.shape)
+            return self.denoise(cache, prefix_length, actions, samples).view(noise.shape)
         positions = prefix_length + torch.arange(ACTION_HORIZON, device=device)
         rope = K.rope_axes(positions[None], (head_dim // 2,))
         schedule = self.modulation_schedule(count)
