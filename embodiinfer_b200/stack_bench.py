@@ -71,18 +71,17 @@ def measure_denoise(policy: Pi05ShapedPolicy, batches=(1, 8, 64), seed: int = 10
 
 
 @torch.no_grad()
-def measure_samples(policy: Pi05ShapedPolicy, observations: int = 8, samples: int = 8, seed: int = 1006) -> dict[str, float]:
-    """Milliseconds of the 10-step denoise of ``samples`` action chunks for each of ``observations`` prefixes of 560 tokens: over
-    one copy of the prefix per observation (bf16 and quantised caches), and over one copy per sample."""
+def measure_samples(policy: Pi05ShapedPolicy, observations: int = 8, samples: int = 8, seed: int = 1006, prefix: int = PREFIX_TOKENS) -> dict[str, float]:
+    """Milliseconds of the 10-step denoise of ``samples`` action chunks for each of ``observations`` prefixes of ``prefix`` tokens: over
+    one copy of the prefix per observation (bf16 and quantised caches), and over one copy per sample, made by the call."""
     device = policy.device_
     generator = torch.Generator(device=device).manual_seed(seed)
-    cache = [tuple(torch.randn((observations, 1, PREFIX_TOKENS, GEMMA_300M.head_dim), device=device, generator=generator).to(torch.bfloat16)
+    cache = [tuple(torch.randn((observations, 1, prefix, GEMMA_300M.head_dim), device=device, generator=generator).to(torch.bfloat16)
                    for _ in range(2)) for _ in policy.expert]
     noise = torch.randn((observations, samples, ACTION_HORIZON, ACTION_DIM), device=device, generator=generator)
-    repeated = [tuple(part.repeat_interleave(samples, 0) for part in pair) for pair in cache]
-    return {"shared": graph_milliseconds(lambda: policy.denoise_samples(cache, PREFIX_TOKENS, noise, shared_prefix=True)),
-            "shared_quantised": graph_milliseconds(lambda: policy.denoise_samples(cache, PREFIX_TOKENS, noise, quantised_cache=True)),
-            "a_copy_per_sample": graph_milliseconds(lambda: policy.denoise(repeated, PREFIX_TOKENS, noise.flatten(0, 1)))}
+    return {"shared": graph_milliseconds(lambda: policy.denoise_samples(cache, prefix, noise, shared_prefix=True)),
+            "shared_quantised": graph_milliseconds(lambda: policy.denoise_samples(cache, prefix, noise, quantised_cache=True)),
+            "a_copy_per_sample": graph_milliseconds(lambda: policy.denoise_samples(cache, prefix, noise, shared_prefix=False))}
 
 
 @torch.no_grad()
