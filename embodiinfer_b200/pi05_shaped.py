@@ -51,6 +51,13 @@ GEMMA_300M = TowerShape(1024, 4096, 18, 8, 1, 256)
 SIGLIP_SO400M = TowerShape(1152, 4304, 27, 16, 16, 72)
 IMAGE_SIZE, PATCH, CAMERAS, TEXT_TOKENS, VOCAB = 224, 14, 2, 48, 257152
 ACTION_HORIZON, ACTION_DIM, DENOISE_STEPS = 10, 32, 10
+# From so many rows on (chunks x prefix tokens, 25 MB a layer) samples read one prefix instead of a copy each.  Below, the attention is a chain
+# of short launches that b2_attention has less of; above, making and reading the copies costs more.  Ten FP8 steps, ms shared / copied:
+#   136 tokens   64 chunks 13.0 / 12.4   128 chunks 14.9 / 14.9-15.3   256 chunks 22.9 / 23.2
+#   560           8  9.5 /  8.2   32 12.6 / 11.9   48 12.9 / 12.9   64 13.6 / 13.8   128 15.5 / 18.5   256 24.3 / 28.6
+#   1072         16 12.2 / 11.8   32 12.5 / 12.8   64 14.6 / 16.1   128 16.6 / 21.7
+#   2096          8  9.9 /  9.1   16 12.7 / 12.9   32 13.0 / 14.9   64 15.0 / 19.2
+SHARED_PREFIX_ROWS = 24576
 
 
 def _random_linear(out_features: int, in_features: int, generator: torch.Generator, device, bias: bool = False) -> nn.Linear:
@@ -634,9 +641,8 @@ class Pi05ShapedPolicy(nn.Module):
                         shared_prefix: bool | None = None) -> torch.Tensor:
         """Several action chunks of every observation: ``noise`` [B, N, 10, 32] fp32, one starting point per sample, to
         [B, N, 10, 32].  ``cache`` is ``encode_prefix``'s for the B observations: the N samples of an observation read its one
-        prefix (``b2_prefix_attention``).  ``shared_prefix=False`` gives every sample a copy (``denoise``); by default calls of
-        at most 64 chunks do, whose attention is a chain of short launches that ``b2_attention`` has less of (ten steps over 560
-        tokens: 8 / 64 / 128 / 256 chunks take 8.1 / 13.4 / 17.5 / 27.0 ms with copies, 9.6 / 13.6 / 15.5 / 24.3 without).
+        prefix (``b2_prefix_attention``).  ``shared_prefix=False`` gives every sample a copy (``denoise``); by default calls that
+        copy fewer than ``SHARED_PREFIX_ROWS`` rows do.
         ``quantised_cache`` holds the prefixes' and the samples' keys and values as e4m3 codes with a scale for each row
         (``b2_kv_cache_write``), half the memory of the one bf16 copy, always shared."""
         batch, samples = noise.shape[:2]
@@ -647,7 +653,7 @@ class Pi05ShapedPolicy(nn.Module):
         if count == 0:
             return noise.clone()
         if shared_prefix is None:
-            shared_prefix = count > 64
+            shared_prefix = count * cache[0][0].shape[2] >= SHARED_PREFIX_ROWS
         if not (shared_prefix or quantised_cache):
             return self.denoise(cache, prefix_length, actions, samples).view(noise.shape)
         positions = prefix_length + torch.arange(ACTION_HORIZON, device=device)

@@ -39,3 +39,12 @@ def test_one_copy_of_the_prefix_per_sample(policy):
     assert buffers > 128 << 20 and torch.cuda.max_memory_allocated() - before < buffers + (64 << 20)
     repeated = [tuple(part.repeat_interleave(12, 0) for part in pair) for pair in cache]
     assert torch.equal(got, policy.denoise(repeated, length, noise.flatten(0, 1)).view(noise.shape))
+
+
+@torch.no_grad()
+@pytest.mark.parametrize("observations,samples,prefix,shared", [(3, 16, 560, True), (3, 14, 560, False), (9, 8, 136, False), (1, 4, 6200, True)])
+def test_the_default_goes_by_the_rows_that_copies_would_hold(policy, observations, samples, prefix, shared):
+    cache, length, noise = random_call(policy, observations, samples, prefix, 2)
+    got = policy.denoise_samples(cache, length, noise)
+    assert torch.equal(got, policy.denoise_samples(cache, length, noise, shared_prefix=shared))
+    assert not torch.equal(got, policy.denoise_samples(cache, length, noise, shared_prefix=not shared))
