@@ -615,15 +615,19 @@ class Pi05ShapedPolicy(nn.Module):
         rope = rope_tables(prefix_length + torch.arange(ACTION_HORIZON, device=self.device_), GEMMA_300M.head_dim)
         dt = -1.0 / DENOISE_STEPS
         schedule = self.modulation_schedule(noise.shape[0])
-        # one key/value buffer per layer: the prefix rows are written once (straight to their place: the copies are the call's largest
-        # memory), the action rows every step
-        def buffer(part):
-            rows = part.new_empty((part.shape[0], samples, part.shape[1], part.shape[2] + ACTION_HORIZON, part.shape[3]))
-            rows[..., : part.shape[2], :] = part.unsqueeze(1)
-            rows[..., part.shape[2]:, :] = 0.0
-            return rows.flatten(0, 1)
-
-        buffers = [tuple(buffer(part) for part in pair) for pair in cache[: len(self.expert)]]
+        # one key/value buffer per layer: the prefix rows are written once, the action rows every step
+        buffers = []
+        for keys, values in cache[: len(self.expert)]:
+            if samples == 1:          # 64 chunks over 560 tokens: 13.4 ms, by assignment as below 13.9
+                pad = keys.new_zeros((*keys.shape[:2], ACTION_HORIZON, keys.shape[-1]))
+                buffers.append((torch.cat((keys, pad), dim=2), torch.cat((values, pad), dim=2)))
+                continue
+            # straight to their place: the copies are the call's largest memory
+            pair = tuple(keys.new_empty((keys.shape[0], samples, keys.shape[1], keys.shape[2] + ACTION_HORIZON, keys.shape[3])) for _ in range(2))
+            for rows, part in zip(pair, (keys, values)):
+                rows[..., : part.shape[2], :] = part.unsqueeze(1)
+                rows[..., part.shape[2]:, :] = 0.0
+            buffers.append(tuple(rows.flatten(0, 1) for rows in pair))
         for step in range(DENOISE_STEPS):
             actions = actions + dt * self._velocity(actions, rope, schedule[step], [dict(kv_buffers=kv) for kv in buffers])
         return actions
