@@ -6,10 +6,11 @@
 //   sine[t, i] = sin(position[a(i), t] f_i), cosine likewise, fp32
 //
 // Angles are counted in turns and in whole numbers: a frequency is held as the fraction of f / 2 pi in 64 bits (2^64 = one turn), and
-// position * fraction modulo 2^64 is the angle's fraction of a turn with nothing lost, however far the position (a video's
-// 2.6e5th frame at f = 1 has no fraction left in fp32).  The top bits name the quadrant, the rest, in [-1/8, 1/8) turns, goes to fp32
-// (an error of 2^-28 turns, 2.3e-8) and into the Taylor series of sine (to the 9th power) and cosine (to the 10th), both at
-// once on the packed fp32 pipe.  Frequencies are formed in fp64, to a few 2^-53 of themselves.
+// position * fraction modulo 2^64 is the angle's fraction of a turn.  The product loses nothing, however far the position (a video's
+// 2.6e5th frame at f = 1 has no fraction left in fp32); the error is the position times the frequency's own, which is formed in
+// fp64 to a few 2^-53 of itself: at most some 2^-30 of a turn at position 2^20, 2^-10 at 2^40.  The top bits name the quadrant, the rest, in
+// [-1/8, 1/8) turns, goes to fp32 (an error of 2^-28 turns, 2.3e-8) and into the Taylor series of sine (to the 9th power) and cosine
+// (to the 10th), both at once on the packed fp32 pipe.
 //
 // Each thread keeps the frequencies of VECTOR neighbouring columns and walks down the tokens: one 16-byte store per table
 // and token.  Measured (B200): 8 x 16384 positions, head dimension 128, 14.9 us (70 MB, 4.7 TB/s), bound by the stores: without the

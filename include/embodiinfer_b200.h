@@ -250,8 +250,8 @@ int b2_attention_nvfp4(const void* q, const void* k, const void* v, void* codes,
  *   sections   HOST int32[axes]: how many of the head_dim / 2 frequencies belong to each axis, in order; their sum is head_dim / 2
  *   sine, cosine  fp32 [tokens, head_dim / 2]:  sin / cos(positions[a(i), t] * f_i)
  * f_i = theta^(-i / (head_dim / 2)), one spectrum dealt to the axes; with B2_ROPE_OWN_SPECTRUM every axis has its own,
- * f = theta^(-j / sections[a]) with j counted inside the section.  The angle is formed in 64 bits, so far positions keep their
- * fraction of a turn.  1 to 4 axes, head_dim even and at most 1024, theta of [1e-300, 1e300].  No reference counterpart on this path
+ * f = theta^(-j / sections[a]) with j counted inside the section.  The angle is formed in 64 bits: far positions keep their
+ * fraction of a turn, to the position times a few 2^-53 of f_i.  1 to 4 axes, head_dim even and at most 1024, theta of [1e-300, 1e300].  No reference counterpart on this path
  * (its towers build one-axis tables with torch). */
 #define B2_ROPE_OWN_SPECTRUM 1
 int b2_rope_axes(const void* positions, int32_t position_bytes, const int32_t* sections, int32_t axes, int64_t tokens,

@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import math
+from decimal import Decimal, localcontext
 
 import pytest
 import torch
@@ -252,3 +253,37 @@ def test_no_keys_at_all_and_members_of_no_group(device):
     assert K.prefix_attention(q, empty, members=whole([1, 2, 4], device), out=out) is out
     assert not out[1:4].any() and (out[[0, 4]] == 7.0).all()
     assert not K.prefix_attention(q, tuple(t[:1] for t in empty), out=out).any()
+
+
+# ---- rotary tables ----------------------------------------------------------------------------------------
+
+PI = Decimal("3.14159265358979323846264338327950288419716939937510582097494459230781640628620899")
+# The series, for the fraction r of a turn in [-1/8, 1/8]: r rounded to fp32 2 pi 2^-28; what the series leave out, (pi/4)^11 / 11!; of the
+# sine's sum the last step (near 2 pi, times 1/8), its constant and the step before (near 41, times 1/64 and 1/8) 2^-25 + 2^-25 + 2 * 2^-28;
+# the product 2^-25.  The cosine's are smaller.
+SERIES = 2 * math.pi * 2.0 ** -28 + (math.pi / 4) ** 11 / 39916800 + 3 * 2.0 ** -25 + 2 * 2.0 ** -28
+
+
+@pytest.mark.parametrize("sections,theta,own_spectrum", [((64,), 500000.0, False), ((6,), 10000.0, True), ((5, 2), 10000.0, True)])
+def test_tables_of_far_positions(device, sections, theta, own_spectrum):
+    """Against angles reduced in 70 decimal digits.  A frequency f is known to some 2^-53 of itself -- theta's logarithm and its division and
+    product 3 log2(theta) 2^-53 ln 2, the exponential 2^-52, the constant and its product 2^-53 each, three steps of 2^-52 (with the ratio's
+    own 3 times that) to the last of four columns -- and to 2^-65 turns; the position multiplies both."""
+    positions = [0, 1, -1, 262143, 2 ** 31 - 1, -2 ** 31, 2 ** 36 + 12345, -(2 ** 33), (1 << 40) + 3]
+    sine, cosine = K.rope_axes(torch.tensor([positions] * len(sections), device=device), sections, theta=theta, own_spectrum=own_spectrum)
+    sine, cosine = sine.cpu().double(), cosine.cpu().double()
+    relative = (3 * math.log2(theta) * math.log(2) + 2 + 2 + 3 * 2 * 4) * 2.0 ** -53
+    column = 0
+    for count in sections:
+        for j in range(count):
+            with localcontext() as context:
+                context.prec = 70
+                power = Decimal(j) / count if own_spectrum else Decimal(column) / sum(sections)
+                frequency = (-power * Decimal(theta).ln()).exp()
+                for t, position in enumerate(positions):
+                    turns = position * frequency / (2 * PI)
+                    angle = float(2 * PI * (turns - turns.to_integral_value()))
+                    bound = SERIES + abs(position) * (float(frequency) * relative + 2 * math.pi * 2.0 ** -65)
+                    assert abs(float(sine[t, column]) - math.sin(angle)) <= bound, (column, position)
+                    assert abs(float(cosine[t, column]) - math.cos(angle)) <= bound, (column, position)
+            column += 1
