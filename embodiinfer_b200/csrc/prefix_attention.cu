@@ -1090,6 +1090,16 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
                 constexpr bool PLAIN = decltype(tag)::value;
 #pragma unroll 1
                 for (int first = thread; first < PA_KEYS * PIECES; first += BATCH * 32 * Shape::VALUE_TEAM) {
+                    if (!PLAIN && (first - thread) / PIECES >= valid) {          // behind the end, all of the batch: no code to look at
+#pragma unroll
+                        for (int n = 0; n < BATCH; ++n) {
+                            const uint32_t i = first + n * 32 * Shape::VALUE_TEAM, key = i / PIECES, piece = i % PIECES, left = (piece & 3u) * 2u;
+                            const uint32_t group = values_smem + c * Shape::VALUE_BYTES + (piece >> 2) * Shape::KV_ATOM_BYTES + key * 128u;
+                            sts_u4(group + ((left ^ (key & 7u)) << 4), 0u, 0u, 0u, 0u);
+                            sts_u4(group + (((left + 1u) ^ (key & 7u)) << 4), 0u, 0u, 0u, 0u);
+                        }
+                        continue;
+                    }
                     uint4 codes[BATCH];
                     uint32_t scale_bits[BATCH];
 #pragma unroll
