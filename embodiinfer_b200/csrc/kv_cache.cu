@@ -14,8 +14,9 @@
 //
 // Both kernels move bytes: 16-byte loads, a row dealt to head_dim / 16 lanes (a lane holds 8 values of the first half and the
 // 8 values they rotate with), the row maximum by shuffles inside those lanes, no shared memory.
-// Measured (B200): 16 prompts of 500 to 1000 tokens, 32 query and 8 key/value heads of 128, written in 58 us (285 MB, 4.9 TB/s): bound by
-// the issue of its arithmetic -- the rotation's separate roundings, row maxima, exact division -- at 31 % occupancy (80 registers: four
+// Measured (B200): 16 prompts of 500 to 1000 tokens, 32 query and 8 key/value heads of 128, written in 58 us (285 MB, 4.9 TB/s).  Neither
+// memory (46 % of DRAM's rate over the launch) nor issue (61 % of the slots: the rotation's separate roundings, row maxima, exact division)
+// is full: 20 warps per SM, 8 cycles from one instruction of a warp to its next.  More of them cost more than they give (80 registers: four
 // rows per thread share their factors; two rows per thread 68 us, 64 registers 66).  8 x 8 x 8192 rows of 128 read in 63 us (406 MB,
 // 6.5 TB/s: copy speed; with two 16-byte stores for each 32 bytes 72).  The few tokens of a decoding step take 2.8 us either way.
 #include "common.cuh"

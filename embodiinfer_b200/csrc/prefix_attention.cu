@@ -6,8 +6,9 @@
 //
 // A group's members, the query heads of one key/value head and the queries are one matrix of rows (row = member, head, query):
 // a CTA takes 128 of them and walks the prefix in tiles of 64 keys -- every key tile is loaded once for all 128 rows -- and then
-// the own keys of the members its rows belong to, where the rows of the other members are masked.  The own part so spends tensor
-// instructions on masked rows; it stays below the time of loading those keys, which nobody else needs.
+// the own keys of the members its rows belong to, where the rows of the other members are masked.  An own key tile so costs as much as a
+// prefix tile, whatever part of the 128 rows sees it: 2 of a row tile's 11 key tiles for ten-query chunks, 151 of 663 for single tokens behind
+// 32768 keys with 4 rows and up to 512 own keys per member.
 //   warps 0-7     two softmax groups of 128 threads, one thread per row, for the even and the odd key tiles: queries into tensor memory,
 //                 scores, reference and sum, probabilities, output
 //   warp 8        which rows and keys; TMA producer: key and value tiles through rings
@@ -22,13 +23,15 @@
 // needs from the other only after it has the maximum of its own tile.  Every wait is bounded and reports through the status word.
 //
 // Measured (B200; a tile is 64 keys for 128 rows, whose products alone are 500 cycles at D = 128 and 1000 at D = 256):
-//   fifty-query chunks of 64 members over 4 x 8192 bf16 keys, D = 256: 187 us (1150 TFLOP/s), 1430 cycles per tile
-//   64 members, one query, 32768 quantised keys, D = 128: 80 us, 1370 cycles per tile; of an earlier 83 without its exponentials 74,
+//   fifty-query chunks of 64 members over 4 x 8192 bf16 keys, D = 256: 188 us (1150 TFLOP/s), 1430 cycles per tile
+//   64 members, one query, 32768 quantised keys, D = 128: 79 us, 1350 cycles per tile; of an earlier 83 without its exponentials 74,
 //   without its products 78, without the conversion of values 74: the chain of a softmax group -- scores out, maximum, exponentials, P in, each with
 //   its latency and two warps per scheduler to hide it -- and not one unit is what bounds the loop
-//   256 ten-query chunks over 32 x 712 quantised keys, D = 256: 41 us (in the groups' order 44): 176 row tiles of 12 key tiles on 148
+//   256 ten-query chunks over 32 x 712 quantised keys, D = 256: 42 us (in the groups' order 44): 176 row tiles of 12 key tiles on 148
 //   SMs, 21 k of a CTA's 41 k cycles before and behind the loop (4.8 k look-up, 3.6 k splitting Q, 5 k output)
-//   four ten-query chunks over 560 bf16 keys, D = 256: 13.6 us, 9 in this kernel for two tiles per CTA, the rest the join
+//   four ten-query chunks over 560 bf16 keys, D = 256: 13.6 us, 9 in this kernel for two tiles per CTA, the rest the join (b2_attention, one cluster
+//   launch over a copy of the keys for each chunk: 8.0 us)
+// The quantised D = 128 kernel spills 40 bytes per thread, the others 12.
 //
 // bf16 cache.  K and V are read as they lie in memory.  What the tensor core must not see is taken out of the value tile in
 // shared memory, because a probability of zero times an infinity or a NaN is not zero: rows behind the end of a segment are set to
@@ -414,7 +417,8 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
         };
         constexpr int MANY = 1 << 29;          // bounds that run backwards may add up to anything: enough for every CTA
         int total_tiles = 0;
-        // More row tiles than SMs: the longest prefixes first, so that the last wave is made of short ones (as far as a warp sees all groups).
+        // More row tiles than SMs: the longest prefixes first, so that the last wave is made of short ones (as far as a warp sees all groups: up
+        // to 32 of them; more are taken in their own order).
         const bool sorted = args.prefix_lengths != nullptr && args.groups <= 32 && int(gridDim.x) > args.sms;
         int group_at = lane;          // sorted: the group at this place
         if (sorted) {

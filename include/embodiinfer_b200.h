@@ -268,7 +268,8 @@ int b2_rope_axes(const void* positions, int32_t position_bytes, const int32_t* s
  *   scale = max|x| / 448,  code = e4m3(x / scale), both in fp32 from the fp32 rotation
  * scale and codes are 0 when max|x| < 2^-50, and the scale is NaN (the whole row reads back as NaN) when max|x| >= 2^40 or a value
  * is not finite.
- * Two tokens of one call that fall on one position (only possible by overlapping sequences' memory) are not ordered.
+ * Two tokens of one call that fall on one position (only possible by overlapping sequences' memory) are not ordered.  `q_out` overlaps no
+ * operand.
  * b2_kv_cache_read: writes bf16(code * scale) of position offsets[b] + t to row t of `k`, `v` (two tensors, any strides that keep
  * their rows apart: each passes over all that the shorter ones reach).  q, q_out, sine and cosine must be NULL.
  * All pointers 16-byte aligned (scales, offsets and lengths: 4), strides not negative and, where there is more than one row along them,
@@ -315,7 +316,9 @@ int b2_kv_cache_read(const b2_kv_cache_desc* desc, void* stream);
  * and 2^-22 of the largest in its 64 keys).  head_dim 128 or 256.
  * `workspace`: NULL, or 32-byte aligned device scratch; with b2_prefix_attention_workspace_bytes(desc) bytes the 128-row tiles that
  * do not fill the device (a small call's, or those of the last partial wave) have their keys cut across the SMs and the parts joined
- * in a fixed order.  It needs no zeroing and holds nothing between calls, but two calls that may run at the same time need one each.  `status` as in b2_linear_desc.
+ * in a fixed order.  It needs no zeroing and holds nothing between calls, but two calls that may run at the same time need one each.
+ * Row tiles of up to 32 groups with prefix_lengths are taken longest prefix first, those of more groups in the groups' order.  `out` overlaps
+ * no operand.  `status` as in b2_linear_desc.
  * Widens b2_attention (one copy of the keys per batch element, head_dim 256, one key/value head, no lengths); the reference
  * attends per sample (embodiinfer/backend/torch/attention.py:97-106). */
 #define B2_ATTENTION_CAUSAL 1
