@@ -41,8 +41,8 @@
 // Quantised cache (e4m3 codes, one fp32 scale per row: ks for keys, vs for values).
 //   Scores.  The codes go to the tensor core as they are (kind::f8f6f4).  Q is split into two e4m3 operands, q 2^e = hi + lo with
 //   2^e bringing the row's largest value into [128, 256): a bf16 value has 8 significant bits, hi takes 4 and lo the rest,
-//   exactly, down to 2^-17 of the row's largest value (of 2^-119 in a row of smaller ones).  Two products at twice the bf16 rate cost what one bf16 product
-//   would, and no key is ever converted.  ks multiplies the score.
+//   exactly, down to 2^-17 of the row's largest value (of 2^-119 in a row of smaller ones).  Two products at twice the bf16 rate cost what one
+//   bf16 product would, and no key is ever converted.  ks multiplies the score.
 //   Output.  The four value warps, two teams a tile apart, turn the codes into f16, exactly, and multiply by vs 2^-E: one rounding of 2^-11 for the scale and
 //   one for the product, beside the 2^-8 of the result.  2^E is the unit of the accumulator, the same for all rows: it follows the
 //   largest vs of a key tile when that leaves [2^-3, 2^6) units (2^-48 is the smallest), and the accumulator is rescaled then as it is for a
@@ -1191,9 +1191,9 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k_map, const 
                 }
                 largest = __reduce_max_sync(0xffffffffu, largest);
                 // the unit 2^E: kept unless the tile's largest scale is outside [2^-3, 2^6) of it (a tile of zeros fits any).  It may fall by any
-                // step: the limit below is what keeps the accumulator, which grows by the step, in fp32's range -- values below 2^40 with weights
-                // of at most 2^15 are below 2^103 of the smallest unit, times the number of keys (2^24 of them, all at both ends).  Scales from 2^-59 on are still 2^-11 of
-                // it, normal numbers of f16.
+                // step, by which the accumulator grows; the smallest unit keeps that in fp32's range: values below 2^40 with weights of at most
+                // 2^15 are below 2^103 units, and 2^24 keys of them below 2^127.  Scales from 2^-59 on are still 2^-11 of the smallest unit,
+                // normal numbers of f16.
                 const int exponent = int(largest >> 23) - 127, relative = exponent - unit_exponent;
                 int change = 0;
                 if (largest != 0u && (j == 0 || relative > 5 || relative < -3)) {
